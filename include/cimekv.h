@@ -235,6 +235,52 @@ int cimekv_backward_noalloc(const float* x, const float* wpos, const float* wneg
                             float* grad_x, float* grad_wpos, float* grad_wneg, void* stream);
 
 /*
+ * Element types of the entry points below that take tensors of several types
+ * (void* with a type argument).
+ */
+enum { CIMEKV_F32 = 0, CIMEKV_BF16 = 1, CIMEKV_F16 = 2 };
+
+/* Widest row the layer norm kernels hold. */
+#define CIMEKV_LAYER_NORM_MAX_COLS 16384
+
+/*
+ * Layer normalisation of `rows` rows of `cols` elements, optionally of the sum
+ * with a residual branch (the digital part of a transformer block around the
+ * CIM layers; nn.LayerNorm and `x + attention(...)` in the reference,
+ * src/isa/language/models.py:81-136):
+ *   h = x + delta, rounded to x's type      (delta and h both given, or both NULL: h = x)
+ *   y = (h - mean) * rstd * weight + bias,  rstd = (var + eps)^-1/2
+ * x and delta have rows of contiguous elements `*_stride` elements apart (0
+ * repeats a row); h and y are contiguous.  weight and bias [cols] share w_type,
+ * either may be NULL.  mean and rstd [rows] are kept for the backward (both may
+ * be NULL).  Outputs must not overlap inputs.
+ */
+int cimekv_layer_norm_forward(const void* x, int x_type, long long x_stride,
+                              const void* delta, int delta_type, long long delta_stride,
+                              const void* weight, const void* bias, int w_type,
+                              long long rows, int cols, float eps,
+                              void* h, void* y, int y_type, float* mean, float* rstd, void* stream);
+
+/* Workspace bytes of cimekv_layer_norm_backward on the current device. */
+size_t cimekv_layer_norm_workspace_bytes(long long rows, int cols);
+
+/*
+ * Backward of cimekv_layer_norm_forward.  dy is the gradient of y, dh (may be
+ * NULL) that of the sum, in h's type; h is the sum (x itself without a branch).
+ *   dx     = rstd (dy w - mean(dy w) - u mean(dy w u)) + dh,  u = (h - mean) rstd
+ *   ddelta = the same values in delta's type
+ *   dw     = sum over rows of dy u,  db = sum over rows of dy   (w_type; zero for no rows)
+ * Each of dx, ddelta, dw and db may be NULL.  workspace (16-byte aligned) is
+ * needed when dw or db is given.  The result is deterministic.
+ */
+int cimekv_layer_norm_backward(const void* dy, int y_type, long long dy_stride,
+                               const void* dh, long long dh_stride,
+                               const void* h, int x_type, long long h_stride,
+                               const void* weight, int w_type, const float* mean, const float* rstd,
+                               long long rows, int cols, void* dx, void* ddelta, int delta_type,
+                               void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Debug support, no counterpart in the reference.  cimekv_debug_build()
  * returns 1 for the library variant built with CIMEKV_DEBUG_BOUNDS=1
  * (libcimekv_debug.so), whose kernels check every table index against the

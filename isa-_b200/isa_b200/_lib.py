@@ -19,6 +19,11 @@ import torch
 _LIB_PATH = Path(os.environ.get("CIMEKV_LIB", Path(__file__).resolve().parent / "_lib" / "libcimekv.so"))
 
 _c_int, _c_float, _c_size, _vp = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
+_c_ll = ctypes.c_longlong
+
+# Element types of the entry points that take several (CIMEKV_F32, ...).
+TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+LAYER_NORM_MAX_COLS = 16384  # CIMEKV_LAYER_NORM_MAX_COLS
 
 # name -> (restype, argtypes); mirrors include/cimekv.h
 SIGNATURES = {
@@ -49,6 +54,11 @@ SIGNATURES = {
     "cimekv_measured_backward_x": (_c_int, [_vp, _vp, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_int,
                                             _c_float, _c_float, _vp, _c_float, _c_float, _vp, _vp, _vp, _vp]),
     "cimekv_lut_index": (_c_int, [_vp, _c_int, _c_int, _c_float, _c_float, _vp, _vp, _vp]),
+    "cimekv_layer_norm_forward": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_int, _c_ll, _vp, _vp, _c_int, _c_ll, _c_int,
+                                           _c_float, _vp, _vp, _c_int, _vp, _vp, _vp]),
+    "cimekv_layer_norm_workspace_bytes": (_c_size, [_c_ll, _c_int]),
+    "cimekv_layer_norm_backward": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _c_int, _c_ll, _vp, _c_int, _vp, _vp,
+                                            _c_ll, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _c_size, _vp]),
     "cimekv_debug_build": (_c_int, []),
     "cimekv_debug_oob_count": (ctypes.c_uint, [_c_int]),
     "cimekv_fp32_probe": (_c_int, [_vp, _c_int, _c_int, ctypes.POINTER(ctypes.c_longlong), _vp]),
@@ -242,6 +252,31 @@ def lut_index(delta: torch.Tensor, table_size: int, delta_min: float, delta_scal
                                  _ptr(index), _ptr(alpha), _stream(stream))
     _check(rc, "cimekv_lut_index")
     return index, alpha
+
+
+def layer_norm_forward(x, x_stride, delta, delta_stride, weight, bias, rows, cols, eps, h, y, mean, rstd,
+                       stream=None) -> None:
+    """x and delta: 2-D rows (strides in elements); weight and bias share a type; see cimekv.h."""
+    affine = weight if weight is not None else bias
+    rc = load().cimekv_layer_norm_forward(
+        _ptr(x), TYPE_CODES[x.dtype], x_stride, _ptr(delta), 0 if delta is None else TYPE_CODES[delta.dtype],
+        delta_stride, _ptr(weight), _ptr(bias), 0 if affine is None else TYPE_CODES[affine.dtype], rows, cols, eps,
+        _ptr(h), _ptr(y), TYPE_CODES[y.dtype], _ptr(mean), _ptr(rstd), _stream(stream))
+    _check(rc, "cimekv_layer_norm_forward")
+
+
+def layer_norm_backward(dy, dy_stride, dh, dh_stride, h, h_stride, weight, w_dtype, mean, rstd, rows, cols, dx, ddelta,
+                        dw, db, stream=None) -> None:
+    """dw and db in ``w_dtype``; the workspace of their sums is allocated here."""
+    ws = None
+    if dw is not None or db is not None:
+        ws = torch.empty(int(load().cimekv_layer_norm_workspace_bytes(rows, cols)), dtype=torch.uint8, device=h.device)
+    rc = load().cimekv_layer_norm_backward(
+        _ptr(dy), TYPE_CODES[dy.dtype], dy_stride, _ptr(dh), dh_stride, _ptr(h), TYPE_CODES[h.dtype], h_stride,
+        _ptr(weight), 0 if w_dtype is None else TYPE_CODES[w_dtype], _ptr(mean), _ptr(rstd), rows, cols, _ptr(dx),
+        _ptr(ddelta), 0 if ddelta is None else TYPE_CODES[ddelta.dtype], _ptr(dw), _ptr(db), _ptr(ws),
+        0 if ws is None else ws.numel(), _stream(stream))
+    _check(rc, "cimekv_layer_norm_backward")
 
 
 def fp32_probe(sink: torch.Tensor, iters: int, blocks: int, stream=None) -> int:
