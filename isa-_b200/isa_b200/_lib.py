@@ -115,7 +115,8 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _stream(stream) -> int | None:
     if stream is None:
-        return torch.cuda.current_stream().cuda_stream
+        # the handle of torch.cuda.current_stream() without making the Stream object
+        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -254,28 +255,51 @@ def lut_index(delta: torch.Tensor, table_size: int, delta_min: float, delta_scal
     return index, alpha
 
 
-def layer_norm_forward(x, x_stride, delta, delta_stride, weight, bias, rows, cols, eps, h, y, mean, rstd,
+class on_device:
+    """Makes ``device`` current for a launch; costs nothing where it is already."""
+
+    __slots__ = ("to", "back")
+
+    def __init__(self, device: torch.device):
+        self.to, self.back = device.index, None
+
+    def __enter__(self):
+        if torch.cuda.current_device() != self.to:
+            self.back = torch.cuda.device(self.to)
+            self.back.__enter__()
+
+    def __exit__(self, *exc):
+        if self.back is not None:
+            self.back.__exit__(*exc)
+
+
+def layer_norm_forward(x, x_stride, delta, delta_stride, weight, bias, rows, cols, eps, h, y, stats,
                        stream=None) -> None:
-    """x and delta: 2-D rows (strides in elements); weight and bias share a type; see cimekv.h."""
+    """x and delta: rows with strides in elements; weight and bias share a type;
+    stats: [2, rows] fp32 for mean and rstd, or None; see cimekv.h."""
     affine = weight if weight is not None else bias
+    mean = _ptr(stats)
     rc = load().cimekv_layer_norm_forward(
-        _ptr(x), TYPE_CODES[x.dtype], x_stride, _ptr(delta), 0 if delta is None else TYPE_CODES[delta.dtype],
+        x.data_ptr(), TYPE_CODES[x.dtype], x_stride, _ptr(delta), 0 if delta is None else TYPE_CODES[delta.dtype],
         delta_stride, _ptr(weight), _ptr(bias), 0 if affine is None else TYPE_CODES[affine.dtype], rows, cols, eps,
-        _ptr(h), _ptr(y), TYPE_CODES[y.dtype], _ptr(mean), _ptr(rstd), _stream(stream))
+        _ptr(h), y.data_ptr(), TYPE_CODES[y.dtype], mean, mean and mean + 4 * rows, _stream(stream))
     _check(rc, "cimekv_layer_norm_forward")
 
 
-def layer_norm_backward(dy, dy_stride, dh, dh_stride, h, h_stride, weight, w_dtype, mean, rstd, rows, cols, dx, ddelta,
+def layer_norm_backward(dy, dy_stride, dh, dh_stride, h, h_stride, weight, w_dtype, stats, rows, cols, dx, ddelta,
                         dw, db, stream=None) -> None:
     """dw and db in ``w_dtype``; the workspace of their sums is allocated here."""
-    ws = None
+    lib = load()
+    ws, ws_bytes = None, 0
     if dw is not None or db is not None:
-        ws = torch.empty(int(load().cimekv_layer_norm_workspace_bytes(rows, cols)), dtype=torch.uint8, device=h.device)
-    rc = load().cimekv_layer_norm_backward(
-        _ptr(dy), TYPE_CODES[dy.dtype], dy_stride, _ptr(dh), dh_stride, _ptr(h), TYPE_CODES[h.dtype], h_stride,
-        _ptr(weight), 0 if w_dtype is None else TYPE_CODES[w_dtype], _ptr(mean), _ptr(rstd), rows, cols, _ptr(dx),
-        _ptr(ddelta), 0 if ddelta is None else TYPE_CODES[ddelta.dtype], _ptr(dw), _ptr(db), _ptr(ws),
-        0 if ws is None else ws.numel(), _stream(stream))
+        ws_bytes = lib.cimekv_layer_norm_workspace_bytes(rows, cols)
+        ws = h.new_empty(ws_bytes, dtype=torch.uint8)
+    mean = stats.data_ptr()
+    rc = lib.cimekv_layer_norm_backward(
+        dy.data_ptr(), TYPE_CODES[dy.dtype], dy_stride, _ptr(dh), dh_stride, h.data_ptr(), TYPE_CODES[h.dtype],
+        h_stride, _ptr(weight), 0 if w_dtype is None else TYPE_CODES[w_dtype], mean, mean and mean + 4 * rows, rows,
+        cols, _ptr(dx), _ptr(ddelta), 0 if ddelta is None else TYPE_CODES[ddelta.dtype], _ptr(dw), _ptr(db), _ptr(ws),
+        ws_bytes, _stream(stream))
     _check(rc, "cimekv_layer_norm_backward")
 
 

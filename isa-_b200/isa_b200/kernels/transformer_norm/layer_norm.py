@@ -67,68 +67,51 @@ def _check_inputs(x: torch.Tensor, delta: Optional[torch.Tensor], weight: Option
 
 def _rows(t: torch.Tensor, cols: int) -> Tuple[torch.Tensor, int]:
     """``t`` as rows of contiguous elements, and their stride."""
+    if t.is_contiguous():
+        return t, cols
     r = t if t.dim() == 2 else t.reshape(-1, cols)
     if cols > 1 and r.stride(1) != 1:
         r = r.contiguous()
     return r, (r.stride(0) if r.shape[0] > 1 else cols)
 
 
-class _on_device:
-    """Makes ``device`` current for a launch; free where it is already."""
-
-    def __init__(self, device: torch.device):
-        self.to = device.index
-        self.back = None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.to:
-            self.back = torch.cuda.device(self.to)
-            self.back.__enter__()
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            self.back.__exit__(*exc)
-
-
-def _forward(x, delta, weight, bias, eps, out_dtype, stats):
-    """Returns (y, h or None, mean, rstd, h as rows, its stride)."""
+def _forward(x, delta, weight, bias, eps, out_dtype, keep):
+    """Returns (y, h or None, [mean, rstd] or None, weight as read)."""
     cols = x.shape[-1]
-    x2, x_stride = _rows(x.detach(), cols)
-    rows = x2.shape[0]
-    d2, d_stride = (None, 0) if delta is None else _rows(delta.detach(), cols)
-    w = None if weight is None else weight.detach().contiguous()
-    b = None if bias is None else bias.detach().contiguous()
-    y = torch.empty(x.shape, dtype=out_dtype, device=x.device)
-    h = None if delta is None else torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    mean = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-    rstd = torch.empty(rows, dtype=torch.float32, device=x.device) if stats else None
-    with _on_device(x.device):
-        _lib.layer_norm_forward(x2, x_stride, d2, d_stride, w, b, rows, cols, float(eps), h, y, mean, rstd)
-    return y, h, mean, rstd, w
+    rows = x.numel() // cols
+    x2, x_stride = _rows(x, cols)
+    d2, d_stride = (None, 0) if delta is None else _rows(delta, cols)
+    w = None if weight is None else weight.contiguous()
+    b = None if bias is None else bias.contiguous()
+    y = x.new_empty(x.shape, dtype=out_dtype)
+    h = None if delta is None else x.new_empty(x.shape)
+    stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
+    with _lib.on_device(x.device):
+        _lib.layer_norm_forward(x2, x_stride, d2, d_stride, w, b, rows, cols, eps, h, y, stats)
+    return y, h, stats, w
 
 
 def _backward(ctx, dy, dh):
     """Gradients (dx, d delta, dw, db) as far as they are needed."""
-    src, weight, mean, rstd = ctx.saved_tensors
+    src, weight, stats = ctx.saved_tensors
     need_x, need_d, need_w, need_b = ctx.need
-    shape, x_dtype, d_dtype, w_dtype = ctx.meta
+    shape, d_dtype, w_dtype = ctx.meta
     cols = shape[-1]
     if dy is None:  # only the sum was used
-        one = dh
         zero = [torch.zeros(cols, dtype=w_dtype, device=src.device) if n else None for n in (need_w, need_b)]
-        return one if need_x else None, one.to(d_dtype) if need_d else None, *zero
+        return dh if need_x else None, dh.to(d_dtype) if need_d else None, *zero
     g2, g_stride = _rows(dy, cols)
     s2, s_stride = _rows(dh, cols) if dh is not None else (None, 0)
     h2, h_stride = _rows(src, cols)
     # one gradient for both where stream and branch have one type
-    shared = need_d and d_dtype == x_dtype
-    dx = torch.empty(shape, dtype=x_dtype, device=src.device) if need_x or shared else None
-    dd = torch.empty(shape, dtype=d_dtype, device=src.device) if need_d and not shared else None
-    dw = torch.empty(cols, dtype=w_dtype, device=src.device) if need_w else None
-    db = torch.empty(cols, dtype=w_dtype, device=src.device) if need_b else None
-    with _on_device(src.device):
-        _lib.layer_norm_backward(g2, g_stride, s2, s_stride, h2, h_stride, weight, w_dtype, mean, rstd, h2.shape[0],
-                                 cols, dx, dd, dw, db)
+    shared = need_d and d_dtype == src.dtype
+    dx = src.new_empty(shape) if need_x or shared else None
+    dd = src.new_empty(shape, dtype=d_dtype) if need_d and not shared else None
+    dw = src.new_empty(cols, dtype=w_dtype) if need_w else None
+    db = src.new_empty(cols, dtype=w_dtype) if need_b else None
+    with _lib.on_device(src.device):
+        _lib.layer_norm_backward(g2, g_stride, s2, s_stride, h2, h_stride, weight, w_dtype, stats,
+                                 src.numel() // cols, cols, dx, dd, dw, db)
     return dx if need_x else None, dx if shared else dd, dw, db
 
 
@@ -136,9 +119,9 @@ class LayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, eps, out_dtype):
         ctx.need = (ctx.needs_input_grad[0], False, ctx.needs_input_grad[1], ctx.needs_input_grad[2])
-        y, _, mean, rstd, w = _forward(x, None, weight, bias, eps, out_dtype, any(ctx.need))
-        ctx.save_for_backward(x, w, mean, rstd)
-        ctx.meta = (x.shape, x.dtype, None, _affine_dtype(weight, bias))
+        y, _, stats, w = _forward(x, None, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(x, w, stats)
+        ctx.meta = (x.shape, None, _affine_dtype(weight, bias))
         return y
 
     @staticmethod
@@ -152,9 +135,9 @@ class AddLayerNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, weight, bias, eps, out_dtype):
         ctx.need = tuple(ctx.needs_input_grad[:4])
-        y, h, mean, rstd, w = _forward(x, delta, weight, bias, eps, out_dtype, any(ctx.need))
-        ctx.save_for_backward(h, w, mean, rstd)
-        ctx.meta = (x.shape, x.dtype, delta.dtype, _affine_dtype(weight, bias))
+        y, h, stats, w = _forward(x, delta, weight, bias, eps, out_dtype, True)
+        ctx.save_for_backward(h, w, stats)
+        ctx.meta = (x.shape, delta.dtype, _affine_dtype(weight, bias))
         ctx.set_materialize_grads(False)
         return y, h
 
