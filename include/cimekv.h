@@ -280,6 +280,46 @@ int cimekv_layer_norm_backward(const void* dy, int y_type, long long dy_stride,
                                long long rows, int cols, void* dx, void* ddelta, int delta_type,
                                void* dw, void* db, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Largest side of a matrix, and most matrices of one cimekv_muon_step call. */
+#define CIMEKV_ORTHOGONALIZE_MAX_SIDE 32768
+#define CIMEKV_MUON_MAX_MATRICES 128
+
+/*
+ * Newton-Schulz orthogonalisation of `batch` matrices of rows x cols elements
+ * (no counterpart in the reference, which trains with AdamW):
+ *   X = G / max(|G|_F, eps);  `steps` times: X = a X + (b A + c A A) X, A = X X^T
+ * (a tall G is worked on transposed).  The singular values of G move towards 1,
+ * its singular vectors stay.  Row r of matrix i begins at g + i*batch_stride +
+ * r*row_stride (elements), rows are contiguous; out [batch][rows][cols] is
+ * contiguous, of the same type, and does not overlap g.  Products run on the tensor
+ * cores with operands of 22 bits and fp32 accumulation.  Coefficients that let
+ * a singular value grow beyond 3.9 are refused.  A matrix with a NaN or an
+ * infinity gives NaN in all its elements and leaves the others alone.
+ * workspace: cimekv_orthogonalize_workspace_bytes(batch, rows, cols), 256-byte
+ * aligned; its content does not matter.  The result is deterministic.
+ */
+size_t cimekv_orthogonalize_workspace_bytes(int batch, int rows, int cols);
+int cimekv_orthogonalize(const void* g, int type, long long batch_stride, long long row_stride,
+                         int batch, int rows, int cols, int steps, float a, float b, float c, float eps,
+                         void* out, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * One Muon step of `count` matrices of one shape, in place:
+ *   m <- momentum m + (1 - momentum) g          (fp32)
+ *   u  = nesterov ? momentum m + (1 - momentum) g : m
+ *   p <- p (1 - lr weight_decay) - lr scale NS(u)   (NS as cimekv_orthogonalize)
+ * params, grads and momenta are HOST arrays of device pointers to contiguous
+ * [rows][cols] matrices (all distinct); they are read before the call returns.
+ * lr_device, when not NULL, is a device scalar read instead of lr, so that a
+ * captured graph follows a schedule.  workspace as for cimekv_orthogonalize
+ * with batch = count.
+ */
+int cimekv_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta,
+                     int p_type, int g_type, int rows, int cols, float lr, const float* lr_device,
+                     float momentum, int nesterov, float weight_decay, float scale,
+                     int steps, float a, float b, float c, float eps,
+                     void* workspace, size_t workspace_bytes, void* stream);
+
 /*
  * Debug support, no counterpart in the reference.  cimekv_debug_build()
  * returns 1 for the library variant built with CIMEKV_DEBUG_BOUNDS=1

@@ -24,6 +24,8 @@ _c_ll = ctypes.c_longlong
 # Element types of the entry points that take several (CIMEKV_F32, ...).
 TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 LAYER_NORM_MAX_COLS = 16384  # CIMEKV_LAYER_NORM_MAX_COLS
+ORTHOGONALIZE_MAX_SIDE = 32768  # CIMEKV_ORTHOGONALIZE_MAX_SIDE
+MUON_MAX_MATRICES = 128  # CIMEKV_MUON_MAX_MATRICES
 
 # name -> (restype, argtypes); mirrors include/cimekv.h
 SIGNATURES = {
@@ -59,6 +61,12 @@ SIGNATURES = {
     "cimekv_layer_norm_workspace_bytes": (_c_size, [_c_ll, _c_int]),
     "cimekv_layer_norm_backward": (_c_int, [_vp, _c_int, _c_ll, _vp, _c_ll, _vp, _c_int, _c_ll, _vp, _c_int, _vp, _vp,
                                             _c_ll, _c_int, _vp, _vp, _c_int, _vp, _vp, _vp, _c_size, _vp]),
+    "cimekv_orthogonalize_workspace_bytes": (_c_size, [_c_int, _c_int, _c_int]),
+    "cimekv_orthogonalize": (_c_int, [_vp, _c_int, _c_ll, _c_ll, _c_int, _c_int, _c_int, _c_int, _c_float, _c_float,
+                                      _c_float, _c_float, _vp, _vp, _c_size, _vp]),
+    "cimekv_muon_step": (_c_int, [_c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _vp, _c_float,
+                                  _c_int, _c_float, _c_float, _c_int, _c_float, _c_float, _c_float, _c_float, _vp,
+                                  _c_size, _vp]),
     "cimekv_debug_build": (_c_int, []),
     "cimekv_debug_oob_count": (ctypes.c_uint, [_c_int]),
     "cimekv_fp32_probe": (_c_int, [_vp, _c_int, _c_int, ctypes.POINTER(ctypes.c_longlong), _vp]),
@@ -301,6 +309,31 @@ def layer_norm_backward(dy, dy_stride, dh, dh_stride, h, h_stride, weight, w_dty
         cols, _ptr(dx), _ptr(ddelta), 0 if ddelta is None else TYPE_CODES[ddelta.dtype], _ptr(dw), _ptr(db), _ptr(ws),
         ws_bytes, _stream(stream))
     _check(rc, "cimekv_layer_norm_backward")
+
+
+def orthogonalize_workspace_bytes(batch: int, rows: int, cols: int) -> int:
+    return int(load().cimekv_orthogonalize_workspace_bytes(batch, rows, cols))
+
+
+def orthogonalize(g, batch_stride, row_stride, batch, rows, cols, steps, coefficients, eps, out, workspace,
+                  stream=None) -> None:
+    """Matrices [batch][rows][cols] with contiguous rows into the contiguous ``out``."""
+    rc = load().cimekv_orthogonalize(
+        g.data_ptr(), TYPE_CODES[g.dtype], batch_stride, row_stride, batch, rows, cols, steps, *coefficients, eps,
+        out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(stream))
+    _check(rc, "cimekv_orthogonalize")
+
+
+def muon_step(params, grads, momenta, p_dtype, g_dtype, rows, cols, lr, lr_tensor, momentum, nesterov, weight_decay,
+              scale, steps, coefficients, eps, workspace, stream=None) -> None:
+    """params, grads, momenta: lists of device addresses of [rows][cols] matrices."""
+    n = len(params)
+    table = ctypes.c_void_p * n
+    rc = load().cimekv_muon_step(
+        n, table(*params), table(*grads), table(*momenta), TYPE_CODES[p_dtype], TYPE_CODES[g_dtype], rows, cols, lr,
+        _ptr(lr_tensor), momentum, int(nesterov), weight_decay, scale, steps, *coefficients, eps,
+        workspace.data_ptr(), workspace.numel(), _stream(stream))
+    _check(rc, "cimekv_muon_step")
 
 
 def fp32_probe(sink: torch.Tensor, iters: int, blocks: int, stream=None) -> int:
