@@ -7,20 +7,25 @@
 //   A = X X^T,   P = a I + b A + c A A,   X <- P X
 //
 // so the singular values s of X go through s (a + b s^2 + c s^4) and close in on
-// one band around 1, while the singular vectors stay.  All three are products of
-// matrices; everything elementwise sits in their epilogues.
+// one band around 1, while the singular vectors stay.  With the square completed,
+//
+//   B = X X^T + (b / 2c) I,   P = c B B + (a - b^2 / 4c) I,   X <- P X
+//
+// all three are one product each with an epilogue alpha D + beta I, so none of
+// them reads anything but its operands.  (c = 0: P = b X X^T + a I is the first
+// product's, and the second falls away.)
 //
 // Precision.  A singular value far below the largest grows by up to a per step
 // (x 485 in five steps), and so does any rounding noise in its direction: with
 // operands rounded to 11 bits the result of a low-rank update is off by 1e-2, more
-// than the half step of a bf16 result.  X, A and P are therefore held as pairs of
-// fp16 planes, value * 2^12 = hi + lo (22 bits; the iteration keeps singular
-// values of X and A below 2 and of P below 15, checked on the host from the
-// coefficients, so the fixed scale neither overflows nor loses small elements), and a
+// than the half step of a bf16 result.  X, B and P are therefore held as pairs of
+// fp16 planes, value * 2^12 = hi + lo (22 bits; singular values stay below 15,
+// checked on the host from the coefficients, so the fixed scale neither overflows
+// nor loses small elements), and a
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
 // tensor core products, closer to the exact result than fp32 FMAs.
 //
-// A and P are symmetric: only tiles on and below the diagonal are computed, the
+// B and P are symmetric: only tiles on and below the diagonal are computed, the
 // epilogue stores each tile and its mirror image.
 
 #include <cuda.h>
@@ -66,14 +71,15 @@ constexpr float kScale = 4096.0f;  // fp16 planes hold value * 2^12
 constexpr int kTile = 128;         // rows (and right-hand rows) that one CTA stages
 constexpr int kK = 64;             // depth of one stage: 64 halves = one 128-byte swizzle row
 constexpr int kStages = 3;
-constexpr int kChunk = 2;                   // stages summed in tensor memory before fp32 registers take over
 constexpr int kOperand = kTile * kK * 2;    // bytes of one operand plane in a stage
 constexpr int kStageBytes = 4 * kOperand;   // left hi, left lo, right hi, right lo
-constexpr int kEpilogueWarps = 8;
+constexpr int kEpilogueWarps = 16;
+constexpr int kTmemColumns = 512;
 constexpr int kGemmThreads = (kEpilogueWarps + 2) * 32;  // and a copy warp, a product warp
-constexpr int kSmemBytes = kStages * kStageBytes + 1024;
+constexpr int kStagingBytes = 2048;         // a collecting warp's 32 rows of 64 bytes on their way out
+constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;
 constexpr int kMaxTable = CIMEKV_MUON_MAX_MATRICES;
-constexpr int kChunks = 64;                 // partial norms per matrix
+constexpr int kMaxParts = 256;              // partial norms per matrix, at most
 
 // ------------------------------------------------------------- PTX pieces --
 
@@ -86,19 +92,29 @@ __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
 }
 
-// Waits for the phase of `parity` to end, for about a second at most: a wait
+__device__ __forceinline__ unsigned long long wall_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits for the phase of `parity` to end, for two seconds at most: a wait
 // that runs out means a lost copy, and its tile is poisoned instead of hanging.
 __device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    for (int i = 0; i < (1 << 20); ++i) {
+    unsigned long long began = 0;
+    for (int i = 0; i < (1 << 28); ++i) {
         uint32_t done;
         asm volatile(
             "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, 1000;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
             "selp.u32 %0, 1, 0, p;\n\t}"
             : "=r"(done)
             : "r"(bar), "r"(parity)
             : "memory");
         if (done) return true;
+        const unsigned long long now = wall_ns();
+        if (!began) began = now;
+        else if (now - began > 2000000000ull) return false;
     }
     return false;
 }
@@ -110,7 +126,7 @@ __device__ __forceinline__ uint32_t cluster_addr(uint32_t addr, uint32_t rank) {
     return r;
 }
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+    asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 __device__ __forceinline__ void cluster_sync() {
     __syncwarp();
@@ -191,21 +207,19 @@ __device__ __forceinline__ void tmem_free(uint32_t tmem, uint32_t columns) {
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(columns) : "memory");
 }
 
-__device__ __forceinline__ void tmem_load32(uint32_t addr, float (&v)[32]) {
-    uint32_t r[32];
+// 16 accumulator columns of this lane's row.
+__device__ __forceinline__ void tmem_load16(uint32_t addr, float (&v)[16]) {
+    uint32_t r[16];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-        "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];\n\t"
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+        "{%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, [%16];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
-          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]),
-          "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]),
-          "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
         : "r"(addr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
 
 // ------------------------------------------------------------------ types ---
@@ -245,34 +259,87 @@ struct PrepParams {
     int pitch;          // of the planes, elements
     long long plane;    // elements from the hi to the lo plane
     float eps;
-    double* part;       // [batch][kChunks]
+    int parts;          // partial norms per matrix
+    double* part;       // [batch][parts]
     __half* x;
 };
 
+// The next kernel of the chain may be set up while this one runs, and this one
+// touches memory only after the one before has finished and its writes are seen.
+__device__ __forceinline__ void chain() {
+    asm volatile("griddepcontrol.launch_dependents;\n\tgriddepcontrol.wait;" ::: "memory");
+}
+
 // The update before orthogonalisation: G itself, or the (Nesterov) momentum after
 // its own update m <- beta m + (1 - beta) g.
+__device__ __forceinline__ float new_momentum(const PrepParams& p, float g, float m) {
+    return fmaf(p.beta, m, (1.0f - p.beta) * g);
+}
 __device__ __forceinline__ float update_of(const PrepParams& p, float g, float m) {
     return p.nesterov ? fmaf(p.beta, m, (1.0f - p.beta) * g) : m;
 }
 
-// Momentum update and the partial sums of squares of one matrix: kChunks CTAs
-// per matrix, in doubles (squares of fp32 values neither overflow nor vanish),
-// added in a fixed order.
+// Four neighbours from an address that is a multiple of four elements.
+__device__ __forceinline__ void load4(const void* p, int type, long long i, float (&v)[4]) {
+    if (type == CIMEKV_F32) {
+        const float4 q = *reinterpret_cast<const float4*>(static_cast<const float*>(p) + i);
+        v[0] = q.x; v[1] = q.y; v[2] = q.z; v[3] = q.w;
+    } else {
+        const uint2 q = *reinterpret_cast<const uint2*>(static_cast<const unsigned short*>(p) + i);
+        if (type == CIMEKV_BF16) {
+            v[0] = __uint_as_float(q.x << 16); v[1] = __uint_as_float(q.x & 0xffff0000u);
+            v[2] = __uint_as_float(q.y << 16); v[3] = __uint_as_float(q.y & 0xffff0000u);
+        } else {
+            const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&q.x));
+            const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&q.y));
+            v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+        }
+    }
+}
+
+// Momentum update and the partial sums of squares of one matrix, p.parts CTAs
+// to a matrix, in doubles (squares of fp32 values neither overflow nor vanish),
+// added in a fixed order.  kFlat: a matrix is one run of elements that vectors of
+// four fit; otherwise row by row.  Bound by HBM.
+template <bool kFlat>
 __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ PrepParams p) {
     const int b = blockIdx.y;
     const void* g = p.g.at(b);
     float* mom = p.mom.tabled ? static_cast<float*>(p.mom.table[b]) : nullptr;
-    const long long total = (long long)p.rows * p.cols;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     double s = 0.0;
-    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += kChunks * 256) {
-        const long long r = i / p.cols, c = i - r * p.cols;
-        float v = load_as_float(g, p.g.type, r * p.g.row_stride + c);
-        if (mom) {
-            const float m = fmaf(p.beta, mom[i], (1.0f - p.beta) * v);
-            mom[i] = m;
-            v = update_of(p, v, m);
+    if constexpr (kFlat) {
+        const long long total = (long long)p.rows * p.cols / 4;
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)p.parts * 256) {
+            float v[4];
+            load4(g, p.g.type, 4 * i, v);
+            if (mom) {
+                float4 m = *reinterpret_cast<const float4*>(mom + 4 * i);
+                m.x = new_momentum(p, v[0], m.x);
+                m.y = new_momentum(p, v[1], m.y);
+                m.z = new_momentum(p, v[2], m.z);
+                m.w = new_momentum(p, v[3], m.w);
+                *reinterpret_cast<float4*>(mom + 4 * i) = m;
+                v[0] = update_of(p, v[0], m.x);
+                v[1] = update_of(p, v[1], m.y);
+                v[2] = update_of(p, v[2], m.z);
+                v[3] = update_of(p, v[3], m.w);
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) s += (double)v[k] * (double)v[k];
         }
-        s += (double)v * (double)v;
+    } else {
+        for (int r = blockIdx.x; r < p.rows; r += p.parts)
+            for (int c = threadIdx.x; c < p.cols; c += 256) {
+                float v = load_as_float(g, p.g.type, r * p.g.row_stride + c);
+                if (mom) {
+                    const long long i = (long long)r * p.cols + c;
+                    const float m = new_momentum(p, v, mom[i]);
+                    mom[i] = m;
+                    v = update_of(p, v, m);
+                }
+                s += (double)v * (double)v;
+            }
     }
     __shared__ double red[8];
 #pragma unroll
@@ -281,67 +348,144 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Pr
     __syncthreads();
     if (threadIdx.x == 0) {
         for (int w = 1; w < 8; ++w) s += red[w];
-        p.part[(long long)b * kChunks + blockIdx.x] = s;
+        p.part[(long long)b * p.parts + blockIdx.x] = s;
     }
 }
 
-__device__ __forceinline__ void split(float scaled, __half& hi, __half& lo) {
-    hi = __float2half_rn(scaled);
-    lo = __float2half_rn(scaled - __half2float(hi));
+// The planes' words of two neighbours (packed conversions: one instruction for both).
+__device__ __forceinline__ void split2(float a, float b, uint32_t& hi, uint32_t& lo) {
+    const __half2 h = __floats2half2_rn(a, b);
+    const float2 back = __half22float2(h);
+    const __half2 l = __floats2half2_rn(a - back.x, b - back.y);
+    hi = *reinterpret_cast<const uint32_t*>(&h);
+    lo = *reinterpret_cast<const uint32_t*>(&l);
+}
+// Two neighbours in a 16-bit type.
+__device__ __forceinline__ uint32_t pack2(int type, float a, float b) {
+    if (type == CIMEKV_BF16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
 }
 
-// X0 as pairs of planes, transposed where G is tall: 32 x 32 tiles through
-// shared memory, so that reads and writes are both along rows.
-__global__ void __launch_bounds__(256) ns_prepare_kernel(const __grid_constant__ PrepParams p) {
-    __shared__ float tile[32][33];
-    __shared__ float factor;
-    const int b = blockIdx.z;
-    if (threadIdx.x == 0) {
+// 2^12 / max(norm, eps) of matrix b, by the first warp for the whole CTA.
+__device__ __forceinline__ float plane_factor(const PrepParams& p, int b, float* shared) {
+    if (threadIdx.x < 32) {
         double s = 0.0;
-        for (int i = 0; i < kChunks; ++i) s += p.part[(long long)b * kChunks + i];
+        for (int i = threadIdx.x; i < p.parts; i += 32) s += p.part[(long long)b * p.parts + i];
+#pragma unroll
+        for (int o = 16; o; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
         const double norm = sqrt(s);
-        factor = (float)((double)kScale / (norm > (double)p.eps || norm != norm ? norm : (double)p.eps));
-    }
-    const void* g = p.g.at(b);
-    const float* mom = p.mom.tabled ? static_cast<const float*>(p.mom.table[b]) : nullptr;
-    const int r0 = blockIdx.y * 32, c0 = blockIdx.x * 32;
-    const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;
-    for (int k = ty; k < 32; k += 8) {
-        const int r = r0 + k, c = c0 + tx;
-        if (r < p.rows && c < p.cols) {
-            float v = load_as_float(g, p.g.type, r * p.g.row_stride + c);
-            if (mom) v = update_of(p, v, mom[(long long)r * p.cols + c]);
-            tile[k][tx] = v;
-        }
+        if (threadIdx.x == 0)
+            *shared = (float)((double)kScale / (norm > (double)p.eps || norm != norm ? norm : (double)p.eps));
     }
     __syncthreads();
-    const int m = p.transposed ? p.cols : p.rows, n = p.transposed ? p.rows : p.cols;
-    __half* x = p.x + (long long)b * m * p.pitch;
-    for (int k = ty; k < 32; k += 8) {
-        const int r = (p.transposed ? c0 : r0) + k, c = (p.transposed ? r0 : c0) + tx;
-        if (r < m && c < n) {
-            __half hi, lo;
-            split((p.transposed ? tile[tx][k] : tile[k][tx]) * factor, hi, lo);
-            x[(long long)r * p.pitch + c] = hi;
-            x[p.plane + (long long)r * p.pitch + c] = lo;
+    return *shared;
+}
+
+// X0 as pairs of planes: a thread's eight neighbours of one row (8 x 256 tiles).
+// kVec: rows of G and of the momenta can be read in vectors of four.
+template <bool kVec>
+__global__ void __launch_bounds__(256) ns_prepare_kernel(const __grid_constant__ PrepParams p) {
+    __shared__ float shared;
+    chain();
+    const int b = blockIdx.z;
+    const float factor = plane_factor(p, b, &shared);
+    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+    if (r >= p.rows || c >= p.cols) return;
+    const void* g = p.g.at(b);
+    const float* mom = p.mom.tabled ? static_cast<const float*>(p.mom.table[b]) + (long long)r * p.cols : nullptr;
+    float v[8] = {};
+    if constexpr (kVec) {
+#pragma unroll
+        for (int h = 0; h < 8; h += 4) {
+            if (c + h < p.cols) {
+                float q[4];
+                load4(g, p.g.type, r * p.g.row_stride + c + h, q);
+                if (mom) {
+                    const float4 m = *reinterpret_cast<const float4*>(mom + c + h);
+                    q[0] = update_of(p, q[0], m.x);
+                    q[1] = update_of(p, q[1], m.y);
+                    q[2] = update_of(p, q[2], m.z);
+                    q[3] = update_of(p, q[3], m.w);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) v[h + k] = q[k];
+            }
         }
+    } else {
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (c + k < p.cols) {
+                v[k] = load_as_float(g, p.g.type, r * p.g.row_stride + c + k);
+                if (mom) v[k] = update_of(p, v[k], mom[c + k]);
+            }
+    }
+    uint32_t hi[4], lo[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) split2(v[2 * k] * factor, v[2 * k + 1] * factor, hi[k], lo[k]);
+    // the pitch is a multiple of 8: a group that begins inside a row ends inside its pitch
+    __half* x = p.x + ((long long)b * p.rows + r) * p.pitch + c;
+    *reinterpret_cast<uint4*>(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+    *reinterpret_cast<uint4*>(x + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+}
+
+// The same for a tall G, transposed: 64 x 64 tiles through shared memory, so
+// that reads and writes are both along rows.
+__global__ void __launch_bounds__(256) ns_prepare_tall_kernel(const __grid_constant__ PrepParams p) {
+    __shared__ float tile[64][65];
+    __shared__ float shared;
+    chain();
+    const int b = blockIdx.z;
+    const float factor = plane_factor(p, b, &shared);
+    const void* g = p.g.at(b);
+    const float* mom = p.mom.tabled ? static_cast<const float*>(p.mom.table[b]) : nullptr;
+    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
+#pragma unroll 4
+    for (int k = ty; k < 64; k += 4) {
+        const int r = r0 + k, c = c0 + tx;
+        float v = 0.0f;
+        if (r < p.rows && c < p.cols) {
+            v = load_as_float(g, p.g.type, r * p.g.row_stride + c);
+            if (mom) v = update_of(p, v, mom[(long long)r * p.cols + c]);
+        }
+        tile[k][tx] = v * factor;
+    }
+    __syncthreads();
+    // X has cols rows and rows columns
+    for (int i = threadIdx.x; i < 64 * 8; i += 256) {
+        const int xr = i >> 3, k = (i & 7) * 8;
+        if (c0 + xr >= p.cols || r0 + k >= p.rows) continue;
+        uint32_t hi[4], lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split2(tile[k + 2 * j][xr], tile[k + 2 * j + 1][xr], hi[j], lo[j]);
+        __half* x = p.x + ((long long)b * p.cols + c0 + xr) * p.pitch + r0 + k;
+        *reinterpret_cast<uint4*>(x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+        *reinterpret_cast<uint4*>(x + p.plane) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
     }
 }
 
 // ---------------------------------------------------------------- products --
 
-enum Mode { kGram = 0, kPoly = 1, kApply = 2, kResult = 3 };
+// kSymmetric: alpha L L^T + beta I, one triangle; kApply: L R; kResult: L R to the caller's matrices.
+enum Mode { kSymmetric = 0, kApply = 1, kResult = 2 };
 
-struct GemmParams {
-    int rows, cols, depth;  // of the product
-    int batch;
-    __half* out;            // planes of the result (kGram, kPoly, kApply)
+// One product of a batch.
+struct Product {
+    int rows, cols, depth;
+    __half* out;            // planes of the result (not kResult)
     long long out_plane;    // elements from hi to lo
     int out_pitch;
-    const __half* a;        // planes of A (kPoly)
-    float ca, cb, cc;
-    // kResult: where X goes
+    float alpha, beta;      // on values as the planes hold them
+};
+
+// Where the last product goes.
+struct Result {
     int transposed;
+    int vec;                // rows of dst can be moved in vectors of 16 bytes
     Matrices dst;           // results, or parameters to update in place
     int update;             // parameters: p <- p (1 - lr decay) - lr scale X
     float lr, decay, scale;
@@ -356,124 +500,184 @@ __device__ __forceinline__ void triangle(int t, int& i, int& j) {
     j = t - i * (i + 1) / 2;
 }
 
-// 32 columns of one row of a finished tile: `v` are sums of scaled products.
-template <int M>
-__device__ __forceinline__ void finish(const GemmParams& p, float (&v)[32], int b, int r, int cb, bool mirrored, float lr) {
-    if constexpr (M == kResult) {
-        void* dst = const_cast<void*>(p.dst.at(b));
+// The new value of an element of the result or parameter.
+__device__ __forceinline__ float result_of(const Result& p, float sum, float old, float lr) {
+    const float o = sum * (1.0f / (kScale * kScale));
+    return p.update ? fmaf(-lr * p.scale, o, fmaf(-lr * p.decay, old, old)) : o;
+}
+
+// Turns rows held by lanes into row segments: on entry lane i holds 64 bytes of
+// row i, on exit d[t] is bytes 16 (i % 4) .. + 15 of row 8 t + i / 4, so that a
+// store covers eight segments of 64 bytes instead of 32 of 16 (an SM moves one
+// 128-byte line a cycle however little of it is used: straight from the registers the
+// stores of a 128 x 128 tile took 6,000 cycles).  Units of 16 bytes are
+// swizzled: both sides are free of bank conflicts.
+__device__ __forceinline__ void turn_rows(uint32_t staging, const uint4 (&r)[4], uint4 (&d)[4]) {
+    const int lane = threadIdx.x & 31;
+    __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            if (cb + i >= p.cols) break;
-            const long long at = p.transposed ? (long long)(cb + i) * p.rows + r : (long long)r * p.cols + cb + i;
-            float o = v[i] * (1.0f / (kScale * kScale));
-            if (p.update) {
-                const float w = load_as_float(dst, p.dst.type, at);
-                o = fmaf(-lr * p.scale, o, fmaf(-lr * p.decay, w, w));
-            }
-            store_float(dst, p.dst.type, at, o);
-        }
-    } else {
-        const long long mat = (long long)b * p.rows * p.out_pitch;
-        uint32_t hi[16], lo[16];
-        const __half* ah = p.a + mat + (long long)r * p.out_pitch + cb;
+    for (int k = 0; k < 4; ++k) {
+        const uint32_t at = staging + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4);
+        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[k].x), "r"(r[k].y), "r"(r[k].z), "r"(r[k].w)
+                     : "memory");
+    }
+    __syncwarp();
 #pragma unroll
-        for (int i = 0; i < 32; ++i) {
-            float o = v[i] * (1.0f / kScale);
-            if (M == kPoly) {
-                const bool in = cb + i < p.cols;
-                const float a = in ? __half2float(ah[i]) + __half2float(ah[p.out_plane + i]) : 0.0f;
-                o = fmaf(p.cc, o, p.cb * a) + (r == cb + i ? p.ca * kScale : 0.0f);
-            }
-            v[i] = o;
-        }
+    for (int t = 0; t < 4; ++t) {
+        const int row = 8 * t + (lane >> 2);
+        const uint32_t at = staging + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4);
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(d[t].x), "=r"(d[t].y), "=r"(d[t].z), "=r"(d[t].w)
+                     : "r"(at)
+                     : "memory");
+    }
+}
+
+// 16 columns from cb of the warp's 32 rows from row0 of the last product, to the
+// caller's matrix.  Called by whole warps.
+__device__ __forceinline__ void finish_result(const Result& p, int rows, int cols, const float (&v)[16], int b, int row0,
+                                              int cb, float lr, uint32_t staging) {
+    void* dst = const_cast<void*>(p.dst.at(b));
+    const int type = p.dst.type, lane = threadIdx.x & 31;
+    if (p.transposed) {  // neighbouring lanes hold neighbouring elements
+        const int r = row0 + lane;
+        if (r >= rows) return;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
-            __half h0, l0, h1, l1;
-            split(v[2 * i], h0, l0);
-            split(v[2 * i + 1], h1, l1);
-            hi[i] = (uint32_t)__half_as_ushort(h0) | (uint32_t)__half_as_ushort(h1) << 16;
-            lo[i] = (uint32_t)__half_as_ushort(l0) | (uint32_t)__half_as_ushort(l1) << 16;
+            if (cb + i >= cols) break;
+            const long long at = (long long)(cb + i) * rows + r;
+            store_float(dst, type, at, result_of(p, v[i], p.update ? load_as_float(dst, type, at) : 0.0f, lr));
         }
-        __half* oh = p.out + mat + (long long)r * p.out_pitch + cb;
+        return;
+    }
+    uint4 in[4], out[4];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {  // the pitch is a multiple of 8: a group that begins inside ends inside
-            if (cb + 8 * i < p.cols) {
-                *reinterpret_cast<uint4*>(oh + 8 * i) = make_uint4(hi[4 * i], hi[4 * i + 1], hi[4 * i + 2], hi[4 * i + 3]);
-                *reinterpret_cast<uint4*>(oh + p.out_plane + 8 * i) =
-                    make_uint4(lo[4 * i], lo[4 * i + 1], lo[4 * i + 2], lo[4 * i + 3]);
+    for (int k = 0; k < 4; ++k)
+        in[k] = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
+                           __float_as_uint(v[4 * k + 3]));
+    turn_rows(staging, in, out);
+    const int c = cb + (lane & 3) * 4;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        const int r = row0 + 8 * t + (lane >> 2);
+        if (r >= rows || c >= cols) continue;
+        const long long at = (long long)r * cols + c;
+        const float x[4] = {__uint_as_float(out[t].x), __uint_as_float(out[t].y), __uint_as_float(out[t].z),
+                            __uint_as_float(out[t].w)};
+        if (p.vec) {  // rows of whole vectors
+            float o[4] = {};
+            if (p.update) load4(dst, type, at, o);
+#pragma unroll
+            for (int k = 0; k < 4; ++k) o[k] = result_of(p, x[k], o[k], lr);
+            if (type == CIMEKV_F32) {
+                *reinterpret_cast<float4*>(static_cast<float*>(dst) + at) = make_float4(o[0], o[1], o[2], o[3]);
+            } else {
+                uint32_t q[2];
+#pragma unroll
+                for (int k = 0; k < 2; ++k)
+                    q[k] = pack2(type, o[2 * k], o[2 * k + 1]);
+                *reinterpret_cast<uint2*>(static_cast<unsigned short*>(dst) + at) = make_uint2(q[0], q[1]);
             }
-        }
-        if (M <= kPoly && mirrored) {
-            __half* mirror = p.out + mat + (long long)cb * p.out_pitch + r;
+        } else {
 #pragma unroll
-            for (int i = 0; i < 32; ++i) {
-                if (cb + i < p.cols) {
-                    const uint32_t h = hi[i / 2] >> (16 * (i & 1)), l = lo[i / 2] >> (16 * (i & 1));
-                    mirror[(long long)i * p.out_pitch] = __ushort_as_half((unsigned short)h);
-                    mirror[p.out_plane + (long long)i * p.out_pitch] = __ushort_as_half((unsigned short)l);
-                }
+            for (int k = 0; k < 4; ++k)
+                if (c + k < cols)
+                    store_float(dst, type, at + k,
+                                result_of(p, x[k], p.update ? load_as_float(dst, type, at + k) : 0.0f, lr));
+        }
+    }
+}
+
+// 32 columns from cb of the warp's 32 rows from row0 of a product that stays in
+// planes, and their mirror image off the diagonal of a symmetric one.  Called by
+// whole warps.
+template <bool kSym>
+__device__ __forceinline__ void finish_planes(const Product& p, const float (&v0)[16], const float (&v1)[16], int b,
+                                              int row0, int cb, bool diagonal, uint32_t staging) {
+    const int lane = threadIdx.x & 31, r = row0 + lane;
+    __half* matrix = p.out + (long long)b * p.rows * p.out_pitch;
+    uint32_t words[2][16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        float o[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            o[k] = (i < 8 ? v0[(2 * i + k) & 15] : v1[(2 * i + k) & 15]) * p.alpha;
+            if (kSym && diagonal && r == cb + 2 * i + k) o[k] += p.beta;
+        }
+        split2(o[0], o[1], words[0][i], words[1][i]);
+    }
+#pragma unroll
+    for (int plane = 0; plane < 2; ++plane) {
+        const uint32_t(&w)[16] = words[plane];
+        uint4 in[4], out[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) in[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
+        turn_rows(staging, in, out);
+        const int c = cb + (lane & 3) * 8;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+            const int row = row0 + 8 * t + (lane >> 2);
+            // the pitch is a multiple of 8: a group that begins inside a row ends inside its pitch
+            if (row < p.rows && c < p.cols)
+                *reinterpret_cast<uint4*>(matrix + plane * p.out_plane + (long long)row * p.out_pitch + c) = out[t];
+        }
+        if (kSym && !diagonal) {
+            // lanes 2k and 2k + 1 exchange, so that the even one holds both rows of an
+            // even column and the odd one those of the next: 32-bit stores along rows
+            const int odd = lane & 1, r2 = r & ~1;
+            __half* mirror = matrix + plane * p.out_plane + (long long)(cb + odd) * p.out_pitch + r2;
+            const uint32_t sel = odd ? 0x3276u : 0x5410u;  // halves {mine, its} of the even, {its, mine} of the odd column
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], 1);
+                if (r2 < p.rows && cb + 2 * i + odd < p.cols)
+                    *reinterpret_cast<uint32_t*>(mirror + (long long)(2 * i) * p.out_pitch) = __byte_perm(w[i], other, sel);
             }
         }
     }
 }
 
-// A persistent loop over output tiles: 128 x 128 by one CTA, or 256 x 256 by a
+// Accumulators in tensor memory (512 columns), and stages summed in one of them.
+__host__ __device__ constexpr int bufs(bool pair) { return pair ? 2 : 4; }
+__host__ __device__ constexpr int chunk_stages(bool pair) { return pair ? 2 : 1; }
+
+// Shared-memory addresses of a CTA's pipeline, and where each role stands in it.
+struct Pipe {
+    uint32_t stages, full, empty, acc_full, acc_empty, tmem;
+    uint32_t rank;          // in the pair
+    int fill;               // copy and product warps: stages so far
+    int chunk;              // product and collecting warps: accumulators so far
+    bool ok;                // no wait has run out
+};
+
+// The tiles first, first + step, ... of one product: 128 x 128 by one CTA, or 256 x 256 by a
 // pair of CTAs whose tensor cores work as one (each stages 128 rows of either
 // operand, holds its 128 rows of the result, and the first CTA issues).  One warp
-// copies stages ahead, one issues products, eight collect.
+// copies stages ahead, one issues products, sixteen collect.
 //
 // The tensor core adds into fp32 accumulators by cutting off, not by rounding:
-// over a long depth that is a drift of half a step per addition.  So a tile's
-// depth is summed in chunks of kChunk stages that alternate between two
-// accumulators, the small cross products of a stage first, and the collecting
-// warps add the chunks in registers with round-to-nearest while the next chunk
-// runs.  The same two accumulators let the next tile start while the last one is
-// stored.
+// over a long depth that is a drift of half a step per addition.  So every stage
+// (4 additions at full size, the small cross products before them) goes into a fresh
+// accumulator, one of two, and the collecting warps add the stages in registers
+// with round-to-nearest while the next stage runs.  The same two accumulators let
+// the next tile start while the last one is stored.
 template <int M, bool kPair>
-__global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
-                                                                  const __grid_constant__ CUtensorMap right,
-                                                                  const __grid_constant__ GemmParams p) {
+__device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right, const Product& p,
+                                        const Result* result, int batch, int first, int step, int tiles) {
     constexpr int kRanks = kPair ? 2 : 1;
-    constexpr int kSide = kTile * kRanks;          // output tile side, and columns of an accumulator
-    constexpr int kWarpCols = kSide / 2;           // columns a collecting warp holds
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kStages + 5];
-    __shared__ uint32_t tmem_slot;
-    const uint32_t stages = (smem_addr(smem_raw) + 1023) & ~1023u;
+    constexpr int kSide = kTile * kRanks;                       // output tile side, and columns of an accumulator
+    constexpr int kWarpCols = kSide / (kEpilogueWarps / 4);     // columns a collecting warp holds
+    constexpr int kBufs = bufs(kPair), kChunk = chunk_stages(kPair);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = kPair ? cluster_rank() : 0;
-    const uint32_t full = smem_addr(bars), empty = full + 8 * kStages, acc_full = full + 16 * kStages,
-                   acc_empty = acc_full + 16, drained = acc_full + 32;
     const int ni = (p.rows + kSide - 1) / kSide, nj = (p.cols + kSide - 1) / kSide;
-    const int per_matrix = M <= kPoly ? ni * (ni + 1) / 2 : ni * nj;
-    const long long tiles = (long long)per_matrix * p.batch;
+    const int per_matrix = M == kSymmetric ? ni * (ni + 1) / 2 : ni * nj;
     const int ksteps = (p.depth + kK - 1) / kK;
-    const int step = gridDim.x / kRanks, first = blockIdx.x / kRanks;
-
-    if (threadIdx.x == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            mbar_init(full + 8 * s, 1);
-            mbar_init(empty + 8 * s, 1);
-        }
-        for (int s = 0; s < 2; ++s) {
-            mbar_init(acc_full + 8 * s, 1);
-            mbar_init(acc_empty + 8 * s, kEpilogueWarps * kRanks);
-        }
-        mbar_init(drained, 1);
-        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    }
-    if (warp == kEpilogueWarps + 1) tmem_alloc<kPair>(smem_addr(&tmem_slot), 2 * kSide);
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if constexpr (kPair) cluster_sync();
-    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-    const uint32_t tmem = tmem_slot;
-
-    const auto place = [&](long long t, int& b, int& row0, int& col0) {
-        b = (int)(t / per_matrix);
-        const int at = (int)(t - (long long)b * per_matrix);
+    const auto place = [&](int t, int& b, int& row0, int& col0) {
+        b = t / per_matrix;
+        const int at = t - b * per_matrix;
         int i, j;
-        if (M <= kPoly) {
+        if (M == kSymmetric) {
             triangle(at, i, j);
         } else {
             i = at / nj;
@@ -485,132 +689,174 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_c
 
     if (warp == kEpilogueWarps) {
         if (lane == 0) {
-            const uint32_t count_at = kPair ? cluster_addr(full, 0) : full;
-            bool ok = true;
-            int fill = 0;
-            for (long long t = first; t < tiles && ok; t += step) {
+            const uint32_t count_at = kPair ? cluster_addr(q.full, 0) : q.full;
+            for (int t = first; t < tiles && q.ok; t += step) {
                 int b, row0, col0;
                 place(t, b, row0, col0);
-                row0 += (int)rank * kTile;
-                col0 += (int)rank * kTile;
-                for (int k = 0; k < ksteps; ++k, ++fill) {
-                    const int s = fill % kStages;
-                    if (fill >= kStages && !(ok = mbar_wait(empty + 8 * s, (fill / kStages - 1) & 1))) break;
-                    const uint32_t base = stages + s * kStageBytes, bar = count_at + 8 * s;
-                    if (rank == 0) mbar_expect(full + 8 * s, kRanks * kStageBytes);
+                row0 += (int)q.rank * kTile;
+                col0 += (int)q.rank * kTile;
+                for (int k = 0; k < ksteps; ++k, ++q.fill) {
+                    const int s = q.fill % kStages;
+                    if (q.fill >= kStages && !(q.ok = mbar_wait(q.empty + 8 * s, (q.fill / kStages - 1) & 1))) break;
+                    const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
+                    const bool same = M == kSymmetric && row0 == col0;  // both operands are the same rows
+                    if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
 #pragma unroll
                     for (int plane = 0; plane < 2; ++plane) {
-                        const int z = plane * p.batch + b;
+                        const int z = plane * batch + b;
                         const uint32_t l = base + plane * kOperand, r = base + (2 + plane) * kOperand;
-                        tma_box<kPair>(l, &left, k * kK, row0, z, bar);
-                        if (M <= kPoly) {
-                            tma_box<kPair>(r, &right, k * kK, col0, z, bar);
+                        tma_box<kPair>(l, left, k * kK, row0, z, bar);
+                        if (same) continue;
+                        if (M == kSymmetric) {
+                            tma_box<kPair>(r, right, k * kK, col0, z, bar);
                         } else {
-                            tma_box<kPair>(r, &right, col0, k * kK, z, bar);
-                            tma_box<kPair>(r + kOperand / 2, &right, col0 + 64, k * kK, z, bar);
+                            tma_box<kPair>(r, right, col0, k * kK, z, bar);
+                            tma_box<kPair>(r + kOperand / 2, right, col0 + 64, k * kK, z, bar);
                         }
                     }
                 }
             }
-            // no copy may still be in flight when the CTA leaves (a pair's are all counted in the first)
-            if (rank == 0)
-                for (int s = 0; s < kStages; ++s) {
-                    const int fills = (fill - s + kStages - 1) / kStages;
-                    if (fills > 0) mbar_wait(full + 8 * s, (fills - 1) & 1);
-                }
         }
     } else if (warp == kEpilogueWarps + 1) {
-        if (lane == 0 && rank == 0) {
+        if (lane == 0 && q.rank == 0) {
             // D fp32, A and B fp16; right operand along K (0) or along its own axis (1)
-            const uint32_t idesc = 1u << 4 | (M <= kPoly ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
+            const uint32_t idesc = 1u << 4 | (M == kSymmetric ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
                                    (uint32_t)(kSide / 16) << 24;
-            bool ok = true;
-            int fill = 0, chunk = 0;
-            for (long long t = first; t < tiles && ok; t += step) {
-                for (int k = 0; k < ksteps && ok; ++chunk) {
-                    const int buf = chunk & 1;
-                    if (chunk >= 2 && !(ok = mbar_wait(acc_empty + 8 * buf, (chunk / 2 - 1) & 1))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t d = tmem + buf * kSide;
+            for (int t = first; t < tiles && q.ok; t += step) {
+                int b, row0, col0;
+                place(t, b, row0, col0);
+                const int r_at = M == kSymmetric && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
+                for (int k = 0; k < ksteps && q.ok; ++q.chunk) {
+                    const int buf = q.chunk % kBufs;
+                    if (q.chunk >= kBufs && !(q.ok = mbar_wait(q.acc_empty + 8 * buf, (q.chunk / kBufs - 1) & 1))) break;
+                    const uint32_t d = q.tmem + buf * kSide;
                     const int end = min(k + kChunk, ksteps);
-                    for (bool fresh = true; k < end; ++k, ++fill, fresh = false) {
-                        const int s = fill % kStages;
-                        if (!(ok = mbar_wait(full + 8 * s, (fill / kStages) & 1))) break;
+                    for (bool fresh = true; k < end; ++k, ++q.fill, fresh = false) {
+                        const int s = q.fill % kStages;
+                        if (!(q.ok = mbar_wait(q.full + 8 * s, (q.fill / kStages) & 1))) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t base = stages + s * kStageBytes;
-                        const auto desc_l = [&](int plane, int q) {
-                            return operand_desc(base + plane * kOperand + q * 32, 16, 1024);
+                        const uint32_t base = q.stages + s * kStageBytes;
+                        const auto desc_l = [&](int plane, int i) {
+                            return operand_desc(base + plane * kOperand + i * 32, 16, 1024);
                         };
-                        const auto desc_r = [&](int plane, int q) {
-                            return M <= kPoly ? operand_desc(base + (2 + plane) * kOperand + q * 32, 16, 1024)
-                                              : operand_desc(base + (2 + plane) * kOperand + q * 2048, 8192, 1024);
+                        const auto desc_r = [&](int plane, int i) {
+                            return M == kSymmetric ? operand_desc(base + r_at + plane * kOperand + i * 32, 16, 1024)
+                                                   : operand_desc(base + r_at + plane * kOperand + i * 2048, 8192, 1024);
                         };
 #pragma unroll
-                        for (int q = 0; q < kK / 16; ++q) {
-                            mma_f16<kPair>(d, desc_l(0, q), desc_r(1, q), idesc, !(fresh && q == 0));
-                            mma_f16<kPair>(d, desc_l(1, q), desc_r(0, q), idesc, 1);
+                        for (int i = 0; i < kK / 16; ++i) {
+                            mma_f16<kPair>(d, desc_l(0, i), desc_r(1, i), idesc, !(fresh && i == 0));
+                            mma_f16<kPair>(d, desc_l(1, i), desc_r(0, i), idesc, 1);
                         }
 #pragma unroll
-                        for (int q = 0; q < kK / 16; ++q) mma_f16<kPair>(d, desc_l(0, q), desc_r(0, q), idesc, 1);
-                        mma_commit<kPair>(empty + 8 * s);
+                        for (int i = 0; i < kK / 16; ++i) mma_f16<kPair>(d, desc_l(0, i), desc_r(0, i), idesc, 1);
+                        mma_commit<kPair>(q.empty + 8 * s);
                     }
-                    if (ok) mma_commit<kPair>(acc_full + 8 * buf);
+                    if (q.ok) mma_commit<kPair>(q.acc_full + 8 * buf);
                 }
             }
-            mma_commit<kPair>(drained);  // no product may still read shared memory when the CTAs leave
-            mbar_wait(drained, 0);
         }
     } else {
-        const int quarter = warp & 3, half = warp >> 2;
-        const uint32_t empty_at = kPair ? cluster_addr(acc_empty, 0) : acc_empty;
-        const float lr = M == kResult && p.update ? (p.lr_dev ? *p.lr_dev : p.lr) : 0.0f;
-        bool ok = true;
-        int chunk = 0;
-        for (long long t = first; t < tiles; t += step) {
+        const int quarter = warp & 3, group = warp >> 2;
+        const uint32_t staging = q.stages + kStages * kStageBytes + warp * kStagingBytes;
+        const uint32_t empty_at = kPair ? cluster_addr(q.acc_empty, 0) : q.acc_empty;
+        float lr = 0.0f;
+        if constexpr (M == kResult) {
+            if (result->update) lr = result->lr_dev ? *result->lr_dev : result->lr;
+        }
+        for (int t = first; t < tiles; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
-            const int r = row0 + (int)rank * kTile + quarter * 32 + lane;
-            const bool mirrored = row0 != col0;
-            col0 += half * kWarpCols;
-            float acc[kWarpCols / 32][32];
+            const int r0 = row0 + (int)q.rank * kTile + quarter * 32;
+            const bool diagonal = row0 == col0;
+            col0 += group * kWarpCols;
+            float acc[kWarpCols / 16][16];
 #pragma unroll
-            for (int g = 0; g < kWarpCols / 32; ++g)
+            for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
-                for (int i = 0; i < 32; ++i) acc[g][i] = 0.0f;
-            for (int k = 0; k < ksteps; k += kChunk, ++chunk) {
-                const int buf = chunk & 1;
-                ok = ok && mbar_wait(acc_full + 8 * buf, (chunk / 2) & 1);
-                __syncwarp();
-                if (!__all_sync(0xffffffffu, ok)) {
-                    ok = false;
-                    continue;
-                }
+                for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
+            for (int k = 0; k < ksteps; k += kChunk, ++q.chunk) {
+                const int buf = q.chunk % kBufs;
+                q.ok = q.ok && mbar_wait(q.acc_full + 8 * buf, (q.chunk / kBufs) & 1);
+                q.ok = __all_sync(0xffffffffu, q.ok);
+                if (!q.ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                const uint32_t src = tmem + ((uint32_t)(quarter * 32) << 16) + buf * kSide + half * kWarpCols;
+                const uint32_t src = q.tmem + ((uint32_t)(quarter * 32) << 16) + buf * kSide + group * kWarpCols;
 #pragma unroll
-                for (int g = 0; g < kWarpCols / 32; ++g) {
-                    float v[32];
-                    tmem_load32(src + g * 32, v);
+                for (int g = 0; g < kWarpCols / 16; ++g) {
+                    float v[16];
+                    tmem_load16(src + g * 16, v);
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[g][i] += v[i];
+                    for (int i = 0; i < 16; ++i) acc[g][i] += v[i];
                 }
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(empty_at + 8 * buf);
             }
-            if (!ok) {  // a lost copy or product shows as NaN, it never passes for a result
+            if (!q.ok) {  // a lost copy or product shows as NaN, it never passes for a result
 #pragma unroll
-                for (int g = 0; g < kWarpCols / 32; ++g)
+                for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) acc[g][i] = __int_as_float(0x7fffffff);
+                    for (int i = 0; i < 16; ++i) acc[g][i] = __int_as_float(0x7fffffff);
             }
-            if (r < p.rows) {
 #pragma unroll
-                for (int g = 0; g < kWarpCols / 32; ++g)
-                    if (col0 + g * 32 < p.cols) finish<M>(p, acc[g], b, r, col0 + g * 32, mirrored, lr);
+            for (int g = 0; g < kWarpCols / 16; ++g) {
+                if (col0 + g * 16 >= p.cols) break;
+                if constexpr (M == kResult)
+                    finish_result(*result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
+                else if (g % 2 == 0)
+                    finish_planes<M == kSymmetric>(p, acc[g], acc[g + 1], b, r0, col0 + g * 16, diagonal, staging);
             }
             __syncwarp();
         }
+    }
+}
+
+// Barriers, tensor memory.  All threads.
+template <bool kPair>
+__device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tmem_slot, uint8_t* smem_raw) {
+    constexpr int kRanks = kPair ? 2 : 1;
+    q.stages = (smem_addr(smem_raw) + 1023) & ~1023u;
+    q.full = smem_addr(bars);
+    q.empty = q.full + 8 * kStages;
+    q.acc_full = q.full + 16 * kStages;
+    q.acc_empty = q.acc_full + 32;
+    q.rank = kPair ? cluster_rank() : 0;
+    q.fill = q.chunk = 0;
+    q.ok = true;
+    if (threadIdx.x == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            mbar_init(q.full + 8 * s, 1);
+            mbar_init(q.empty + 8 * s, 1);
+        }
+        for (int s = 0; s < bufs(kPair); ++s) {
+            mbar_init(q.acc_full + 8 * s, 1);
+            mbar_init(q.acc_empty + 8 * s, kEpilogueWarps * kRanks);
+        }
+        mbar_init(q.acc_full + 64, 1);
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    }
+    if ((threadIdx.x >> 5) == kEpilogueWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), kTmemColumns);
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if constexpr (kPair) cluster_sync();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    q.tmem = *tmem_slot;
+}
+
+// Nothing may be in flight when the CTA leaves: copies (a pair's are all
+// counted in the first CTA), products.  All threads.
+template <bool kPair>
+__device__ __forceinline__ void pipe_close(Pipe& q) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (warp == kEpilogueWarps && lane == 0 && q.rank == 0) {
+        for (int s = 0; s < kStages; ++s) {
+            const int fills = (q.fill - s + kStages - 1) / kStages;
+            if (fills > 0) mbar_wait(q.full + 8 * s, (fills - 1) & 1);
+        }
+    } else if (warp == kEpilogueWarps + 1 && lane == 0 && q.rank == 0) {
+        mma_commit<kPair>(q.acc_full + 64);
+        mbar_wait(q.acc_full + 64, 0);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -618,8 +864,82 @@ __global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_c
     if (warp == kEpilogueWarps + 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_free<kPair>(tmem, 2 * kSide);
+        tmem_free<kPair>(q.tmem, kTmemColumns);
     }
+}
+
+// One product of all matrices, a persistent loop over its tiles.
+template <int M, bool kPair>
+__global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
+                                                                  const __grid_constant__ CUtensorMap right,
+                                                                  const __grid_constant__ Product p,
+                                                                  const __grid_constant__ Result result, int batch, int tiles) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
+    __shared__ uint32_t tmem_slot;
+    Pipe q;
+    pipe_open<kPair>(q, bars, &tmem_slot, smem_raw);
+    chain();
+    constexpr int kRanks = kPair ? 2 : 1;
+    product<M, kPair>(q, &left, &right, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
+    pipe_close<kPair>(q);
+}
+
+// All steps of one matrix by one cluster: the products of a small matrix are
+// a few microseconds each, less than it takes to end one kernel and start the
+// next, so here a cluster barrier stands between them.
+struct Steps {
+    Product gram, square, apply;    // square.rows = 0: c = 0, no square
+    __half* x[2];
+    int steps;
+};
+struct StepMaps {
+    CUtensorMap x[2], right[2], b, p;
+};
+__global__ void __launch_bounds__(kGemmThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
+                                                                   const __grid_constant__ Steps st,
+                                                                   const __grid_constant__ Result result, int batch) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
+    __shared__ uint32_t tmem_slot;
+    Pipe q;
+    pipe_open<false>(q, bars, &tmem_slot, smem_raw);
+    chain();
+    uint32_t size;
+    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
+    const int matrix = blockIdx.x / size;
+    const int ni = (st.gram.rows + kTile - 1) / kTile, nj = (st.apply.cols + kTile - 1) / kTile;
+    const int triangle_tiles = ni * (ni + 1) / 2, all_tiles = ni * nj;
+    const auto ends = [&](int tiles, int& first, int& end) {
+        first = matrix * tiles + (int)cluster_rank();
+        end = (matrix + 1) * tiles;
+    };
+    // planes are written by ordinary stores and read by copies of the other CTAs
+    const auto next = [&]() {
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+        cluster_sync();
+        if (threadIdx.x == kEpilogueWarps * 32) asm volatile("fence.proxy.async.global;" ::: "memory");
+    };
+    for (int k = 0; k < st.steps; ++k) {
+        int first, end;
+        ends(triangle_tiles, first, end);
+        product<kSymmetric, false>(q, &maps.x[k & 1], &maps.x[k & 1], st.gram, nullptr, batch, first, size, end);
+        next();
+        if (st.square.rows) {
+            product<kSymmetric, false>(q, &maps.b, &maps.b, st.square, nullptr, batch, first, size, end);
+            next();
+        }
+        ends(all_tiles, first, end);
+        if (k + 1 < st.steps) {
+            Product p = st.apply;
+            p.out = st.x[(k + 1) & 1];
+            product<kApply, false>(q, &maps.p, &maps.right[k & 1], p, nullptr, batch, first, size, end);
+            next();
+        } else {
+            product<kResult, false>(q, &maps.p, &maps.right[k & 1], st.apply, &result, batch, first, size, end);
+        }
+    }
+    pipe_close<false>(q);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -658,6 +978,7 @@ int plane_map(EncodeFn encode, CUtensorMap* map, __half* base, int batch, int ro
 // Workspace: partial norms, X twice, A, P (pairs of planes each).
 struct Layout {
     int m, n, xp, ap;               // sides (m <= n) and pitches
+    int parts;                      // partial norms per matrix: one per 4096 elements
     size_t part, x0, x1, a, p, bytes;
     long long x_plane, a_plane;     // elements
 
@@ -674,7 +995,9 @@ struct Layout {
             at += (b + 255) / 256 * 256;
             return here;
         };
-        part = take((size_t)batch * kChunks * sizeof(double));
+        const long long want = ((long long)rows * cols + 4095) / 4096;
+        parts = want < kMaxParts ? (int)want : kMaxParts;
+        part = take((size_t)batch * parts * sizeof(double));
         x0 = take((size_t)x_plane * 4);
         x1 = take((size_t)x_plane * 4);
         a = take((size_t)a_plane * 4);
@@ -689,24 +1012,28 @@ int check_iteration(int batch, int rows, int cols, int steps, float a, float b, 
     if (batch < 0 || rows < 0 || cols < 0) return fail(CIMEKV_EINVAL_SHAPE, "negative size");
     if (rows > kMaxSide || cols > kMaxSide || batch > 65535)
         return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: sides of at most 32768, at most 65535 matrices");
+    const long long tiles = ((rows + 127LL) / 128) * ((cols + 127LL) / 128) * batch;
+    if (tiles > 0x3fffffff) return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: too many elements for one call");
     if (steps < 1 || steps > 64) return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: 1 to 64 steps");
     if (!(eps > 0.0f)) return fail(CIMEKV_EINVAL_SHAPE, "eps must be > 0");
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
         return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: coefficients must be finite");
-    // Largest singular value over the steps, and largest |a + b l + c l^2| on its
-    // range: both must fit the planes' fixed scale (16 / 2^12-scaled fp16).
+    // Largest singular values of X, B and P over the steps: they must fit the
+    // planes' fixed scale (2^16 / 2^12).
+    const double shift = c != 0.0f ? 0.5 * b / c : 0.0;
     double s = 1.001;
     for (int k = 0; k < steps; ++k) {
-        double next = 0.0, poly = 0.0;
+        double next = 0.0, most = std::fabs(shift);
         for (int i = 0; i <= 1024; ++i) {
             const double t = s * i / 1024.0, q = a + (b + c * t * t) * t * t;
             next = std::fmax(next, std::fabs(t * q));
-            poly = std::fmax(poly, std::fabs(q));
+            most = std::fmax(most, std::fmax(std::fabs(q), std::fabs(t * t + shift)));
         }
         s = next * 1.001;
-        if (!(s <= 3.9 && poly <= 15.0))
+        if (!(s <= 3.9 && most <= 15.0))
             return fail(CIMEKV_EINVAL_SHAPE,
-                        "orthogonalize: these coefficients let singular values grow beyond 3.9 (or their factor beyond 15)");
+                        "orthogonalize: these coefficients let singular values grow beyond 3.9, or a + b s^2 + c s^4 or "
+                        "s^2 + b / 2c beyond 15");
     }
     return CIMEKV_OK;
 }
@@ -719,45 +1046,85 @@ int sm_count(int* sms) {
     return CIMEKV_OK;
 }
 
-long long tile_count(int mode, int side, const GemmParams& p) {
-    const long long ni = (p.rows + side - 1) / side, nj = (p.cols + side - 1) / side;
-    return (mode <= kPoly ? ni * (ni + 1) / 2 : ni * nj) * p.batch;
+long long tile_count(int mode, int side, int rows, int cols) {
+    const long long ni = (rows + side - 1) / side, nj = (cols + side - 1) / side;
+    return mode == kSymmetric ? ni * (ni + 1) / 2 : ni * nj;
+}
+
+// Launches `kernel` as a link of the chain (see chain()).
+template <typename... Args>
+int launch_chained(const char* what, void (*kernel)(Args...), dim3 grid, int threads, size_t smem, int cluster,
+                   cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e == cudaSuccess) return CIMEKV_OK;
+    (void)cudaGetLastError();
+    char msg[256];
+    snprintf(msg, sizeof(msg), "%s: %s", what, cudaGetErrorString(e));
+    return fail(CIMEKV_ECUDA, msg);
 }
 
 template <int M, bool kPair>
-int launch_as(const CUtensorMap& l, const CUtensorMap& r, const GemmParams& p, int sms, cudaStream_t s) {
-    cudaError_t e = cudaFuncSetAttribute(ns_gemm_kernel<M, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+int launch_as(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
+              cudaStream_t s) {
+    const cudaError_t e =
+        cudaFuncSetAttribute(ns_gemm_kernel<M, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
     if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
     constexpr int ranks = kPair ? 2 : 1;
-    const long long tiles = tile_count(M, kTile * ranks, p), most = sms / ranks;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(tiles < most ? tiles : most) * ranks);
-    cfg.blockDim = dim3(kGemmThreads);
-    cfg.dynamicSmemBytes = kSmemBytes;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeClusterDimension;
-    attr[0].val.clusterDim.x = ranks;
-    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = kPair ? 1 : 0;
-    e = cudaLaunchKernelEx(&cfg, ns_gemm_kernel<M, kPair>, l, r, p);
-    if (e != cudaSuccess) {
-        (void)cudaGetLastError();
-        return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
-    }
-    return CIMEKV_OK;
+    const long long tiles = tile_count(M, kTile * ranks, p.rows, p.cols) * batch, most = sms / ranks;
+    return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kPair>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
+                          kGemmThreads, kSmemBytes, ranks, s, l, r, p, result, batch, (int)tiles);
 }
 
 // Pairs once single tiles would fill every SM anyway: the larger tile halves
 // the operand traffic; below that the smaller one spreads over more SMs.
 template <int M>
-int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const GemmParams& p, int sms, cudaStream_t s) {
-    return tile_count(M, kTile, p) > sms ? launch_as<M, true>(l, r, p, sms, s) : launch_as<M, false>(l, r, p, sms, s);
+int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
+                cudaStream_t s) {
+    return tile_count(M, kTile, p.rows, p.cols) * batch > sms ? launch_as<M, true>(l, r, p, result, batch, sms, s)
+                                                              : launch_as<M, false>(l, r, p, result, batch, sms, s);
+}
+
+// CTAs per matrix when all steps run in one kernel, 0 when each product is its own.
+int steps_cluster(int batch, int m, int n, int sms) {
+    const long long tiles = tile_count(kApply, kTile, m, n);
+    static const char* force = getenv("NS_CLUSTER");
+    if (force) return (int)std::min<long long>(tiles, atoi(force));
+    return 0;
+}
+
+int type_bytes(int type) { return type == CIMEKV_F32 ? 4 : 2; }
+
+// Whether every matrix begins on a multiple of `bytes`.
+bool aligned(const Matrices& m, int batch, int bytes) {
+    if (m.tabled) {
+        for (int i = 0; i < batch; ++i)
+            if ((uintptr_t)m.table[i] % bytes) return false;
+        return true;
+    }
+    return (uintptr_t)m.base % bytes == 0 && (batch == 1 || m.batch_stride * type_bytes(m.type) % bytes == 0);
+}
+
+// Whether every row of every matrix can be read in vectors of four elements.
+bool rows_in_fours(const Matrices& m, int batch, int cols) {
+    if (!m.tabled && !m.base) return true;
+    return cols % 4 == 0 && m.row_stride % 4 == 0 && aligned(m, batch, 4 * type_bytes(m.type));
 }
 
 // Everything after the arguments are checked: norms, X0, the steps, the result.
-int run(PrepParams& prep, GemmParams& out, int batch, int rows, int cols, int steps, float a, float b, float c,
+int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int steps, float a, float b, float c,
         uint8_t* ws, cudaStream_t s) {
     const Layout lay(batch, rows, cols);
     EncodeFn encode;
@@ -767,58 +1134,81 @@ int run(PrepParams& prep, GemmParams& out, int batch, int rows, int cols, int st
     __half* x[2] = {reinterpret_cast<__half*>(ws + lay.x0), reinterpret_cast<__half*>(ws + lay.x1)};
     __half* am = reinterpret_cast<__half*>(ws + lay.a);
     __half* pm = reinterpret_cast<__half*>(ws + lay.p);
-    // X as rows along K (Gram) and as the right operand whose rows are K (apply)
-    CUtensorMap xmap[2], xright[2], amap, pmap;
+    StepMaps maps;  // X as rows along K (Gram) and as the right operand whose rows are K (apply)
     for (int i = 0; i < 2; ++i) {
-        if ((rc = plane_map(encode, &xmap[i], x[i], batch, lay.m, lay.n, lay.xp, kTile))) return rc;
-        if ((rc = plane_map(encode, &xright[i], x[i], batch, lay.m, lay.n, lay.xp, kK))) return rc;
+        if ((rc = plane_map(encode, &maps.x[i], x[i], batch, lay.m, lay.n, lay.xp, kTile))) return rc;
+        if ((rc = plane_map(encode, &maps.right[i], x[i], batch, lay.m, lay.n, lay.xp, kK))) return rc;
     }
-    if ((rc = plane_map(encode, &amap, am, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
-    if ((rc = plane_map(encode, &pmap, pm, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
+    if ((rc = plane_map(encode, &maps.b, am, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
+    if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
 
     prep.rows = rows;
     prep.cols = cols;
     prep.transposed = rows > cols;
     prep.pitch = lay.xp;
     prep.plane = lay.x_plane;
+    prep.parts = lay.parts;
     prep.part = reinterpret_cast<double*>(ws + lay.part);
     prep.x = x[0];
+    const bool vec = rows_in_fours(prep.g, batch, cols) && rows_in_fours(prep.mom, batch, cols);
+    const bool flat = vec && (prep.g.row_stride == cols || rows == 1);
     if ((rc = cimekv_internal_no_pending_error())) return rc;
-    ns_norm_kernel<<<dim3(kChunks, batch), 256, 0, s>>>(prep);
+    const dim3 norm_grid(lay.parts, batch);
+    if (flat) ns_norm_kernel<true><<<norm_grid, 256, 0, s>>>(prep);
+    else ns_norm_kernel<false><<<norm_grid, 256, 0, s>>>(prep);
     if ((rc = launched("ns_norm_kernel"))) return rc;
-    ns_prepare_kernel<<<dim3((cols + 31) / 32, (rows + 31) / 32, batch), 256, 0, s>>>(prep);
-    if ((rc = launched("ns_prepare_kernel"))) return rc;
+    if (prep.transposed)
+        rc = launch_chained("ns_prepare_tall_kernel", ns_prepare_tall_kernel,
+                            dim3((cols + 63) / 64, (rows + 63) / 64, batch), 256, 0, 1, s, prep);
+    else
+        rc = launch_chained("ns_prepare_kernel", vec ? ns_prepare_kernel<true> : ns_prepare_kernel<false>,
+                            dim3((cols + 255) / 256, (rows + 7) / 8, batch), 256, 0, 1, s, prep);
+    if (rc) return rc;
 
-    GemmParams g = {};
-    g.batch = batch;
-    g.ca = a;
-    g.cb = b;
-    g.cc = c;
+    // sums of products of two planes are 2^24 times the value, planes 2^12 times
+    const bool squared = c != 0.0f;
+    Steps st = {};
+    st.steps = steps;
+    st.x[0] = x[0];
+    st.x[1] = x[1];
+    st.gram.rows = st.gram.cols = lay.m;
+    st.gram.depth = lay.n;
+    st.gram.out = squared ? am : pm;
+    st.gram.out_plane = lay.a_plane;
+    st.gram.out_pitch = lay.ap;
+    st.gram.alpha = (squared ? 1.0f : b) / kScale;
+    st.gram.beta = (squared ? (float)(0.5 * b / c) : a) * kScale;
+    if (squared) {
+        st.square = st.gram;
+        st.square.depth = lay.m;
+        st.square.out = pm;
+        st.square.alpha = c / kScale;
+        st.square.beta = (float)(a - 0.25 * (double)b * b / c) * kScale;
+    }
+    st.apply.rows = st.apply.depth = lay.m;
+    st.apply.cols = lay.n;
+    st.apply.out_plane = lay.x_plane;
+    st.apply.out_pitch = lay.xp;
+    st.apply.alpha = 1.0f / kScale;
+    result.transposed = prep.transposed;
+    result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
+
+    const int cluster = steps_cluster(batch, lay.m, lay.n, sms);
+    if (cluster) {
+        cudaError_t e = cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        if (e == cudaSuccess && cluster > 8)
+            e = cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
+        if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
+        return launch_chained("ns_steps_kernel", ns_steps_kernel, dim3((unsigned)batch * cluster), kGemmThreads,
+                              kSmemBytes, cluster, s, maps, st, result, batch);
+    }
     for (int k = 0; k < steps; ++k) {
-        g.rows = g.cols = lay.m;
-        g.out_pitch = lay.ap;
-        g.out_plane = lay.a_plane;
-        g.depth = lay.n;
-        g.out = am;
-        if ((rc = launch_gemm<kGram>(xmap[k & 1], xmap[k & 1], g, sms, s))) return rc;
-        g.depth = lay.m;
-        g.a = am;
-        g.out = pm;
-        if ((rc = launch_gemm<kPoly>(amap, amap, g, sms, s))) return rc;
-        g.cols = lay.n;
-        if (k + 1 < steps) {
-            g.out = x[(k + 1) & 1];
-            g.out_pitch = lay.xp;
-            g.out_plane = lay.x_plane;
-            if ((rc = launch_gemm<kApply>(pmap, xright[k & 1], g, sms, s))) return rc;
-        } else {
-            out.batch = batch;
-            out.rows = lay.m;
-            out.cols = lay.n;
-            out.depth = lay.m;
-            out.transposed = prep.transposed;
-            if ((rc = launch_gemm<kResult>(pmap, xright[k & 1], out, sms, s))) return rc;
-        }
+        if ((rc = launch_gemm<kSymmetric>(maps.x[k & 1], maps.x[k & 1], st.gram, result, batch, sms, s))) return rc;
+        if (squared && (rc = launch_gemm<kSymmetric>(maps.b, maps.b, st.square, result, batch, sms, s))) return rc;
+        st.apply.out = x[(k + 1) & 1];
+        rc = k + 1 < steps ? launch_gemm<kApply>(maps.p, maps.right[k & 1], st.apply, result, batch, sms, s)
+                           : launch_gemm<kResult>(maps.p, maps.right[k & 1], st.apply, result, batch, sms, s);
+        if (rc) return rc;
     }
     return CIMEKV_OK;
 }
@@ -851,7 +1241,7 @@ extern "C" int cimekv_orthogonalize(const void* g, int type, long long batch_str
     prep.g.row_stride = row_stride;
     prep.g.type = type;
     prep.eps = eps;
-    GemmParams last = {};
+    Result last = {};
     last.dst.base = out;
     last.dst.batch_stride = (long long)rows * cols;
     last.dst.type = type;
@@ -887,12 +1277,12 @@ extern "C" int cimekv_muon_step(int count, void* const* params, const void* cons
         return fail(CIMEKV_EWORKSPACE, "muon step workspace too small");
     if ((uintptr_t)workspace % 256) return fail(CIMEKV_EINVAL_SHAPE, "workspace must be 256-byte aligned");
     PrepParams prep = {};
-    GemmParams last = {};
+    Result last = {};
     prep.g.tabled = prep.mom.tabled = last.dst.tabled = 1;
     prep.g.type = g_type;
     prep.mom.type = CIMEKV_F32;
     last.dst.type = p_type;
-    prep.g.row_stride = cols;
+    prep.g.row_stride = prep.mom.row_stride = cols;
     for (int i = 0; i < count; ++i) {
         prep.g.table[i] = const_cast<void*>(grads[i]);
         prep.mom.table[i] = momenta[i];
