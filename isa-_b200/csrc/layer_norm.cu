@@ -5,15 +5,25 @@
 //   u = (h - mean(h)) * rstd,  rstd = (var(h) + eps)^-1/2,  y = u w + b
 //   dx = rstd (g w - mean(g w) - u mean(g w u)) + dh,  dw = sum_rows g u,  db = sum_rows g
 //
-// Both directions are bound by HBM: every row is read once into registers, the
-// row sums are taken there (mean first, then the centred squares: no
-// cancellation for rows far from zero), and the results leave in the same pass.
-// A row belongs to one warp up to 1024 columns, to one CTA above.  The weight
-// gradients are column sums: each thread keeps the sums of its own columns over
-// all rows of its CTA in registers, the CTA's warps join theirs in shared memory,
-// and a second small kernel adds the CTAs' partials in a fixed order, so the
-// result is the same in every run.  All arithmetic is fp32; 16-bit types are
-// rounded once, at the store.
+// Both directions are bound by HBM: every row is read once, the row sums are taken
+// in registers (mean first, then the centred squares: no cancellation for rows far
+// from zero), and the results leave in the same pass.  A row belongs to one to
+// sixteen warps, so that a thread holds at most 16 elements of usual widths.  Rows
+// come through shared memory by bulk copies, a ring of up to four per row group:
+// enough bytes are under way whatever the registers allow (with the next row's
+// loads held in registers the fp16 backward took 54 us at 50,432 x 384, not 33).
+// The weight gradients are column sums: each thread keeps the sums of its own
+// columns over all rows of its warps in registers, the CTA's row groups join theirs in
+// shared memory, and a second small kernel adds the CTAs' partials in a fixed
+// order, so the result is the same in every run.  All arithmetic is fp32; 16-bit
+// types are rounded once, at the store.
+//
+// Widths that are no multiple of the vector (4 elements of an fp32 row, 8 of a
+// 16-bit one) begin rows at any of V places in a vector.  The rows of one group
+// of warps are V (or a multiple) apart, so that they all begin at the same place
+// and a thread's vectors stay aligned and its columns the same; only the first and
+// last vector of a row is stored by elements.  A copy takes the 16-byte units that
+// hold the row.
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -21,6 +31,8 @@
 
 #include <cstdint>
 #include <cstdio>
+#include <initializer_list>
+#include <utility>
 
 #include "cimekv.h"
 #include <nvtx3/nvToolsExt.h>
@@ -46,110 +58,226 @@ constexpr int kReduceLanes = 32;  // partial rows added side by side by one bloc
 
 __host__ __device__ inline int type_bytes(int type) { return type == CIMEKV_F32 ? 4 : 2; }
 
-// One row's elements of a thread: E groups of V neighbours, groups T*V apart.
+// ------------------------------------------------------------- PTX pieces --
+
+__device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
+__device__ __forceinline__ unsigned long long wall_ns() {
+    unsigned long long t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+
+// Waits for the phase of `parity` to end, for two seconds at most.
+__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
+    unsigned long long began = 0;
+    for (int i = 0; i < (1 << 28); ++i) {
+        uint32_t done;
+        asm volatile(
+            "{\n\t.reg .pred p;\n\t"
+            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
+            "selp.u32 %0, 1, 0, p;\n\t}"
+            : "=r"(done)
+            : "r"(bar), "r"(parity)
+            : "memory");
+        if (done) return true;
+        const unsigned long long now = wall_ns();
+        if (!began) began = now;
+        else if (now - began > 2000000000ull) return false;
+    }
+    return false;
+}
+
+// Copies the 16-byte units that hold `bytes` from `src` (the units before and
+// after belong to the same allocation: they hold some of the row).
+__device__ __forceinline__ uint32_t units(uintptr_t src, uint32_t bytes) {
+    return (((uint32_t)src & 15u) + bytes + 15u) & ~15u;
+}
+__device__ __forceinline__ void copy_row(uint32_t dst, uintptr_t src, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(dst),
+                 "l"(src & ~(uintptr_t)15), "r"(units(src, bytes)), "r"(bar)
+                 : "memory");
+}
+
+// A row's place in shared memory: room for the units that hold it, and for a
+// vector that begins before or ends behind it.
+constexpr int kPad = 32;
+__host__ __device__ inline uint32_t row_room(int cols, int type) {
+    return ((uint32_t)cols * type_bytes(type) + 15 + 2 * kPad + 15) & ~15u;
+}
+
+// E vectors of V neighbours of a staged row, vector e at column col0 + e * step, as
+// fp32; zeros outside the row.  `at`: shared address of column 0.
 template <int V, int E>
-struct Row {
-    uint32_t raw[E][V];  // fp32 bits; two 16-bit values to a word while raw (V = 4), one in the low half (V = 1)
-
-    // Issues the row's loads; nothing here waits for them.
-    __device__ __forceinline__ void load(const void* base, int type, int t, int T, int cols) {
-        if (type == CIMEKV_F32) {
-            const float* p = static_cast<const float*>(base);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int col = (e * T + t) * V;
-                if (col < cols) {
-                    if constexpr (V == 4) {
-                        const uint4 v = __ldg(reinterpret_cast<const uint4*>(p + col));
-                        raw[e][0] = v.x; raw[e][1] = v.y; raw[e][2] = v.z; raw[e][3] = v.w;
-                    } else {
-                        raw[e][0] = __float_as_uint(__ldg(p + col));
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < V; ++i) raw[e][i] = 0u;
-                }
-            }
-        } else {
-            const unsigned short* p = static_cast<const unsigned short*>(base);
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int col = (e * T + t) * V;
-                if (col < cols) {
-                    if constexpr (V == 4) {
-                        const uint2 v = __ldg(reinterpret_cast<const uint2*>(p + col));
-                        raw[e][0] = v.x; raw[e][1] = v.y;
-                    } else {
-                        raw[e][0] = __ldg(p + col);
-                    }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < (V == 4 ? 2 : 1); ++i) raw[e][i] = 0u;
-                }
-            }
-        }
-    }
-
-    // Raw words to fp32 bits, in place.
-    __device__ __forceinline__ void widen(int type) {
-        if (type == CIMEKV_F32) return;
-        if (type == CIMEKV_BF16) {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if constexpr (V == 4) {
-                    const uint32_t a = raw[e][0], b = raw[e][1];
-                    raw[e][0] = a << 16; raw[e][1] = a & 0xffff0000u;
-                    raw[e][2] = b << 16; raw[e][3] = b & 0xffff0000u;
-                } else {
-                    raw[e][0] <<= 16;
-                }
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < E; ++e) {
-                if constexpr (V == 4) {
-                    const uint32_t a = raw[e][0], b = raw[e][1];
-                    raw[e][0] = half_bits(a); raw[e][1] = half_bits(a >> 16);
-                    raw[e][2] = half_bits(b); raw[e][3] = half_bits(b >> 16);
-                } else {
-                    raw[e][0] = half_bits(raw[e][0]);
-                }
-            }
-        }
-    }
-
-    static __device__ __forceinline__ uint32_t half_bits(uint32_t h) {
-        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
-    }
-    __device__ __forceinline__ float get(int e, int i) const { return __uint_as_float(raw[e][i]); }
-    __device__ __forceinline__ void set(int e, int i, float v) { raw[e][i] = __float_as_uint(v); }
-
-    // Rounds to `type` and stores; what the row then holds is not rounded.
-    __device__ __forceinline__ void store(void* base, int type, int t, int T, int cols) const {
+__device__ __forceinline__ void read_row(float (&v)[E][V], uint32_t at, int type, int col0, int step, int cols) {
+    if (type == CIMEKV_F32) {
 #pragma unroll
         for (int e = 0; e < E; ++e) {
-            const int col = (e * T + t) * V;
-            if (col >= cols) continue;
-            if (type == CIMEKV_F32) {
-                float* p = static_cast<float*>(base) + col;
-                if constexpr (V == 4) *reinterpret_cast<uint4*>(p) = make_uint4(raw[e][0], raw[e][1], raw[e][2], raw[e][3]);
-                else *p = get(e, 0);
-            } else {
-                unsigned short* p = static_cast<unsigned short*>(base) + col;
-                unsigned short s[V];
+            const int col = col0 + e * step;
+            uint32_t w[V];
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    s[i] = type == CIMEKV_BF16 ? __bfloat16_as_ushort(__float2bfloat16_rn(get(e, i)))
-                                               : __half_as_ushort(__float2half_rn(get(e, i)));
+            for (int i = 0; i < V; ++i) w[i] = 0u;
+            if (col < cols) {
+                if constexpr (V == 1) {
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(at + col * 4) : "memory");
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i += 4)
+                        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                                     : "=r"(w[i]), "=r"(w[i + 1]), "=r"(w[i + 2]), "=r"(w[i + 3])
+                                     : "r"(at + (col + i) * 4)
+                                     : "memory");
                 }
-                if constexpr (V == 4)
-                    *reinterpret_cast<uint2*>(p) = make_uint2(s[0] | (uint32_t)s[1] << 16, s[2] | (uint32_t)s[3] << 16);
-                else
-                    *p = s[0];
+            }
+            if (V > 1 && (col < 0 || col + V > cols)) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if ((unsigned)(col + i) >= (unsigned)cols) w[i] = 0u;
+            }
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[e][i] = __uint_as_float(w[i]);
+        }
+        return;
+    }
+    constexpr int kWords = (V + 1) / 2;
+    uint32_t w[E][kWords];
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int col = col0 + e * step;
+#pragma unroll
+        for (int i = 0; i < kWords; ++i) w[e][i] = 0u;
+        if (col < cols) {
+            const uint32_t from = at + col * 2;
+            if constexpr (V == 1) {
+                unsigned short h;
+                asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(from) : "memory");
+                w[e][0] = h;
+            } else if constexpr (V == 4) {
+                asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[e][0]), "=r"(w[e][1]) : "r"(from) : "memory");
+            } else {
+                asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
+                             : "=r"(w[e][0]), "=r"(w[e][1]), "=r"(w[e][2]), "=r"(w[e][3])
+                             : "r"(from)
+                             : "memory");
             }
         }
+        if (V > 1 && (col < 0 || col + V > cols)) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if ((unsigned)(col + i) >= (unsigned)cols) w[e][i / 2] &= i % 2 ? 0x0000ffffu : 0xffff0000u;
+        }
     }
-};
+    if (type == CIMEKV_BF16) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                v[e][i] = __uint_as_float(i % 2 ? w[e][i / 2] & 0xffff0000u : w[e][i / 2] << 16);
+    } else {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < V; i += 2) {
+                const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[e][i / 2]));
+                v[e][i] = f.x;
+                if (i + 1 < V) v[e][i + 1 < V ? i + 1 : i] = f.y;
+            }
+    }
+}
+
+template <bool kBf16>
+__device__ __forceinline__ uint32_t pack2(float a, float b) {
+    if (kBf16) {
+        const __nv_bfloat162 v = __floats2bfloat162_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&v);
+    }
+    const __half2 v = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&v);
+}
+
+template <int V, int E, bool kBf16>
+__device__ __forceinline__ void store_row16(const float (&v)[E][V], unsigned short* row, int col0, int step, int cols) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+        const int col = col0 + e * step;
+        unsigned short* p = row + col;
+        uint32_t w[(V + 1) / 2];
+#pragma unroll
+        for (int i = 0; i < V; i += 2) w[i / 2] = pack2<kBf16>(v[e][i], i + 1 < V ? v[e][i + 1 < V ? i + 1 : i] : 0.0f);
+        if (col >= 0 && col + V <= cols) {
+            if constexpr (V == 1) *p = (unsigned short)w[0];
+            else if constexpr (V == 4) *reinterpret_cast<uint2*>(p) = make_uint2(w[0], w[1]);
+            else *reinterpret_cast<uint4*>(p) = make_uint4(w[0], w[1], w[2], w[3]);
+        } else if (V > 1 && col < cols) {
+#pragma unroll
+            for (int i = 0; i < V; ++i)
+                if ((unsigned)(col + i) < (unsigned)cols) p[i] = (unsigned short)(w[i / 2] >> (16 * (i % 2)));
+        }
+    }
+}
+
+// Rounds to `type` and stores.
+template <int V, int E>
+__device__ __forceinline__ void store_row(const float (&v)[E][V], void* base, int type, int col0, int step, int cols) {
+    if (type == CIMEKV_F32) {
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+            const int col = col0 + e * step;
+            float* p = static_cast<float*>(base) + col;
+            if (col >= 0 && col + V <= cols) {
+                if constexpr (V == 1) {
+                    *p = v[e][0];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < V; i += 4)
+                        *reinterpret_cast<float4*>(p + i) = make_float4(v[e][i], v[e][i + 1], v[e][i + 2], v[e][i + 3]);
+                }
+            } else if (V > 1 && col < cols) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if ((unsigned)(col + i) < (unsigned)cols) p[i] = v[e][i];
+            }
+        }
+    } else if (type == CIMEKV_BF16) {
+        store_row16<V, E, true>(v, static_cast<unsigned short*>(base), col0, step, cols);
+    } else {
+        store_row16<V, E, false>(v, static_cast<unsigned short*>(base), col0, step, cols);
+    }
+}
+
+// Values as they are after rounding to `type`.
+template <int V, int E>
+__device__ __forceinline__ void round_row(float (&v)[E][V], int type) {
+    if (type == CIMEKV_BF16) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[e][i] = __bfloat162float(__float2bfloat16_rn(v[e][i]));
+    } else if (type == CIMEKV_F16) {
+#pragma unroll
+        for (int e = 0; e < E; ++e)
+#pragma unroll
+            for (int i = 0; i < V; ++i) v[e][i] = __half2float(__float2half_rn(v[e][i]));
+    }
+}
+
+// Per-column values in registers, for all rows of a thread.
+template <int V, int E>
+__device__ __forceinline__ void load_columns(float (&v)[E][V], const void* p, int type, float absent, int col0, int stride,
+                                             int cols) {
+#pragma unroll
+    for (int e = 0; e < E; ++e)
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            const int c = col0 + e * stride + i;
+            v[e][i] = absent;
+            if (p && (unsigned)c < (unsigned)cols) {
+                if (type == CIMEKV_F32) v[e][i] = __ldg(static_cast<const float*>(p) + c);
+                else if (type == CIMEKV_BF16)
+                    v[e][i] = __uint_as_float((uint32_t)__ldg(static_cast<const unsigned short*>(p) + c) << 16);
+                else v[e][i] = __half2float(__ushort_as_half(__ldg(static_cast<const unsigned short*>(p) + c)));
+            }
+        }
+}
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -157,25 +285,31 @@ __device__ __forceinline__ float warp_sum(float v) {
     return v;
 }
 
-// Sum over the W warps of a row (W == 1: the row's own warp), the same bits in
-// every thread.  `slot` alternates between two buffers, so one barrier is enough:
-// a buffer is written again only after the barrier of the sum in between.
+constexpr int kMaxWarps = 16;
+// Rows side by side in a CTA of eight warps (sixteen for the widest rows).
+__host__ __device__ constexpr int cta_warps(int W) { return W == 16 ? 16 : 8; }
+__host__ __device__ constexpr int cta_rows(int W) { return cta_warps(W) / W; }
+__host__ __device__ constexpr int cta_threads(int W) { return cta_warps(W) * 32; }
+
+// Sum over the W warps of a row, the same bits in every thread.  `slot` alternates
+// between two buffers, so one barrier of the row's warps is enough: a buffer is
+// written again only after the barrier of the sum in between.
 template <int W, int N>
-__device__ __forceinline__ void row_sum(float (&v)[N], float (*buf)[W][N], int& slot) {
+__device__ __forceinline__ void row_sum(float (&v)[N], float (*buf)[kMaxWarps][2], int& slot) {
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = warp_sum(v[i]);
     if constexpr (W > 1) {
-        float(*b)[N] = buf[slot];
+        const int warp = threadIdx.x >> 5, group = warp / W;
         if ((threadIdx.x & 31) == 0) {
 #pragma unroll
-            for (int i = 0; i < N; ++i) b[threadIdx.x >> 5][i] = v[i];
+            for (int i = 0; i < N; ++i) buf[slot][warp][i] = v[i];
         }
-        __syncthreads();
+        asm volatile("bar.sync %0, %1;" ::"r"(group + 1), "n"(W * 32) : "memory");
 #pragma unroll
         for (int i = 0; i < N; ++i) {
             float s = 0.0f;
 #pragma unroll
-            for (int w = 0; w < W; ++w) s += b[w][i];
+            for (int w = 0; w < W; ++w) s += buf[slot][group * W + w][i];
             v[i] = s;
         }
         slot ^= 1;
@@ -198,188 +332,282 @@ struct NormParams {
     float* part;
     long long rows, x_stride, d_stride, dy_stride, dh_stride;
     int cols, x_type, d_type, w_type, y_type;
+    int stages;  // rows under way per row group
+    int places;  // row r begins r * places mod V elements into a vector (the strides mod V)
     float eps;
 };
 
-__device__ __forceinline__ const void* row_of(const void* p, int type, long long row, long long stride) {
-    return static_cast<const char*>(p) + row * stride * type_bytes(type);
-}
 __device__ __forceinline__ void* row_of(void* p, int type, long long row, long long stride) {
     return static_cast<char*>(p) + row * stride * type_bytes(type);
 }
 
-// Threads of a CTA: one row per CTA above one warp per row, eight rows below.
-__host__ __device__ constexpr int cta_threads(int W) { return W == 1 ? 256 : W * 32; }
-__host__ __device__ constexpr int cta_rows(int W) { return W == 1 ? 8 : 1; }
+constexpr int kMaxStages = 4;
+
+// The rows of one row group on their way through shared memory: up to three
+// tensors a row.  One thread of the group copies, all read.
+template <int W, int N>
+struct Ring {
+    uintptr_t next[N];          // address of the row to copy next
+    long long step[N];          // bytes from one of the group's rows to the next
+    uint32_t low[N];            // low bits of the current row's address
+    uint32_t bytes[N], room[N], memory, at_stage, bars, stage_bytes;
+    int stages, stage, phase, lost;
+    bool ok;
+
+    __device__ __forceinline__ void tensor(int k, const void* base, int type, long long stride, long long row, long long rows_apart,
+                                           int cols) {
+        const int size = type_bytes(type);
+        next[k] = (uintptr_t)base + row * stride * size;
+        low[k] = (uint32_t)next[k];
+        step[k] = rows_apart * stride * size;
+        bytes[k] = (uint32_t)cols * size;
+        room[k] = row_room(cols, type);
+    }
+    // `memory_`: of the CTA; `bars_`: the group's kMaxStages barriers.  All threads of
+    // the CTA, after its tensors.
+    __device__ __forceinline__ void open(uint32_t memory_, uint32_t bars_, int stages_) {
+        stages = stages_;
+        stage_bytes = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) stage_bytes += room[k];
+        at_stage = memory = memory_ + threadIdx.x / (W * 32) * stages * stage_bytes;
+        bars = bars_;
+        stage = phase = lost = 0;
+        ok = true;
+        if (threadIdx.x % (W * 32) == 0) {
+            for (int s = 0; s < kMaxStages; ++s)
+                asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(bars + 8 * s) : "memory");
+            asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        }
+        __syncthreads();
+    }
+    // The group's next row into `place`, by the copying thread.
+    __device__ __forceinline__ void copy(int place) {
+        uint32_t total = 0;
+#pragma unroll
+        for (int k = 0; k < N; ++k) total += units(next[k], bytes[k]);
+        const uint32_t bar = bars + 8 * place;
+        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(total) : "memory");
+        uint32_t dst = memory + place * stage_bytes + kPad;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            copy_row(dst, next[k], bytes[k], bar);
+            dst += room[k];
+            next[k] += step[k];
+        }
+    }
+    // The next row of the group is in shared memory.  After a wait that ran out
+    // no row is copied any more; those under way are still waited for.
+    __device__ __forceinline__ void wait() {
+        if (lost == stages) return;
+        ok = mbar_wait(bars + 8 * stage, phase) && ok;
+        if (!ok) ++lost;
+    }
+    // Shared address of column 0 of tensor k of the current row.
+    __device__ __forceinline__ uint32_t at(int k) const {
+        uint32_t a = at_stage + kPad + (low[k] & 15u);
+#pragma unroll
+        for (int i = 0; i < N; ++i)
+            if (i < k) a += room[i];
+        return a;
+    }
+    // After all threads of the group have read the current row (and met): its
+    // place takes another one, if there is one.
+    __device__ __forceinline__ void take(bool more) {
+        if (threadIdx.x % (W * 32) == 0 && more && ok) copy(stage);
+#pragma unroll
+        for (int k = 0; k < N; ++k) low[k] += (uint32_t)step[k];
+        at_stage += stage_bytes;
+        if (++stage == stages) {
+            stage = 0;
+            at_stage = memory;
+            phase ^= 1;
+        }
+    }
+};
+
+// s / n to the last bit or so, by a reciprocal taken once.
+__device__ __forceinline__ float divide(float s, float n, float inv) {
+    const float q = s * inv;
+    return fmaf(fmaf(-q, n, s), inv, q);
+}
+
+// All threads of a row's warps meet.
+template <int W>
+__device__ __forceinline__ void row_sync() {
+    if constexpr (W == 1) __syncwarp();
+    else asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / (W * 32) + 1), "n"(W * 32) : "memory");
+}
 
 template <int V, int E, int W, bool kDelta>
 __global__ void __launch_bounds__(cta_threads(W)) norm_fwd_kernel(NormParams p) {
-    constexpr int T = W * 32;
-    __shared__ float red[2][W][1];
+    constexpr int T = W * 32, kStep = T * V, N = kDelta ? 2 : 1;
+    extern __shared__ __align__(16) uint8_t memory[];
+    __shared__ __align__(8) uint64_t bars[cta_rows(W)][kMaxStages];
+    __shared__ float red[2][kMaxWarps][2];
     int slot = 0;
-    const int t = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const long long first = W == 1 ? (long long)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
-    for (long long row = first; row < p.rows; row += (long long)gridDim.x * cta_rows(W)) {
-        Row<V, E> h;
-        h.load(row_of(p.x, p.x_type, row, p.x_stride), p.x_type, t, T, p.cols);
+    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    long long row = (long long)blockIdx.x * cta_rows(W) + group;
+    const long long step = (long long)gridDim.x * cta_rows(W);
+    const int col0 = t * V - (int)((unsigned)row * (unsigned)p.places % V);
+    const float n = (float)p.cols, inv = 1.0f / n;
+    Ring<W, N> ring;
+    ring.tensor(0, p.x, p.x_type, p.x_stride, row, step, p.cols);
+    if constexpr (kDelta) ring.tensor(1, p.d, p.d_type, p.d_stride, row, step, p.cols);
+    ring.open(smem_addr(memory), smem_addr(bars[group]), p.stages);
+    if (row >= p.rows) return;  // whole groups of warps
+    if (t == 0)
+        for (int s = 0; s < p.stages && row + s * step < p.rows; ++s) ring.copy(s);
+    float w[E][V], b[E][V];
+    load_columns(w, p.w, p.w_type, 1.0f, col0, kStep, p.cols);
+    load_columns(b, p.b, p.w_type, 0.0f, col0, kStep, p.cols);
+    for (; row < p.rows; row += step) {
+        float h[E][V];
+        ring.wait();
+        read_row<V, E>(h, ring.at(0), p.x_type, col0, kStep, p.cols);
         if constexpr (kDelta) {
-            Row<V, E> d;
-            d.load(row_of(p.d, p.d_type, row, p.d_stride), p.d_type, t, T, p.cols);
-            h.widen(p.x_type);
-            d.widen(p.d_type);
+            float d[E][V];
+            read_row<V, E>(d, ring.at(1), p.d_type, col0, kStep, p.cols);
 #pragma unroll
             for (int e = 0; e < E; ++e)
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    float s = h.get(e, i) + d.get(e, i);
-                    // y is the norm of the sum as it is held (and as the backward reads it)
-                    if (p.x_type == CIMEKV_BF16) s = __bfloat162float(__float2bfloat16_rn(s));
-                    else if (p.x_type == CIMEKV_F16) s = __half2float(__float2half_rn(s));
-                    h.set(e, i, s);
-                }
-            h.store(row_of(p.h, p.x_type, row, p.cols), p.x_type, t, T, p.cols);
-        } else {
-            h.widen(p.x_type);
+                for (int i = 0; i < V; ++i) h[e][i] += d[e][i];
+            store_row<V, E>(h, row_of(p.h, p.x_type, row, p.cols), p.x_type, col0, kStep, p.cols);
+            // y is the norm of the sum as it is held (and as the backward reads it)
+            round_row<V, E>(h, p.x_type);
         }
         float s[1] = {0.0f};
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int i = 0; i < V; ++i) s[0] += h.get(e, i);
+            for (int i = 0; i < V; ++i) s[0] += h[e][i];
         row_sum<W, 1>(s, red, slot);
-        const float mean = s[0] / (float)p.cols;
+        if (W == 1) __syncwarp();
+        ring.take(row + p.stages * step < p.rows);  // the sum was taken by all: all have read
+        const float mean = ring.ok ? divide(s[0], n, inv) : __int_as_float(0x7fffffff);  // a lost copy shows as NaN
         float q[1] = {0.0f};
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-            if ((e * T + t) * V < p.cols) {
+        for (int e = 0; e < E; ++e) {
+            const int col = col0 + e * kStep;
 #pragma unroll
-                for (int i = 0; i < V; ++i) {
-                    const float c = h.get(e, i) - mean;
-                    h.set(e, i, c);
-                    q[0] = fmaf(c, c, q[0]);
-                }
+            for (int i = 0; i < V; ++i) h[e][i] -= mean;
+            if (col < 0 || col + V > p.cols) {
+#pragma unroll
+                for (int i = 0; i < V; ++i)
+                    if ((unsigned)(col + i) >= (unsigned)p.cols) h[e][i] = 0.0f;
             }
+#pragma unroll
+            for (int i = 0; i < V; ++i) {
+                q[0] = fmaf(h[e][i], h[e][i], q[0]);
+            }
+        }
         row_sum<W, 1>(q, red, slot);
-        const float rstd = rsqrtf(q[0] / (float)p.cols + p.eps);
+        const float rstd = rsqrtf(divide(q[0], n, inv) + p.eps);
         if (t == 0 && p.mean) {
             p.mean[row] = mean;
             p.rstd[row] = rstd;
         }
-        Row<V, E> w;
-        if (p.w) {
-            w.load(p.w, p.w_type, t, T, p.cols);
-            w.widen(p.w_type);
-        }
 #pragma unroll
         for (int e = 0; e < E; ++e)
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float u = h.get(e, i) * rstd;
-                h.set(e, i, p.w ? u * w.get(e, i) : u);
-            }
-        if (p.b) {
-            w.load(p.b, p.w_type, t, T, p.cols);
-            w.widen(p.w_type);
-#pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < V; ++i) h.set(e, i, h.get(e, i) + w.get(e, i));
-        }
-        h.store(row_of(p.y, p.y_type, row, p.cols), p.y_type, t, T, p.cols);
+            for (int i = 0; i < V; ++i) h[e][i] = h[e][i] * rstd * w[e][i] + b[e][i];
+        store_row<V, E>(h, row_of(p.y, p.y_type, row, p.cols), p.y_type, col0, kStep, p.cols);
     }
 }
 
 // kSum: the sum's own gradient dh is added to dx.  p.part: the CTA's column sums
 // [gridDim][2][cols] (dw, db), or null when no weight gradient is wanted.
 template <int V, int E, int W, bool kSum>
-__global__ void __launch_bounds__(cta_threads(W)) norm_bwd_kernel(NormParams p) {
-    constexpr int T = W * 32;
-    __shared__ float red[2][W][2];
+__global__ void __launch_bounds__(cta_threads(W), W == 16 ? 1 : 2) norm_bwd_kernel(NormParams p) {
+    constexpr int T = W * 32, kStep = T * V, N = kSum ? 3 : 2;
+    extern __shared__ __align__(16) uint8_t memory[];
+    __shared__ __align__(8) uint64_t bars[cta_rows(W)][kMaxStages];
+    __shared__ float red[2][kMaxWarps][2];
     int slot = 0;
-    const int t = W == 1 ? (threadIdx.x & 31) : threadIdx.x;
-    const long long first = W == 1 ? (long long)blockIdx.x * 8 + (threadIdx.x >> 5) : blockIdx.x;
+    const int t = threadIdx.x % T, group = threadIdx.x / T;
+    long long row = (long long)blockIdx.x * cta_rows(W) + group;
+    const long long step = (long long)gridDim.x * cta_rows(W);
+    const int col0 = t * V - (int)((unsigned)row * (unsigned)p.places % V);
+    const float n = (float)p.cols, inv = 1.0f / n;
+    Ring<W, N> ring;
+    ring.tensor(0, p.x, p.x_type, p.x_stride, row, step, p.cols);
+    ring.tensor(1, p.dy, p.y_type, p.dy_stride, row, step, p.cols);
+    if constexpr (kSum) ring.tensor(2, p.dh, p.x_type, p.dh_stride, row, step, p.cols);
+    ring.open(smem_addr(memory), smem_addr(bars[group]), p.stages);
     float dw[E][V] = {}, db[E][V] = {};
-    for (long long row = first; row < p.rows; row += (long long)gridDim.x * cta_rows(W)) {
-        Row<V, E> u, g, a;
-        u.load(row_of(p.x, p.x_type, row, p.x_stride), p.x_type, t, T, p.cols);
-        g.load(row_of(p.dy, p.y_type, row, p.dy_stride), p.y_type, t, T, p.cols);
-        if constexpr (kSum) a.load(row_of(p.dh, p.x_type, row, p.dh_stride), p.x_type, t, T, p.cols);
-        const float mean = __ldg(p.mean + row), rstd = __ldg(p.rstd + row);
-        u.widen(p.x_type);
-        g.widen(p.y_type);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const bool in = (e * T + t) * V < p.cols;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float v = in ? (u.get(e, i) - mean) * rstd : 0.0f;
-                u.set(e, i, v);
-                dw[e][i] = fmaf(g.get(e, i), v, dw[e][i]);
-                db[e][i] += g.get(e, i);
+    if (row < p.rows) {
+        if (t == 0)
+            for (int s = 0; s < p.stages && row + s * step < p.rows; ++s) ring.copy(s);
+        float w[E][V];
+        load_columns(w, p.w, p.w_type, 1.0f, col0, kStep, p.cols);
+        float next_mean = __ldg(p.mean + row), next_rstd = __ldg(p.rstd + row);
+        for (; row < p.rows; row += step) {
+            const float mean = next_mean, rstd = next_rstd;
+            if (row + step < p.rows) {
+                next_mean = __ldg(p.mean + row + step);
+                next_rstd = __ldg(p.rstd + row + step);
             }
-        }
-        if (p.w) {
-            Row<V, E> w;
-            w.load(p.w, p.w_type, t, T, p.cols);
-            w.widen(p.w_type);
+            float u[E][V], g[E][V];
+            ring.wait();
+            read_row<V, E>(u, ring.at(0), p.x_type, col0, kStep, p.cols);
+            read_row<V, E>(g, ring.at(1), p.y_type, col0, kStep, p.cols);
+            float s[2] = {0.0f, 0.0f};
 #pragma unroll
             for (int e = 0; e < E; ++e)
 #pragma unroll
-                for (int i = 0; i < V; ++i) g.set(e, i, g.get(e, i) * w.get(e, i));
+                for (int i = 0; i < V; ++i) {  // outside the row g is zero, and u only meets g
+                    u[e][i] = (u[e][i] - mean) * rstd;
+                    dw[e][i] = fmaf(g[e][i], u[e][i], dw[e][i]);
+                    db[e][i] += g[e][i];
+                    g[e][i] *= w[e][i];
+                    s[0] += g[e][i];
+                    s[1] = fmaf(g[e][i], u[e][i], s[1]);
+                }
+            row_sum<W, 2>(s, red, slot);
+            const float scale = ring.ok ? rstd : __int_as_float(0x7fffffff);  // a lost copy shows as NaN
+            const float c1 = scale * divide(s[0], n, inv), c2 = scale * divide(s[1], n, inv);
+#pragma unroll
+            for (int e = 0; e < E; ++e)
+#pragma unroll
+                for (int i = 0; i < V; ++i) g[e][i] = fmaf(scale, g[e][i], -fmaf(c2, u[e][i], c1));
+            if constexpr (kSum) {
+                read_row<V, E>(u, ring.at(2), p.x_type, col0, kStep, p.cols);
+#pragma unroll
+                for (int e = 0; e < E; ++e)
+#pragma unroll
+                    for (int i = 0; i < V; ++i) g[e][i] += u[e][i];
+            }
+            if (kSum || W == 1) row_sync<W>();
+            ring.take(row + p.stages * step < p.rows);
+            if (p.dx) store_row<V, E>(g, row_of(p.dx, p.x_type, row, p.cols), p.x_type, col0, kStep, p.cols);
+            if (p.dd) store_row<V, E>(g, row_of(p.dd, p.d_type, row, p.cols), p.d_type, col0, kStep, p.cols);
         }
-        float s[2] = {0.0f, 0.0f};
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                s[0] += g.get(e, i);
-                s[1] = fmaf(g.get(e, i), u.get(e, i), s[1]);
-            }
-        row_sum<W, 2>(s, red, slot);
-        const float c1 = s[0] / (float)p.cols, c2 = s[1] / (float)p.cols;
-        if constexpr (kSum) a.widen(p.x_type);
-#pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                const float v = rstd * (g.get(e, i) - c1 - u.get(e, i) * c2);
-                g.set(e, i, kSum ? v + a.get(e, i) : v);
-            }
-        if (p.dx) g.store(row_of(p.dx, p.x_type, row, p.cols), p.x_type, t, T, p.cols);
-        if (p.dd) g.store(row_of(p.dd, p.d_type, row, p.cols), p.d_type, t, T, p.cols);
+        if (!ring.ok) dw[0][0] = db[0][0] = __int_as_float(0x7fffffff);
     }
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (!p.part) return;
+    // [2][cols] where row groups share a CTA, over the rows' places once all are taken
+    float* join = reinterpret_cast<float*>(memory);
     float* out = p.part + (long long)blockIdx.x * 2 * p.cols;
-    if constexpr (W == 1) {
-        // join the eight warps' sums, one array after the other
-        __shared__ float join[8][T * V * E];
-        for (int k = 0; k < 2; ++k) {
-            __syncthreads();
+    float* to = cta_rows(W) > 1 ? join : out;
+    __syncthreads();
+    for (int g = 0; g < cta_rows(W); ++g) {  // one row group after the other: a fixed order
+        if (group == g) {
 #pragma unroll
             for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < V; ++i) join[threadIdx.x >> 5][(e * T + t) * V + i] = k ? db[e][i] : dw[e][i];
-            __syncthreads();
-            for (int c = threadIdx.x; c < p.cols; c += 256) {
-                float s = 0.0f;
-#pragma unroll
-                for (int w = 0; w < 8; ++w) s += join[w][c];
-                out[k * p.cols + c] = s;
-            }
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int col = (e * T + t) * V;
-            if (col < p.cols) {
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
-                    out[col + i] = dw[e][i];
-                    out[p.cols + col + i] = db[e][i];
+                    const int c = col0 + e * kStep + i;
+                    if ((unsigned)c < (unsigned)p.cols) {
+                        to[c] = g ? to[c] + dw[e][i] : dw[e][i];
+                        to[p.cols + c] = g ? to[p.cols + c] + db[e][i] : db[e][i];
+                    }
                 }
-            }
         }
+        if (cta_rows(W) > 1) __syncthreads();
     }
+    if (cta_rows(W) > 1)
+        for (int c = threadIdx.x; c < 2 * p.cols; c += cta_threads(W)) out[c] = join[c];
 }
 
 // dw / db (blockIdx.y) of 32 columns: kReduceLanes partial rows side by side,
@@ -389,10 +617,12 @@ __global__ void __launch_bounds__(32 * kReduceLanes) norm_cols_kernel(const floa
     __shared__ float s[kReduceLanes][33];
     void* out = blockIdx.y ? db : dw;
     if (!out) return;
+    asm volatile("griddepcontrol.wait;" ::: "memory");
     const int c = blockIdx.x * 32 + threadIdx.x;
     float v = 0.0f;
     if (c < cols) {
         const float* src = part + (long long)blockIdx.y * cols + c;
+#pragma unroll 8
         for (int r = threadIdx.y; r < nparts; r += kReduceLanes) v += src[(long long)r * 2 * cols];
     }
     s[threadIdx.y][threadIdx.x] = v;
@@ -410,40 +640,49 @@ __global__ void __launch_bounds__(32 * kReduceLanes) norm_cols_kernel(const floa
 
 struct Shape {
     int v, e, w;
+    constexpr int capacity() const { return v * e * w * 32; }
 };
 
-// Row layout by width: the smallest of these that holds the row.  Vectors of
-// four need widths, strides and addresses that are multiples of four elements.
-constexpr Shape kShapes[] = {{4, 1, 1}, {4, 2, 1}, {4, 3, 1}, {4, 4, 1},  {4, 6, 1},  {4, 8, 1},  {4, 4, 4},
-                             {4, 4, 8}, {4, 8, 8}, {4, 8, 16}, {1, 8, 1}, {1, 32, 1}, {1, 16, 8}, {1, 32, 16}};
+// Layouts of a row by width, for vectors of 4 (fp32 rows), of 8 (16-bit rows) and
+// single elements (strides or addresses that no vector fits): the first that
+// holds the row is taken.
+constexpr Shape kShapes[] = {{4, 1, 1}, {4, 2, 1}, {4, 3, 1}, {4, 4, 1}, {4, 3, 2}, {4, 4, 2}, {4, 4, 4}, {4, 4, 8},
+                             {4, 4, 16}, {4, 8, 16},
+                             {8, 1, 1}, {8, 2, 1}, {8, 2, 2}, {8, 2, 4}, {8, 2, 8}, {8, 2, 16}, {8, 4, 16},
+                             {1, 8, 1}, {1, 8, 4}, {1, 16, 8}, {1, 32, 16}};
 constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
 
-int pick_shape(int cols, bool vec) {
-    for (int i = 0; i < kNumShapes; ++i) {
-        const Shape s = kShapes[i];
-        if ((s.v == 4) == vec && s.v * s.e * s.w * 32 >= cols) return i;
-    }
-    return kNumShapes - 1;
+int pick_shape(int cols, int v) {
+    for (int i = 0; i < kNumShapes; ++i)
+        // rows that begin inside a vector need room for one more
+        if (kShapes[i].v == v && kShapes[i].capacity() >= cols + (cols % v ? v - 1 : 0)) return i;
+    return -1;
 }
 
 using Kernel = void (*)(NormParams);
-
+struct Kernels {
+    Kernel fwd[2], bwd[2];  // without and with a branch / a gradient of the sum
+};
 template <int I>
-constexpr Kernel fwd_of(bool delta) {
+constexpr Kernels kernels_of() {
     constexpr Shape s = kShapes[I];
-    return delta ? (Kernel)norm_fwd_kernel<s.v, s.e, s.w, true> : (Kernel)norm_fwd_kernel<s.v, s.e, s.w, false>;
+    return {{norm_fwd_kernel<s.v, s.e, s.w, false>, norm_fwd_kernel<s.v, s.e, s.w, true>},
+            {norm_bwd_kernel<s.v, s.e, s.w, false>, norm_bwd_kernel<s.v, s.e, s.w, true>}};
 }
-template <int I>
-constexpr Kernel bwd_of(bool sum) {
-    constexpr Shape s = kShapes[I];
-    return sum ? (Kernel)norm_bwd_kernel<s.v, s.e, s.w, true> : (Kernel)norm_bwd_kernel<s.v, s.e, s.w, false>;
+template <int... I>
+const Kernels& kernels(int i, std::integer_sequence<int, I...>) {
+    static const Kernels table[] = {kernels_of<I>()...};
+    return table[i];
 }
+const Kernels& kernels(int i) { return kernels(i, std::make_integer_sequence<int, kNumShapes>()); }
 
-#define CIMEKV_NORM_TABLE(F, flag) \
-    {F<0>(flag), F<1>(flag), F<2>(flag), F<3>(flag), F<4>(flag), F<5>(flag), F<6>(flag), \
-     F<7>(flag), F<8>(flag), F<9>(flag), F<10>(flag), F<11>(flag), F<12>(flag), F<13>(flag)}
-const Kernel kFwd[2][kNumShapes] = {CIMEKV_NORM_TABLE(fwd_of, false), CIMEKV_NORM_TABLE(fwd_of, true)};
-const Kernel kBwd[2][kNumShapes] = {CIMEKV_NORM_TABLE(bwd_of, false), CIMEKV_NORM_TABLE(bwd_of, true)};
+// Rows under way per row group: as many as fit a share of shared memory that
+// leaves room for two CTAs per SM (one for the widest rows), at most four.
+int ring_stages(const Shape& s, size_t row_bytes) {
+    const size_t share = s.w == 16 ? 200 << 10 : 100 << 10;
+    const size_t n = share / (row_bytes * cta_rows(s.w));
+    return n > kMaxStages ? kMaxStages : n < 1 ? 1 : (int)n;
+}
 
 int sm_count(int* sms) {
     int dev;
@@ -453,21 +692,46 @@ int sm_count(int* sms) {
     return CIMEKV_OK;
 }
 
-// CTAs per SM that the row loops are spread over (both directions keep at least
-// this many resident).
-int ctas_per_sm(const Shape& s) { return s.w == 1 ? 4 : s.w == 4 ? 8 : s.w == 8 ? 4 : 2; }
-
+// CTAs of a launch: two to an SM (one of sixteen warps); a multiple of V, so that a
+// group's rows all begin at the same place of a vector.
 long long grid_size(long long rows, const Shape& s, int sms) {
     const long long need = (rows + cta_rows(s.w) - 1) / cta_rows(s.w);
-    const long long most = (long long)sms * ctas_per_sm(s);
-    return need < most ? need : most;
+    const long long most = (long long)sms * (s.w == 16 ? 1 : 2);
+    return ((need < most ? need : most) + s.v - 1) / s.v * s.v;
 }
 
 bool valid_type(int t) { return t == CIMEKV_F32 || t == CIMEKV_BF16 || t == CIMEKV_F16; }
 
-// Whether rows of `p` can be moved in vectors of four elements.
-bool vec_ok(const void* p, int type, long long stride) {
-    return !p || (((uintptr_t)p % (4 * (size_t)type_bytes(type))) == 0 && stride % 4 == 0);
+// One tensor of a call: address, type, row stride.
+struct Tensor {
+    const void* p;
+    int type;
+    long long stride;
+};
+
+// Elements per vector that all tensors' rows allow: 4 or 8 when every address is a
+// multiple of it and all rows begin at the same places, else 1.  places: how
+// far a row's beginning moves in a vector from row to row.
+int vector_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* places) {
+    const int v = x_type == CIMEKV_F32 ? 4 : 8;
+    *places = -1;
+    for (const Tensor& t : ts) {
+        if (!t.p) continue;
+        const int here = (int)(t.stride % v);
+        if ((uintptr_t)t.p % ((size_t)v * type_bytes(t.type)) != 0 || (*places >= 0 && *places != here)) {
+            *places = 0;
+            return 1;
+        }
+        *places = here;
+    }
+    if (*places < 0) *places = 0;
+    return pick_shape(cols, v) < 0 ? 1 : v;  // the widest rows that do not begin on vectors
+}
+
+int allow_smem(const void* kernel, size_t bytes) {
+    if (bytes <= (48 << 10)) return CIMEKV_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return e == cudaSuccess ? CIMEKV_OK : fail(CIMEKV_ECUDA, cudaGetErrorString(e));
 }
 
 int check_sizes(long long rows, int cols) {
@@ -504,11 +768,10 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
     if (!x || !y || (delta != nullptr) != (h != nullptr) || (mean != nullptr) != (rstd != nullptr))
         return fail(CIMEKV_EINVAL_SHAPE, "null pointer");
     if (x_stride < 0 || delta_stride < 0) return fail(CIMEKV_EINVAL_SHAPE, "negative stride");
-    const bool vec = cols % 4 == 0 && vec_ok(x, x_type, x_stride) && vec_ok(delta, delta_type, delta_stride) &&
-                     vec_ok(h, x_type, cols) && vec_ok(y, y_type, cols) && vec_ok(weight, w_type, 0) &&
-                     vec_ok(bias, w_type, 0);
-    const int i = pick_shape(cols, vec);
-    int sms;
+    int places, sms;
+    const int v = vector_of(x_type, cols, {{x, x_type, x_stride}, {delta, delta_type, delta_stride}, {h, x_type, cols}, {y, y_type, cols}},
+                            &places);
+    const int i = pick_shape(cols, v);
     if ((rc = sm_count(&sms))) return rc;
     NormParams p = {};
     p.x = x;
@@ -527,10 +790,15 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
     p.d_type = delta_type;
     p.w_type = w_type;
     p.y_type = y_type;
+    p.places = places;
     p.eps = eps;
     if ((rc = cimekv_internal_no_pending_error())) return rc;
-    kFwd[delta != nullptr][i]<<<(unsigned)grid_size(rows, kShapes[i], sms), cta_threads(kShapes[i].w), 0,
-                                (cudaStream_t)stream>>>(p);
+    const size_t row_bytes = row_room(cols, x_type) + (delta ? row_room(cols, delta_type) : 0);
+    p.stages = ring_stages(kShapes[i], row_bytes);
+    const Kernel kernel = kernels(i).fwd[delta != nullptr];
+    const size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
+    if ((rc = allow_smem((const void*)kernel, smem))) return rc;
+    kernel<<<(unsigned)grid_size(rows, kShapes[i], sms), cta_threads(kShapes[i].w), smem, (cudaStream_t)stream>>>(p);
     return launched("norm_fwd_kernel");
 }
 
@@ -541,8 +809,9 @@ extern "C" size_t cimekv_layer_norm_workspace_bytes(long long rows, int cols) {
     int sms;
     if (sm_count(&sms)) return 0;
     long long most = 0;
-    for (const bool vec : {false, true}) {
-        const long long g = grid_size(rows, kShapes[pick_shape(cols, vec)], sms);
+    for (const int v : {1, 4, 8}) {
+        const int i = pick_shape(cols, v);
+        const long long g = i < 0 ? 0 : grid_size(rows, kShapes[i], sms);
         if (g > most) most = g;
     }
     return (size_t)most * 2 * (size_t)cols * sizeof(float);
@@ -565,12 +834,11 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
     cudaStream_t s = (cudaStream_t)stream;
     int nparts = 0;
     if (rows > 0) {
-        const bool vec = cols % 4 == 0 && vec_ok(h, x_type, h_stride) && vec_ok(dy, y_type, dy_stride) &&
-                         vec_ok(dh, x_type, dh_stride) && vec_ok(dx, x_type, cols) &&
-                         vec_ok(ddelta, delta_type, cols) && vec_ok(weight, w_type, 0);
-        const int i = pick_shape(cols, vec);
-        int sms;
-        if ((rc = sm_count(&sms))) return rc;
+        int places, sms;
+        const int v = vector_of(x_type, cols, {{h, x_type, h_stride}, {dy, y_type, dy_stride}, {dh, x_type, dh_stride},
+                                         {dx, x_type, cols}, {ddelta, delta_type, cols}}, &places);
+        const int i = pick_shape(cols, v);
+            if ((rc = sm_count(&sms))) return rc;
         const long long grid = grid_size(rows, kShapes[i], sms);
         if (want_w) {
             if (!workspace || workspace_bytes < (size_t)grid * 2 * cols * sizeof(float))
@@ -596,8 +864,14 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
         p.d_type = delta_type;
         p.w_type = w_type;
         p.y_type = y_type;
-        if ((rc = cimekv_internal_no_pending_error())) return rc;
-        kBwd[dh != nullptr][i]<<<(unsigned)grid, cta_threads(kShapes[i].w), 0, s>>>(p);
+        p.places = places;
+        const size_t row_bytes = row_room(cols, y_type) + (dh ? 2 : 1) * (size_t)row_room(cols, x_type);
+        p.stages = ring_stages(kShapes[i], row_bytes);
+        const Kernel kernel = kernels(i).bwd[dh != nullptr];
+        size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
+        if (cta_rows(kShapes[i].w) > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
+        if ((rc = cimekv_internal_no_pending_error()) || (rc = allow_smem((const void*)kernel, smem))) return rc;
+        kernel<<<(unsigned)grid, cta_threads(kShapes[i].w), smem, s>>>(p);
         if ((rc = launched("norm_bwd_kernel"))) return rc;
         nparts = (int)grid;
     } else if ((rc = cimekv_internal_no_pending_error())) {
@@ -605,7 +879,18 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
     }
     if (!want_w) return CIMEKV_OK;
     // no rows: the sums over none of them are zero
-    norm_cols_kernel<<<dim3((unsigned)(cols + 31) / 32, 2), dim3(32, kReduceLanes), 0, s>>>(
-        static_cast<const float*>(workspace), nparts, cols, dw, db, w_type);
-    return launched("norm_cols_kernel");
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(cols + 31) / 32, 2);
+    cfg.blockDim = dim3(32, kReduceLanes);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;  // set up while the rows finish
+    attr[0].val.programmaticStreamSerializationAllowed = rows > 0;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, norm_cols_kernel, static_cast<const float*>(workspace), nparts, cols, dw,
+                                             db, w_type);
+    if (e == cudaSuccess) return CIMEKV_OK;
+    (void)cudaGetLastError();
+    return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
 }
