@@ -279,6 +279,47 @@ __device__ __forceinline__ void load_columns(float (&v)[E][V], const void* p, in
         }
 }
 
+// Two fp32 operations in one instruction (the same roundings as one by one); both
+// directions issue at 60 % without, and most of what they issue is this.
+struct Pair {
+    float x, y;
+};
+__device__ __forceinline__ Pair both(float v) { return {v, v}; }
+__device__ __forceinline__ Pair add2(Pair a, Pair b) {
+    Pair d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ Pair mul2(Pair a, Pair b) {
+    Pair d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmul.rn.f32x2 d, a, b;\n\t"
+        "mov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+__device__ __forceinline__ Pair fma2(Pair a, Pair b, Pair c) {
+    Pair d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+// Elements 2 k and 2 k + 1 of a thread (the number of its elements is even).
+template <int V, int E>
+__device__ __forceinline__ Pair get2(const float (&v)[E][V], int k) {
+    return {v[2 * k / V][2 * k % V], v[(2 * k + 1) / V][(2 * k + 1) % V]};
+}
+template <int V, int E>
+__device__ __forceinline__ void set2(float (&v)[E][V], int k, Pair p) {
+    v[2 * k / V][2 * k % V] = p.x;
+    v[(2 * k + 1) / V][(2 * k + 1) % V] = p.y;
+}
+
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
     for (int o = 16; o; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
@@ -469,38 +510,35 @@ __global__ void __launch_bounds__(cta_threads(W)) norm_fwd_kernel(NormParams p) 
             float d[E][V];
             read_row<V, E>(d, ring.at(1), p.d_type, col0, kStep, p.cols);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < V; ++i) h[e][i] += d[e][i];
+            for (int k = 0; k < E * V / 2; ++k) set2(h, k, add2(get2(h, k), get2(d, k)));
             store_row<V, E>(h, row_of(p.h, p.x_type, row, p.cols), p.x_type, col0, kStep, p.cols);
             // y is the norm of the sum as it is held (and as the backward reads it)
             round_row<V, E>(h, p.x_type);
         }
-        float s[1] = {0.0f};
+        Pair sum = both(0.0f);
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < V; ++i) s[0] += h[e][i];
+        for (int k = 0; k < E * V / 2; ++k) sum = add2(sum, get2(h, k));
+        float s[1] = {sum.x + sum.y};
         row_sum<W, 1>(s, red, slot);
         if (W == 1) __syncwarp();
         ring.take(row + p.stages * step < p.rows);  // the sum was taken by all: all have read
         const float mean = ring.ok ? divide(s[0], n, inv) : __int_as_float(0x7fffffff);  // a lost copy shows as NaN
-        float q[1] = {0.0f};
+        const Pair minus = both(-mean);
+#pragma unroll
+        for (int k = 0; k < E * V / 2; ++k) set2(h, k, add2(get2(h, k), minus));
 #pragma unroll
         for (int e = 0; e < E; ++e) {
             const int col = col0 + e * kStep;
-#pragma unroll
-            for (int i = 0; i < V; ++i) h[e][i] -= mean;
             if (col < 0 || col + V > p.cols) {
 #pragma unroll
                 for (int i = 0; i < V; ++i)
                     if ((unsigned)(col + i) >= (unsigned)p.cols) h[e][i] = 0.0f;
             }
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                q[0] = fmaf(h[e][i], h[e][i], q[0]);
-            }
         }
+        Pair squares = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < E * V / 2; ++k) squares = fma2(get2(h, k), get2(h, k), squares);
+        float q[1] = {squares.x + squares.y};
         row_sum<W, 1>(q, red, slot);
         const float rstd = rsqrtf(divide(q[0], n, inv) + p.eps);
         if (t == 0 && p.mean) {
@@ -508,9 +546,8 @@ __global__ void __launch_bounds__(cta_threads(W)) norm_fwd_kernel(NormParams p) 
             p.rstd[row] = rstd;
         }
 #pragma unroll
-        for (int e = 0; e < E; ++e)
-#pragma unroll
-            for (int i = 0; i < V; ++i) h[e][i] = h[e][i] * rstd * w[e][i] + b[e][i];
+        for (int k = 0; k < E * V / 2; ++k)
+            set2(h, k, fma2(mul2(get2(h, k), both(rstd)), get2(w, k), get2(b, k)));
         store_row<V, E>(h, row_of(p.y, p.y_type, row, p.cols), p.y_type, col0, kStep, p.cols);
     }
 }
@@ -551,31 +588,30 @@ __global__ void __launch_bounds__(cta_threads(W), W == 16 ? 1 : 2) norm_bwd_kern
             ring.wait();
             read_row<V, E>(u, ring.at(0), p.x_type, col0, kStep, p.cols);
             read_row<V, E>(g, ring.at(1), p.y_type, col0, kStep, p.cols);
-            float s[2] = {0.0f, 0.0f};
+            const Pair minus = both(-mean), unit = both(rstd);
+            Pair s0 = both(0.0f), s1 = both(0.0f);
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < V; ++i) {  // outside the row g is zero, and u only meets g
-                    u[e][i] = (u[e][i] - mean) * rstd;
-                    dw[e][i] = fmaf(g[e][i], u[e][i], dw[e][i]);
-                    db[e][i] += g[e][i];
-                    g[e][i] *= w[e][i];
-                    s[0] += g[e][i];
-                    s[1] = fmaf(g[e][i], u[e][i], s[1]);
-                }
+            for (int k = 0; k < E * V / 2; ++k) {  // outside the row g is zero, and u only meets g
+                const Pair v = mul2(add2(get2(u, k), minus), unit), y = get2(g, k);
+                set2(u, k, v);
+                set2(dw, k, fma2(y, v, get2(dw, k)));
+                set2(db, k, add2(y, get2(db, k)));
+                const Pair z = mul2(y, get2(w, k));
+                set2(g, k, z);
+                s0 = add2(z, s0);
+                s1 = fma2(z, v, s1);
+            }
+            float s[2] = {s0.x + s0.y, s1.x + s1.y};
             row_sum<W, 2>(s, red, slot);
             const float scale = ring.ok ? rstd : __int_as_float(0x7fffffff);  // a lost copy shows as NaN
-            const float c1 = scale * divide(s[0], n, inv), c2 = scale * divide(s[1], n, inv);
+            const Pair c1 = both(-scale * divide(s[0], n, inv)), c2 = both(-scale * divide(s[1], n, inv));
 #pragma unroll
-            for (int e = 0; e < E; ++e)
-#pragma unroll
-                for (int i = 0; i < V; ++i) g[e][i] = fmaf(scale, g[e][i], -fmaf(c2, u[e][i], c1));
+            for (int k = 0; k < E * V / 2; ++k)
+                set2(g, k, fma2(both(scale), get2(g, k), fma2(c2, get2(u, k), c1)));
             if constexpr (kSum) {
                 read_row<V, E>(u, ring.at(2), p.x_type, col0, kStep, p.cols);
 #pragma unroll
-                for (int e = 0; e < E; ++e)
-#pragma unroll
-                    for (int i = 0; i < V; ++i) g[e][i] += u[e][i];
+                for (int k = 0; k < E * V / 2; ++k) set2(g, k, add2(get2(g, k), get2(u, k)));
             }
             if (kSum || W == 1) row_sync<W>();
             ring.take(row + p.stages * step < p.rows);
@@ -709,23 +745,30 @@ struct Tensor {
     long long stride;
 };
 
-// Elements per vector that all tensors' rows allow: 4 or 8 when every address is a
-// multiple of it and all rows begin at the same places, else 1.  places: how
-// far a row's beginning moves in a vector from row to row.
-int vector_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* places) {
-    const int v = x_type == CIMEKV_F32 ? 4 : 8;
+// Whether vectors of v elements fit: every address is a multiple, and all rows
+// begin at the same places.  places: how far a row's beginning moves in a vector
+// from row to row.
+bool vectors_fit(int v, std::initializer_list<Tensor> ts, int* places) {
     *places = -1;
     for (const Tensor& t : ts) {
         if (!t.p) continue;
         const int here = (int)(t.stride % v);
-        if ((uintptr_t)t.p % ((size_t)v * type_bytes(t.type)) != 0 || (*places >= 0 && *places != here)) {
-            *places = 0;
-            return 1;
-        }
+        if ((uintptr_t)t.p % ((size_t)v * type_bytes(t.type)) != 0 || (*places >= 0 && *places != here)) return false;
         *places = here;
     }
     if (*places < 0) *places = 0;
-    return pick_shape(cols, v) < 0 ? 1 : v;  // the widest rows that do not begin on vectors
+    return true;
+}
+
+// The layout for a call's tensors.  16-bit rows take vectors of eight, or of four
+// where those leave fewer threads idle (384 columns: 384 places against 512).
+int layout_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* places) {
+    const int four = pick_shape(cols, 4), eight = x_type == CIMEKV_F32 ? -1 : pick_shape(cols, 8);
+    if (eight >= 0 && (four < 0 || kShapes[eight].capacity() <= kShapes[four].capacity()) && vectors_fit(8, ts, places))
+        return eight;
+    if (four >= 0 && vectors_fit(4, ts, places)) return four;
+    *places = 0;
+    return pick_shape(cols, 1);
 }
 
 int allow_smem(const void* kernel, size_t bytes) {
@@ -769,9 +812,8 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
         return fail(CIMEKV_EINVAL_SHAPE, "null pointer");
     if (x_stride < 0 || delta_stride < 0) return fail(CIMEKV_EINVAL_SHAPE, "negative stride");
     int places, sms;
-    const int v = vector_of(x_type, cols, {{x, x_type, x_stride}, {delta, delta_type, delta_stride}, {h, x_type, cols}, {y, y_type, cols}},
-                            &places);
-    const int i = pick_shape(cols, v);
+    const int i = layout_of(x_type, cols, {{x, x_type, x_stride}, {delta, delta_type, delta_stride}, {h, x_type, cols},
+                                           {y, y_type, cols}}, &places);
     if ((rc = sm_count(&sms))) return rc;
     NormParams p = {};
     p.x = x;
@@ -835,10 +877,9 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
     int nparts = 0;
     if (rows > 0) {
         int places, sms;
-        const int v = vector_of(x_type, cols, {{h, x_type, h_stride}, {dy, y_type, dy_stride}, {dh, x_type, dh_stride},
-                                         {dx, x_type, cols}, {ddelta, delta_type, cols}}, &places);
-        const int i = pick_shape(cols, v);
-            if ((rc = sm_count(&sms))) return rc;
+        const int i = layout_of(x_type, cols, {{h, x_type, h_stride}, {dy, y_type, dy_stride}, {dh, x_type, dh_stride},
+                                               {dx, x_type, cols}, {ddelta, delta_type, cols}}, &places);
+        if ((rc = sm_count(&sms))) return rc;
         const long long grid = grid_size(rows, kShapes[i], sms);
         if (want_w) {
             if (!workspace || workspace_bytes < (size_t)grid * 2 * cols * sizeof(float))
