@@ -332,6 +332,14 @@ __host__ __device__ constexpr int cta_warps(int W) { return W == 16 ? 16 : 8; }
 __host__ __device__ constexpr int cta_rows(int W) { return cta_warps(W) / W; }
 __host__ __device__ constexpr int cta_threads(int W) { return cta_warps(W) * 32; }
 
+// CTAs kept resident on an SM: three in the forward where a thread's elements leave
+// the registers for it (25.0 -> 22.3 us at 50,432 x 384 fp16, but with 16 elements
+// and spilled registers 90 -> 152 us at 16,384 x 4,096), two in the backward
+// (three: 40 -> 58 us), one of the widest rows.
+__host__ __device__ constexpr int ctas_per_sm(int elements, int W, bool forward) {
+    return W == 16 ? 1 : forward && elements <= 12 ? 3 : 2;
+}
+
 // Sum over the W warps of a row, the same bits in every thread.  `slot` alternates
 // between two buffers, so one barrier of the row's warps is enough: a buffer is
 // written again only after the barrier of the sum in between.
@@ -481,7 +489,7 @@ __device__ __forceinline__ void row_sync() {
 }
 
 template <int V, int E, int W, bool kDelta>
-__global__ void __launch_bounds__(cta_threads(W)) norm_fwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) norm_fwd_kernel(NormParams p) {
     constexpr int T = W * 32, kStep = T * V, N = kDelta ? 2 : 1;
     extern __shared__ __align__(16) uint8_t memory[];
     __shared__ __align__(8) uint64_t bars[cta_rows(W)][kMaxStages];
@@ -555,7 +563,7 @@ __global__ void __launch_bounds__(cta_threads(W)) norm_fwd_kernel(NormParams p) 
 // kSum: the sum's own gradient dh is added to dx.  p.part: the CTA's column sums
 // [gridDim][2][cols] (dw, db), or null when no weight gradient is wanted.
 template <int V, int E, int W, bool kSum>
-__global__ void __launch_bounds__(cta_threads(W), W == 16 ? 1 : 2) norm_bwd_kernel(NormParams p) {
+__global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, false)) norm_bwd_kernel(NormParams p) {
     constexpr int T = W * 32, kStep = T * V, N = kSum ? 3 : 2;
     extern __shared__ __align__(16) uint8_t memory[];
     __shared__ __align__(8) uint64_t bars[cta_rows(W)][kMaxStages];
@@ -712,10 +720,10 @@ const Kernels& kernels(int i, std::integer_sequence<int, I...>) {
 }
 const Kernels& kernels(int i) { return kernels(i, std::make_integer_sequence<int, kNumShapes>()); }
 
-// Rows under way per row group: as many as fit a share of shared memory that
-// leaves room for two CTAs per SM (one for the widest rows), at most four.
-int ring_stages(const Shape& s, size_t row_bytes) {
-    const size_t share = s.w == 16 ? 200 << 10 : 100 << 10;
+// Rows under way per row group: as many as fit a CTA's share of 200 KB of shared
+// memory, at most four.
+int ring_stages(const Shape& s, size_t row_bytes, bool forward) {
+    const size_t share = (200 << 10) / ctas_per_sm(s.v * s.e, s.w, forward);
     const size_t n = share / (row_bytes * cta_rows(s.w));
     return n > kMaxStages ? kMaxStages : n < 1 ? 1 : (int)n;
 }
@@ -728,11 +736,11 @@ int sm_count(int* sms) {
     return CIMEKV_OK;
 }
 
-// CTAs of a launch: two to an SM (one of sixteen warps); a multiple of V, so that a
-// group's rows all begin at the same place of a vector.
-long long grid_size(long long rows, const Shape& s, int sms) {
+// CTAs of a launch: what is resident at once; a multiple of V, so that a group's rows
+// all begin at the same place of a vector.
+long long grid_size(long long rows, const Shape& s, int sms, bool forward) {
     const long long need = (rows + cta_rows(s.w) - 1) / cta_rows(s.w);
-    const long long most = (long long)sms * (s.w == 16 ? 1 : 2);
+    const long long most = (long long)sms * ctas_per_sm(s.v * s.e, s.w, forward);
     return ((need < most ? need : most) + s.v - 1) / s.v * s.v;
 }
 
@@ -836,11 +844,11 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
     p.eps = eps;
     if ((rc = cimekv_internal_no_pending_error())) return rc;
     const size_t row_bytes = row_room(cols, x_type) + (delta ? row_room(cols, delta_type) : 0);
-    p.stages = ring_stages(kShapes[i], row_bytes);
+    p.stages = ring_stages(kShapes[i], row_bytes, true);
     const Kernel kernel = kernels(i).fwd[delta != nullptr];
     const size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
     if ((rc = allow_smem((const void*)kernel, smem))) return rc;
-    kernel<<<(unsigned)grid_size(rows, kShapes[i], sms), cta_threads(kShapes[i].w), smem, (cudaStream_t)stream>>>(p);
+    kernel<<<(unsigned)grid_size(rows, kShapes[i], sms, true), cta_threads(kShapes[i].w), smem, (cudaStream_t)stream>>>(p);
     return launched("norm_fwd_kernel");
 }
 
@@ -853,7 +861,7 @@ extern "C" size_t cimekv_layer_norm_workspace_bytes(long long rows, int cols) {
     long long most = 0;
     for (const int v : {1, 4, 8}) {
         const int i = pick_shape(cols, v);
-        const long long g = i < 0 ? 0 : grid_size(rows, kShapes[i], sms);
+        const long long g = i < 0 ? 0 : grid_size(rows, kShapes[i], sms, false);
         if (g > most) most = g;
     }
     return (size_t)most * 2 * (size_t)cols * sizeof(float);
@@ -880,7 +888,7 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
         const int i = layout_of(x_type, cols, {{h, x_type, h_stride}, {dy, y_type, dy_stride}, {dh, x_type, dh_stride},
                                                {dx, x_type, cols}, {ddelta, delta_type, cols}}, &places);
         if ((rc = sm_count(&sms))) return rc;
-        const long long grid = grid_size(rows, kShapes[i], sms);
+        const long long grid = grid_size(rows, kShapes[i], sms, false);
         if (want_w) {
             if (!workspace || workspace_bytes < (size_t)grid * 2 * cols * sizeof(float))
                 return fail(CIMEKV_EWORKSPACE, "layer norm backward workspace too small");
@@ -907,7 +915,7 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
         p.y_type = y_type;
         p.places = places;
         const size_t row_bytes = row_room(cols, y_type) + (dh ? 2 : 1) * (size_t)row_room(cols, x_type);
-        p.stages = ring_stages(kShapes[i], row_bytes);
+        p.stages = ring_stages(kShapes[i], row_bytes, false);
         const Kernel kernel = kernels(i).bwd[dh != nullptr];
         size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
         if (cta_rows(kShapes[i].w) > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
