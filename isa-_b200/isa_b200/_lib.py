@@ -10,6 +10,7 @@ import of this module fails.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 import threading
 from pathlib import Path
@@ -20,12 +21,6 @@ _LIB_PATH = Path(os.environ.get("CIMEKV_LIB", Path(__file__).resolve().parent / 
 
 _c_int, _c_float, _c_size, _vp = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
 _c_ll = ctypes.c_longlong
-
-# Element types of the entry points that take several (CIMEKV_F32, ...).
-TYPE_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
-LAYER_NORM_MAX_COLS = 16384  # CIMEKV_LAYER_NORM_MAX_COLS
-ORTHOGONALIZE_MAX_SIDE = 32768  # CIMEKV_ORTHOGONALIZE_MAX_SIDE
-MUON_MAX_MATRICES = 128  # CIMEKV_MUON_MAX_MATRICES
 
 # name -> (restype, argtypes); mirrors include/cimekv.h
 SIGNATURES = {
@@ -72,8 +67,11 @@ SIGNATURES = {
     "cimekv_fp32_probe": (_c_int, [_vp, _c_int, _c_int, ctypes.POINTER(ctypes.c_longlong), _vp]),
 }
 
+_BINDING_PATH = Path(__file__).resolve().parent / "_lib" / "cimekv_torch.so"
+
 _lock = threading.Lock()
 _lib = None
+_binding = None
 
 
 def load() -> ctypes.CDLL:
@@ -93,6 +91,27 @@ def load() -> ctypes.CDLL:
                 fn.argtypes = args
             _lib = lib
     return _lib
+
+
+def binding():
+    """The C++ tensor binding of the digital operators (csrc/torch_binding.cpp),
+    tied to the library that load() opened (raises if it has not been built)."""
+    global _binding
+    if _binding is None:
+        lib = load()
+        with _lock:
+            if _binding is None:
+                if not _BINDING_PATH.exists():
+                    raise RuntimeError(
+                        f"cimekv_torch.so not found at {_BINDING_PATH}; build it with `python -m isa_b200.build` "
+                        "(the layer norm and Newton-Schulz operators have no other implementation)"
+                    )
+                spec = importlib.util.spec_from_file_location("cimekv_torch", _BINDING_PATH)
+                module = importlib.util.module_from_spec(spec)
+                spec.loader.exec_module(module)
+                module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES})
+                _binding = module
+    return _binding
 
 
 def open_variant(path) -> ctypes.CDLL:
@@ -123,8 +142,7 @@ def _ptr(t: torch.Tensor | None) -> int | None:
 
 def _stream(stream) -> int | None:
     if stream is None:
-        # the handle of torch.cuda.current_stream() without making the Stream object
-        return torch._C._cuda_getCurrentRawStream(torch.cuda.current_device())
+        return torch.cuda.current_stream().cuda_stream
     return stream.cuda_stream if hasattr(stream, "cuda_stream") else int(stream)
 
 
@@ -261,79 +279,6 @@ def lut_index(delta: torch.Tensor, table_size: int, delta_min: float, delta_scal
                                  _ptr(index), _ptr(alpha), _stream(stream))
     _check(rc, "cimekv_lut_index")
     return index, alpha
-
-
-class on_device:
-    """Makes ``device`` current for a launch; costs nothing where it is already."""
-
-    __slots__ = ("to", "back")
-
-    def __init__(self, device: torch.device):
-        self.to, self.back = device.index, None
-
-    def __enter__(self):
-        if torch.cuda.current_device() != self.to:
-            self.back = torch.cuda.device(self.to)
-            self.back.__enter__()
-
-    def __exit__(self, *exc):
-        if self.back is not None:
-            self.back.__exit__(*exc)
-
-
-def layer_norm_forward(x, x_stride, delta, delta_stride, weight, bias, rows, cols, eps, h, y, stats,
-                       stream=None) -> None:
-    """x and delta: rows with strides in elements; weight and bias share a type;
-    stats: [2, rows] fp32 for mean and rstd, or None; see cimekv.h."""
-    affine = weight if weight is not None else bias
-    mean = _ptr(stats)
-    rc = load().cimekv_layer_norm_forward(
-        x.data_ptr(), TYPE_CODES[x.dtype], x_stride, _ptr(delta), 0 if delta is None else TYPE_CODES[delta.dtype],
-        delta_stride, _ptr(weight), _ptr(bias), 0 if affine is None else TYPE_CODES[affine.dtype], rows, cols, eps,
-        _ptr(h), y.data_ptr(), TYPE_CODES[y.dtype], mean, mean and mean + 4 * rows, _stream(stream))
-    _check(rc, "cimekv_layer_norm_forward")
-
-
-def layer_norm_backward(dy, dy_stride, dh, dh_stride, h, h_stride, weight, w_dtype, stats, rows, cols, dx, ddelta,
-                        dw, db, stream=None) -> None:
-    """dw and db in ``w_dtype``; the workspace of their sums is allocated here."""
-    lib = load()
-    ws, ws_bytes = None, 0
-    if dw is not None or db is not None:
-        ws_bytes = lib.cimekv_layer_norm_workspace_bytes(rows, cols)
-        ws = h.new_empty(ws_bytes, dtype=torch.uint8)
-    mean = stats.data_ptr()
-    rc = lib.cimekv_layer_norm_backward(
-        dy.data_ptr(), TYPE_CODES[dy.dtype], dy_stride, _ptr(dh), dh_stride, h.data_ptr(), TYPE_CODES[h.dtype],
-        h_stride, _ptr(weight), 0 if w_dtype is None else TYPE_CODES[w_dtype], mean, mean and mean + 4 * rows, rows,
-        cols, _ptr(dx), _ptr(ddelta), 0 if ddelta is None else TYPE_CODES[ddelta.dtype], _ptr(dw), _ptr(db), _ptr(ws),
-        ws_bytes, _stream(stream))
-    _check(rc, "cimekv_layer_norm_backward")
-
-
-def orthogonalize_workspace_bytes(batch: int, rows: int, cols: int) -> int:
-    return int(load().cimekv_orthogonalize_workspace_bytes(batch, rows, cols))
-
-
-def orthogonalize(g, batch_stride, row_stride, batch, rows, cols, steps, coefficients, eps, out, workspace,
-                  stream=None) -> None:
-    """Matrices [batch][rows][cols] with contiguous rows into the contiguous ``out``."""
-    rc = load().cimekv_orthogonalize(
-        g.data_ptr(), TYPE_CODES[g.dtype], batch_stride, row_stride, batch, rows, cols, steps, *coefficients, eps,
-        out.data_ptr(), workspace.data_ptr(), workspace.numel(), _stream(stream))
-    _check(rc, "cimekv_orthogonalize")
-
-
-def muon_step(params, grads, momenta, p_dtype, g_dtype, rows, cols, lr, lr_tensor, momentum, nesterov, weight_decay,
-              scale, steps, coefficients, eps, workspace, stream=None) -> None:
-    """params, grads, momenta: lists of device addresses of [rows][cols] matrices."""
-    n = len(params)
-    table = ctypes.c_void_p * n
-    rc = load().cimekv_muon_step(
-        n, table(*params), table(*grads), table(*momenta), TYPE_CODES[p_dtype], TYPE_CODES[g_dtype], rows, cols, lr,
-        _ptr(lr_tensor), momentum, int(nesterov), weight_decay, scale, steps, *coefficients, eps,
-        workspace.data_ptr(), workspace.numel(), _stream(stream))
-    _check(rc, "cimekv_muon_step")
 
 
 def fp32_probe(sink: torch.Tensor, iters: int, blocks: int, stream=None) -> int:

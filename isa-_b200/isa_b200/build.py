@@ -1,9 +1,10 @@
-"""Build the sm_100a C-ABI library ``libcimekv.so`` in-tree.
+"""Build the sm_100a C-ABI library ``libcimekv.so`` and its C++ tensor binding
+``cimekv_torch.so`` in-tree.
 
     python -m isa_b200.build        (or isa_b200.build.build_library())
 
-nvcc cross-compiles for sm_100a without a GPU.  The library lands next to this
-file in ``_lib/`` so it travels with the source tree.
+nvcc cross-compiles for sm_100a without a GPU.  Both land next to this file in
+``_lib/`` so they travel with the source tree.
 """
 
 from __future__ import annotations
@@ -12,6 +13,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG_DIR = Path(__file__).resolve().parent
@@ -20,12 +22,13 @@ REPO_ROOT = PKG_DIR.parent.parent
 INCLUDE_DIR = REPO_ROOT / "include"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libcimekv.so"
+BINDING_PATH = LIB_DIR / "cimekv_torch.so"
 DEBUG_LIB_PATH = LIB_DIR / "libcimekv_debug.so"  # table-index bounds checks (CIMEKV_DEBUG_BOUNDS=1)
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",
     "-O3", "-lineinfo", "-std=c++17",
-    "-Xcompiler", "-fPIC", "-shared",
+    "-Xcompiler", "-fPIC", "-shared", "--threads", "0",
 ]
 
 
@@ -42,7 +45,10 @@ def sources() -> list[Path]:
 
 def build_library(force: bool = False, verbose: bool = False, debug: bool = False) -> Path:
     """Compile csrc/*.cu into _lib/libcimekv.so (or the bounds-checking
-    libcimekv_debug.so with debug=True); skipped when up to date."""
+    libcimekv_debug.so with debug=True); skipped when up to date.  The release
+    build brings the tensor binding with it."""
+    if not debug:
+        build_binding(force)
     srcs = sources()
     deps = srcs + sorted(INCLUDE_DIR.glob("*.h")) + sorted(SRC_DIR.glob("*.cuh"))
     out = DEBUG_LIB_PATH if debug else LIB_PATH
@@ -59,6 +65,31 @@ def build_library(force: bool = False, verbose: bool = False, debug: bool = Fals
         cmd.insert(1, "-Xptxas=-v")
         print(" ".join(cmd), file=sys.stderr)
     subprocess.run(cmd, check=True)
+    os.replace(tmp, out)
+    return out
+
+
+def build_binding(force: bool = False) -> Path:
+    """Compile csrc/torch_binding.cpp into _lib/cimekv_torch.so; skipped when up to date."""
+    src, out = SRC_DIR / "torch_binding.cpp", BINDING_PATH
+    deps = [src, *INCLUDE_DIR.glob("*.h")]
+    if not force and out.exists() and all(p.stat().st_mtime <= out.stat().st_mtime for p in deps):
+        return out
+    import torch
+    from torch.utils.cpp_extension import include_paths
+
+    cxx = shutil.which("g++")
+    if cxx is None:
+        raise RuntimeError("g++ not found: a C++ compiler is required to build the tensor binding")
+    torch_lib = Path(torch.__file__).resolve().parent / "lib"
+    cuda = Path(_nvcc()).resolve().parent.parent / "include"
+    includes = [*include_paths("cuda"), sysconfig.get_paths()["include"], str(cuda)]
+    LIB_DIR.mkdir(parents=True, exist_ok=True)
+    tmp = out.with_suffix(".so.tmp")
+    subprocess.run([cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-DTORCH_EXTENSION_NAME=cimekv_torch",
+                    f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                    *(f"-isystem{p}" for p in includes), f"-I{INCLUDE_DIR}", str(src), "-o", str(tmp), f"-L{torch_lib}",
+                    "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"], check=True)
     os.replace(tmp, out)
     return out
 
