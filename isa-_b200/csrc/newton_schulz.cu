@@ -68,16 +68,30 @@ int launched(const char* what) {
 }
 
 constexpr float kScale = 4096.0f;  // fp16 planes hold value * 2^12
-constexpr int kTile = 128;         // rows (and right-hand rows) that one CTA stages
 constexpr int kK = 64;             // depth of one stage: 64 halves = one 128-byte swizzle row
-constexpr int kStages = 3;
-constexpr int kOperand = kTile * kK * 2;    // bytes of one operand plane in a stage
-constexpr int kStageBytes = 4 * kOperand;   // left hi, left lo, right hi, right lo
-constexpr int kEpilogueWarps = 16;
-constexpr int kTmemColumns = 512;
-constexpr int kGemmThreads = (kEpilogueWarps + 2) * 32;  // and a copy warp, a product warp
-constexpr int kStagingBytes = 2048;         // a collecting warp's 32 rows of 64 bytes on their way out
-constexpr int kSmemBytes = kStages * kStageBytes + kEpilogueWarps * kStagingBytes + 1024;
+constexpr int kMaxStages = 6;
+
+// The three kinds of output tile (see product()), by their side.
+template <int kSide>
+struct Tile {
+    static constexpr bool kPair = kSide == 256;
+    static constexpr int kRanks = kPair ? 2 : 1;
+    static constexpr int kRows = kSide / kRanks;            // rows of either operand that one CTA stages
+    static constexpr int kStages = kSide == 64 ? 6 : 3;     // 192 KB of them
+    static constexpr int kOperand = kRows * kK * 2;         // bytes of one operand plane in a stage
+    static constexpr int kStageBytes = 4 * kOperand;        // left hi, left lo, right hi, right lo
+    static constexpr int kWarpRows = kRows / 4;             // result rows of a collecting warp (its quarter of
+                                                            // tensor memory; 64 rows fill half of each)
+    static constexpr int kWarps = kSide == 64 ? 8 : 16;     // collecting warps
+    static constexpr int kWarpCols = kSide / (kWarps / 4);  // result columns of a collecting warp
+    static constexpr int kThreads = (kWarps + 2) * 32;      // and a copy warp, a product warp
+    static constexpr int kBufs = kPair ? 2 : 4;             // accumulators in tensor memory
+    static constexpr int kChunk = kPair ? 2 : 1;            // stages summed in one of them
+    static constexpr int kColumns = kBufs * kSide;          // tensor memory columns
+    static constexpr int kStaging = kWarpRows * 64;         // a collecting warp's row segments on their way out
+    static constexpr int kSmem = kStages * kStageBytes + kWarps * kStaging + 1024;
+};
+
 constexpr int kMaxTable = CIMEKV_MUON_MAX_MATRICES;
 constexpr int kMaxParts = 256;              // partial norms per matrix, at most
 
@@ -152,6 +166,16 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes "
             "[%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x), "r"(y), "r"(z), "r"(bar)
             : "memory");
+}
+
+// One lane of a converged warp.  The copy and product warps run whole, with values
+// that are the same in all lanes, and only issue from one: coordinates and
+// descriptors then live in uniform registers, where these instructions want them
+// (issued from an `if (lane == 0)` a stage's twelve products took 1,450 cycles).
+__device__ __forceinline__ bool elect_one() {
+    uint32_t one;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(one));
+    return one != 0;
 }
 
 // Shared-memory operand descriptors, 128-byte swizzle.  Rows along K (a plane's
@@ -261,6 +285,7 @@ struct PrepParams {
     float eps;
     int parts;          // partial norms per matrix
     double* part;       // [batch][parts]
+    unsigned* arrivals; // [batch], zeroed here for ns_steps_kernel
     __half* x;
 };
 
@@ -307,6 +332,7 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Pr
     const void* g = p.g.at(b);
     float* mom = p.mom.tabled ? static_cast<float*>(p.mom.table[b]) : nullptr;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.arrivals[b] = 0;
     double s = 0.0;
     if constexpr (kFlat) {
         const long long total = (long long)p.rows * p.cols / 4;
@@ -506,24 +532,28 @@ __device__ __forceinline__ float result_of(const Result& p, float sum, float old
     return p.update ? fmaf(-lr * p.scale, o, fmaf(-lr * p.decay, old, old)) : o;
 }
 
-// Turns rows held by lanes into row segments: on entry lane i holds 64 bytes of
-// row i, on exit d[t] is bytes 16 (i % 4) .. + 15 of row 8 t + i / 4, so that a
+// Turns rows held by lanes into row segments: on entry lane i < kRows holds 64 bytes
+// of row i, on exit d[t] is bytes 16 (i % 4) .. + 15 of row 8 t + i / 4, so that a
 // store covers eight segments of 64 bytes instead of 32 of 16 (an SM moves one
 // 128-byte line a cycle however little of it is used: straight from the registers the
 // stores of a 128 x 128 tile took 6,000 cycles).  Units of 16 bytes are
 // swizzled: both sides are free of bank conflicts.
-__device__ __forceinline__ void turn_rows(uint32_t staging, const uint4 (&r)[4], uint4 (&d)[4]) {
+template <int kRows>
+__device__ __forceinline__ void turn_rows(uint32_t staging, const uint4 (&r)[4], uint4 (&d)[kRows / 8]) {
     const int lane = threadIdx.x & 31;
     __syncwarp();
+    if (kRows == 32 || lane < kRows) {
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const uint32_t at = staging + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4);
-        asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[k].x), "r"(r[k].y), "r"(r[k].z), "r"(r[k].w)
-                     : "memory");
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t at = staging + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4);
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(r[k].x), "r"(r[k].y), "r"(r[k].z),
+                         "r"(r[k].w)
+                         : "memory");
+        }
     }
     __syncwarp();
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < kRows / 8; ++t) {
         const int row = 8 * t + (lane >> 2);
         const uint32_t at = staging + row * 64 + (((lane & 3) ^ ((row >> 1) & 3)) << 4);
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
@@ -533,15 +563,16 @@ __device__ __forceinline__ void turn_rows(uint32_t staging, const uint4 (&r)[4],
     }
 }
 
-// 16 columns from cb of the warp's 32 rows from row0 of the last product, to the
+// 16 columns from cb of the warp's kRows rows from row0 of the last product, to the
 // caller's matrix.  Called by whole warps.
+template <int kRows>
 __device__ __forceinline__ void finish_result(const Result& p, int rows, int cols, const float (&v)[16], int b, int row0,
                                               int cb, float lr, uint32_t staging) {
     void* dst = const_cast<void*>(p.dst.at(b));
     const int type = p.dst.type, lane = threadIdx.x & 31;
     if (p.transposed) {  // neighbouring lanes hold neighbouring elements
         const int r = row0 + lane;
-        if (r >= rows) return;
+        if (lane >= kRows || r >= rows) return;
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             if (cb + i >= cols) break;
@@ -550,15 +581,15 @@ __device__ __forceinline__ void finish_result(const Result& p, int rows, int col
         }
         return;
     }
-    uint4 in[4], out[4];
+    uint4 in[4], out[kRows / 8];
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         in[k] = make_uint4(__float_as_uint(v[4 * k]), __float_as_uint(v[4 * k + 1]), __float_as_uint(v[4 * k + 2]),
                            __float_as_uint(v[4 * k + 3]));
-    turn_rows(staging, in, out);
+    turn_rows<kRows>(staging, in, out);
     const int c = cb + (lane & 3) * 4;
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
+    for (int t = 0; t < kRows / 8; ++t) {
         const int r = row0 + 8 * t + (lane >> 2);
         if (r >= rows || c >= cols) continue;
         const long long at = (long long)r * cols + c;
@@ -588,10 +619,10 @@ __device__ __forceinline__ void finish_result(const Result& p, int rows, int col
     }
 }
 
-// 32 columns from cb of the warp's 32 rows from row0 of a product that stays in
+// 32 columns from cb of the warp's kRows rows from row0 of a product that stays in
 // planes, and their mirror image off the diagonal of a symmetric one.  Called by
 // whole warps.
-template <bool kSym>
+template <bool kSym, int kRows>
 __device__ __forceinline__ void finish_planes(const Product& p, const float (&v0)[16], const float (&v1)[16], int b,
                                               int row0, int cb, bool diagonal, uint32_t staging) {
     const int lane = threadIdx.x & 31, r = row0 + lane;
@@ -610,13 +641,13 @@ __device__ __forceinline__ void finish_planes(const Product& p, const float (&v0
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
         const uint32_t(&w)[16] = words[plane];
-        uint4 in[4], out[4];
+        uint4 in[4], out[kRows / 8];
 #pragma unroll
         for (int k = 0; k < 4; ++k) in[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        turn_rows(staging, in, out);
+        turn_rows<kRows>(staging, in, out);
         const int c = cb + (lane & 3) * 8;
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
+        for (int t = 0; t < kRows / 8; ++t) {
             const int row = row0 + 8 * t + (lane >> 2);
             // the pitch is a multiple of 8: a group that begins inside a row ends inside its pitch
             if (row < p.rows && c < p.cols)
@@ -631,16 +662,12 @@ __device__ __forceinline__ void finish_planes(const Product& p, const float (&v0
 #pragma unroll
             for (int i = 0; i < 16; ++i) {
                 const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], 1);
-                if (r2 < p.rows && cb + 2 * i + odd < p.cols)
+                if (lane < kRows && r2 < p.rows && cb + 2 * i + odd < p.cols)
                     *reinterpret_cast<uint32_t*>(mirror + (long long)(2 * i) * p.out_pitch) = __byte_perm(w[i], other, sel);
             }
         }
     }
 }
-
-// Accumulators in tensor memory (512 columns), and stages summed in one of them.
-__host__ __device__ constexpr int bufs(bool pair) { return pair ? 2 : 4; }
-__host__ __device__ constexpr int chunk_stages(bool pair) { return pair ? 2 : 1; }
 
 // Shared-memory addresses of a CTA's pipeline, and where each role stands in it.
 struct Pipe {
@@ -651,25 +678,30 @@ struct Pipe {
     bool ok;                // no wait has run out
 };
 
-// The tiles first, first + step, ... of one product: 128 x 128 by one CTA, or 256 x 256 by a
-// pair of CTAs whose tensor cores work as one (each stages 128 rows of either
-// operand, holds its 128 rows of the result, and the first CTA issues).  One warp
-// copies stages ahead, one issues products, sixteen collect.
+// The tiles first, first + step, ... of one product.  Tiles are 128 x 128 by one CTA,
+// 256 x 256 by a pair of CTAs whose tensor cores work as one (each stages 128
+// rows of either operand, holds its 128 rows of the result, and the first CTA
+// issues), or 64 x 64 by one CTA.  One warp copies stages ahead, one
+// issues products, the others collect.  An SM takes in about 43 bytes a cycle and
+// puts out about 30: a stage of 64 KB (768 cycles of products for a 128 tile, 1,536
+// for a pair) feeds only the pair's tensor cores, which is why many tiles go to
+// pairs and few to the tile that spreads them over the most SMs.
 //
 // The tensor core adds into fp32 accumulators by cutting off, not by rounding:
 // over a long depth that is a drift of half a step per addition.  So every stage
-// (4 additions at full size, the small cross products before them) goes into a fresh
-// accumulator, one of two, and the collecting warps add the stages in registers
-// with round-to-nearest while the next stage runs.  The same two accumulators let
-// the next tile start while the last one is stored.
-template <int M, bool kPair>
+// (4 additions at full size, the small cross products before them; two stages of a
+// pair) goes into a fresh accumulator, one of several, and the collecting warps add
+// them in registers with round-to-nearest while the next ones run.  The same
+// accumulators let the next tile start while the last one is stored.
+template <int M, int kSide>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right, const Product& p,
                                         const Result* result, int batch, int first, int step, int tiles) {
-    constexpr int kRanks = kPair ? 2 : 1;
-    constexpr int kSide = kTile * kRanks;                       // output tile side, and columns of an accumulator
-    constexpr int kWarpCols = kSide / (kEpilogueWarps / 4);     // columns a collecting warp holds
-    constexpr int kBufs = bufs(kPair), kChunk = chunk_stages(kPair);
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    using T = Tile<kSide>;
+    constexpr bool kPair = T::kPair;
+    constexpr int kRanks = T::kRanks, kRows = T::kRows, kOperand = T::kOperand, kStageBytes = T::kStageBytes;
+    constexpr int kWarpCols = T::kWarpCols, kWarps = T::kWarps, kBufs = T::kBufs, kChunk = T::kChunk;
+    constexpr int kStages = T::kStages;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // known to be uniform
     const int ni = (p.rows + kSide - 1) / kSide, nj = (p.cols + kSide - 1) / kSide;
     const int per_matrix = M == kSymmetric ? ni * (ni + 1) / 2 : ni * nj;
     const int ksteps = (p.depth + kK - 1) / kK;
@@ -687,19 +719,19 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
         col0 = j * kSide;
     };
 
-    if (warp == kEpilogueWarps) {
-        if (lane == 0) {
-            const uint32_t count_at = kPair ? cluster_addr(q.full, 0) : q.full;
-            for (int t = first; t < tiles && q.ok; t += step) {
-                int b, row0, col0;
-                place(t, b, row0, col0);
-                row0 += (int)q.rank * kTile;
-                col0 += (int)q.rank * kTile;
-                for (int k = 0; k < ksteps; ++k, ++q.fill) {
-                    const int s = q.fill % kStages;
-                    if (q.fill >= kStages && !(q.ok = mbar_wait(q.empty + 8 * s, (q.fill / kStages - 1) & 1))) break;
-                    const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
-                    const bool same = M == kSymmetric && row0 == col0;  // both operands are the same rows
+    if (warp == kWarps) {
+        const uint32_t count_at = kPair ? cluster_addr(q.full, 0) : q.full;
+        for (int t = first; t < tiles && q.ok; t += step) {
+            int b, row0, col0;
+            place(t, b, row0, col0);
+            const bool same = M == kSymmetric && row0 == col0;  // both operands are the same rows
+            row0 += (int)q.rank * kRows;
+            col0 += (int)q.rank * kRows;
+            for (int k = 0; k < ksteps; ++k, ++q.fill) {
+                const int s = q.fill % kStages;
+                if (q.fill >= kStages && !(q.ok = mbar_wait(q.empty + 8 * s, (q.fill / kStages - 1) & 1))) break;
+                const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
+                if (elect_one()) {
                     if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
 #pragma unroll
                     for (int plane = 0; plane < 2; ++plane) {
@@ -711,14 +743,15 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                             tma_box<kPair>(r, right, k * kK, col0, z, bar);
                         } else {
                             tma_box<kPair>(r, right, col0, k * kK, z, bar);
-                            tma_box<kPair>(r + kOperand / 2, right, col0 + 64, k * kK, z, bar);
+                            if (kRows == 128) tma_box<kPair>(r + kOperand / 2, right, col0 + 64, k * kK, z, bar);
                         }
                     }
                 }
+                __syncwarp();
             }
         }
-    } else if (warp == kEpilogueWarps + 1) {
-        if (lane == 0 && q.rank == 0) {
+    } else if (warp == kWarps + 1) {
+        if (q.rank == 0) {
             // D fp32, A and B fp16; right operand along K (0) or along its own axis (1)
             const uint32_t idesc = 1u << 4 | (M == kSymmetric ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
                                    (uint32_t)(kSide / 16) << 24;
@@ -731,34 +764,35 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                     if (q.chunk >= kBufs && !(q.ok = mbar_wait(q.acc_empty + 8 * buf, (q.chunk / kBufs - 1) & 1))) break;
                     const uint32_t d = q.tmem + buf * kSide;
                     const int end = min(k + kChunk, ksteps);
-                    for (bool fresh = true; k < end; ++k, ++q.fill, fresh = false) {
+                    for (uint32_t more = 0; k < end; ++k, ++q.fill, more = 1) {
                         const int s = q.fill % kStages;
                         if (!(q.ok = mbar_wait(q.full + 8 * s, (q.fill / kStages) & 1))) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t base = q.stages + s * kStageBytes;
-                        const auto desc_l = [&](int plane, int i) {
-                            return operand_desc(base + plane * kOperand + i * 32, 16, 1024);
-                        };
-                        const auto desc_r = [&](int plane, int i) {
-                            return M == kSymmetric ? operand_desc(base + r_at + plane * kOperand + i * 32, 16, 1024)
-                                                   : operand_desc(base + r_at + plane * kOperand + i * 2048, 8192, 1024);
-                        };
+                        // both planes of either operand; a step of 16 along K moves the address alone
+                        const uint64_t l0 = operand_desc(base, 16, 1024), l1 = operand_desc(base + kOperand, 16, 1024);
+                        const uint64_t r0 = operand_desc(base + r_at, M == kSymmetric ? 16 : 8192, 1024);
+                        const uint64_t r1 = operand_desc(base + r_at + kOperand, M == kSymmetric ? 16 : 8192, 1024);
+                        constexpr uint64_t kL = 32 >> 4, kR = (M == kSymmetric ? 32 : 2048) >> 4;
+                        if (elect_one()) {
 #pragma unroll
-                        for (int i = 0; i < kK / 16; ++i) {
-                            mma_f16<kPair>(d, desc_l(0, i), desc_r(1, i), idesc, !(fresh && i == 0));
-                            mma_f16<kPair>(d, desc_l(1, i), desc_r(0, i), idesc, 1);
+                            for (uint64_t i = 0; i < kK / 16; ++i) {
+                                mma_f16<kPair>(d, l0 + i * kL, r1 + i * kR, idesc, i ? 1u : more);
+                                mma_f16<kPair>(d, l1 + i * kL, r0 + i * kR, idesc, 1);
+                            }
+#pragma unroll
+                            for (uint64_t i = 0; i < kK / 16; ++i) mma_f16<kPair>(d, l0 + i * kL, r0 + i * kR, idesc, 1);
+                            mma_commit<kPair>(q.empty + 8 * s);
+                            if (k + 1 == end) mma_commit<kPair>(q.acc_full + 8 * buf);
                         }
-#pragma unroll
-                        for (int i = 0; i < kK / 16; ++i) mma_f16<kPair>(d, desc_l(0, i), desc_r(0, i), idesc, 1);
-                        mma_commit<kPair>(q.empty + 8 * s);
+                        __syncwarp();
                     }
-                    if (q.ok) mma_commit<kPair>(q.acc_full + 8 * buf);
                 }
             }
         }
     } else {
         const int quarter = warp & 3, group = warp >> 2;
-        const uint32_t staging = q.stages + kStages * kStageBytes + warp * kStagingBytes;
+        const uint32_t staging = q.stages + kStages * kStageBytes + warp * T::kStaging;
         const uint32_t empty_at = kPair ? cluster_addr(q.acc_empty, 0) : q.acc_empty;
         float lr = 0.0f;
         if constexpr (M == kResult) {
@@ -767,7 +801,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
         for (int t = first; t < tiles; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
-            const int r0 = row0 + (int)q.rank * kTile + quarter * 32;
+            const int r0 = row0 + (int)q.rank * kRows + quarter * T::kWarpRows;
             const bool diagonal = row0 == col0;
             col0 += group * kWarpCols;
             float acc[kWarpCols / 16][16];
@@ -803,9 +837,9 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             for (int g = 0; g < kWarpCols / 16; ++g) {
                 if (col0 + g * 16 >= p.cols) break;
                 if constexpr (M == kResult)
-                    finish_result(*result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
+                    finish_result<T::kWarpRows>(*result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
                 else if (g % 2 == 0)
-                    finish_planes<M == kSymmetric>(p, acc[g], acc[g + 1], b, r0, col0 + g * 16, diagonal, staging);
+                    finish_planes<M == kSymmetric, T::kWarpRows>(p, acc[g], acc[g + 1], b, r0, col0 + g * 16, diagonal, staging);
             }
             __syncwarp();
         }
@@ -813,9 +847,10 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
 }
 
 // Barriers, tensor memory.  All threads.
-template <bool kPair>
+template <int kSide>
 __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tmem_slot, uint8_t* smem_raw) {
-    constexpr int kRanks = kPair ? 2 : 1;
+    constexpr bool kPair = Tile<kSide>::kPair;
+    constexpr int kStages = Tile<kSide>::kStages;
     q.stages = (smem_addr(smem_raw) + 1023) & ~1023u;
     q.full = smem_addr(bars);
     q.empty = q.full + 8 * kStages;
@@ -829,14 +864,14 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
             mbar_init(q.full + 8 * s, 1);
             mbar_init(q.empty + 8 * s, 1);
         }
-        for (int s = 0; s < bufs(kPair); ++s) {
+        for (int s = 0; s < Tile<kSide>::kBufs; ++s) {
             mbar_init(q.acc_full + 8 * s, 1);
-            mbar_init(q.acc_empty + 8 * s, kEpilogueWarps * kRanks);
+            mbar_init(q.acc_empty + 8 * s, Tile<kSide>::kWarps * Tile<kSide>::kRanks);
         }
         mbar_init(q.acc_full + 64, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if ((threadIdx.x >> 5) == kEpilogueWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), kTmemColumns);
+    if ((threadIdx.x >> 5) == Tile<kSide>::kWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), Tile<kSide>::kColumns);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if constexpr (kPair) cluster_sync();
@@ -846,100 +881,125 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
 
 // Nothing may be in flight when the CTA leaves: copies (a pair's are all
 // counted in the first CTA), products.  All threads.
-template <bool kPair>
+template <int kSide>
 __device__ __forceinline__ void pipe_close(Pipe& q) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    if (warp == kEpilogueWarps && lane == 0 && q.rank == 0) {
+    constexpr bool kPair = Tile<kSide>::kPair;
+    constexpr int kWarps = Tile<kSide>::kWarps, kStages = Tile<kSide>::kStages;
+    const int warp = threadIdx.x >> 5;
+    if (warp == kWarps && q.rank == 0) {
         for (int s = 0; s < kStages; ++s) {
             const int fills = (q.fill - s + kStages - 1) / kStages;
             if (fills > 0) mbar_wait(q.full + 8 * s, (fills - 1) & 1);
         }
-    } else if (warp == kEpilogueWarps + 1 && lane == 0 && q.rank == 0) {
-        mma_commit<kPair>(q.acc_full + 64);
+    } else if (warp == kWarps + 1 && q.rank == 0) {
+        if (elect_one()) mma_commit<kPair>(q.acc_full + 64);
+        __syncwarp();
         mbar_wait(q.acc_full + 64, 0);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if constexpr (kPair) cluster_sync();  // the other CTA may still signal or read here
-    if (warp == kEpilogueWarps + 1) {
+    if (warp == kWarps + 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_free<kPair>(q.tmem, kTmemColumns);
+        tmem_free<kPair>(q.tmem, Tile<kSide>::kColumns);
     }
 }
 
 // One product of all matrices, a persistent loop over its tiles.
-template <int M, bool kPair>
-__global__ void __launch_bounds__(kGemmThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
-                                                                  const __grid_constant__ CUtensorMap right,
-                                                                  const __grid_constant__ Product p,
-                                                                  const __grid_constant__ Result result, int batch, int tiles) {
+template <int M, int kSide>
+__global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
+                                                                           const __grid_constant__ CUtensorMap right,
+                                                                           const __grid_constant__ Product p,
+                                                                           const __grid_constant__ Result result, int batch,
+                                                                           int tiles) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 9];
     __shared__ uint32_t tmem_slot;
     Pipe q;
-    pipe_open<kPair>(q, bars, &tmem_slot, smem_raw);
+    pipe_open<kSide>(q, bars, &tmem_slot, smem_raw);
     chain();
-    constexpr int kRanks = kPair ? 2 : 1;
-    product<M, kPair>(q, &left, &right, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
-    pipe_close<kPair>(q);
+    constexpr int kRanks = Tile<kSide>::kRanks;
+    product<M, kSide>(q, &left, &right, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
+    pipe_close<kSide>(q);
 }
 
-// All steps of one matrix by one cluster: the products of a small matrix are
-// a few microseconds each, less than it takes to end one kernel and start the
-// next, so here a cluster barrier stands between them.
+// All steps in one kernel, for matrices whose products are a few microseconds
+// each, less than it takes to end one kernel and start the next: `group` CTAs work on
+// a matrix with 64 x 64 tiles and meet between its products.  A cooperative
+// launch, so that all of them are resident while they wait for one another.
 struct Steps {
     Product gram, square, apply;    // square.rows = 0: c = 0, no square
     __half* x[2];
-    int steps;
+    unsigned* arrivals;             // per matrix, zeroed by ns_norm_kernel
+    int steps, group;
 };
 struct StepMaps {
-    CUtensorMap x[2], right[2], b, p;
+    CUtensorMap x[2], b, p;
 };
-__global__ void __launch_bounds__(kGemmThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
-                                                                   const __grid_constant__ Steps st,
-                                                                   const __grid_constant__ Result result, int batch) {
-    extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kStages + 9];
-    __shared__ uint32_t tmem_slot;
-    Pipe q;
-    pipe_open<false>(q, bars, &tmem_slot, smem_raw);
-    chain();
-    uint32_t size;
-    asm("mov.u32 %0, %%cluster_nctarank;" : "=r"(size));
-    const int matrix = blockIdx.x / size;
-    const int ni = (st.gram.rows + kTile - 1) / kTile, nj = (st.apply.cols + kTile - 1) / kTile;
-    const int triangle_tiles = ni * (ni + 1) / 2, all_tiles = ni * nj;
-    const auto ends = [&](int tiles, int& first, int& end) {
-        first = matrix * tiles + (int)cluster_rank();
-        end = (matrix + 1) * tiles;
-    };
-    // planes are written by ordinary stores and read by copies of the other CTAs
-    const auto next = [&]() {
-        asm volatile("fence.proxy.async.global;" ::: "memory");
-        cluster_sync();
-        if (threadIdx.x == kEpilogueWarps * 32) asm volatile("fence.proxy.async.global;" ::: "memory");
-    };
-    for (int k = 0; k < st.steps; ++k) {
-        int first, end;
-        ends(triangle_tiles, first, end);
-        product<kSymmetric, false>(q, &maps.x[k & 1], &maps.x[k & 1], st.gram, nullptr, batch, first, size, end);
-        next();
-        if (st.square.rows) {
-            product<kSymmetric, false>(q, &maps.b, &maps.b, st.square, nullptr, batch, first, size, end);
-            next();
-        }
-        ends(all_tiles, first, end);
-        if (k + 1 < st.steps) {
-            Product p = st.apply;
-            p.out = st.x[(k + 1) & 1];
-            product<kApply, false>(q, &maps.p, &maps.right[k & 1], p, nullptr, batch, first, size, end);
-            next();
-        } else {
-            product<kResult, false>(q, &maps.p, &maps.right[k & 1], st.apply, &result, batch, first, size, end);
+
+// All CTAs of a matrix have finished a product: planes are written by ordinary
+// stores and read by copies of the other CTAs.  For two seconds at most.
+__device__ __forceinline__ void group_meet(unsigned* arrivals, unsigned target, unsigned group, Pipe& q, int* lost) {
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    __syncthreads();
+    if (group > 1 && threadIdx.x == 0) {
+        __threadfence();
+        atomicAdd(arrivals, 1u);
+        unsigned long long began = 0;
+        for (;;) {
+            unsigned seen;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(arrivals) : "memory");
+            if (seen >= target) break;
+            const unsigned long long now = wall_ns();
+            if (!began) began = now;
+            else if (now - began > 2000000000ull) {
+                *lost = 1;
+                break;
+            }
         }
     }
-    pipe_close<false>(q);
+    __syncthreads();
+    if (*lost) q.ok = false;
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+}
+
+__global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
+                                                                         const __grid_constant__ Steps st,
+                                                                         const __grid_constant__ Result result, int batch) {
+    extern __shared__ uint8_t smem_raw[];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 9];
+    __shared__ uint32_t tmem_slot;
+    __shared__ int lost;
+    if (threadIdx.x == 0) lost = 0;
+    Pipe q;
+    pipe_open<64>(q, bars, &tmem_slot, smem_raw);
+    const int ni = (st.gram.rows + 63) / 64, nj = (st.apply.cols + 63) / 64;
+    const int half = ni * (ni + 1) / 2, all = ni * nj, rank = blockIdx.x % st.group;
+    const int groups = gridDim.x / st.group;
+    for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
+        unsigned target = 0;
+        const auto meet = [&]() { group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost); };
+        const int half0 = matrix * half + rank, half1 = (matrix + 1) * half;
+        const int all0 = matrix * all + rank, all1 = (matrix + 1) * all;
+        for (int k = 0; k < st.steps; ++k) {
+            product<kSymmetric, 64>(q, &maps.x[k & 1], &maps.x[k & 1], st.gram, nullptr, batch, half0, st.group, half1);
+            meet();
+            if (st.square.rows) {
+                product<kSymmetric, 64>(q, &maps.b, &maps.b, st.square, nullptr, batch, half0, st.group, half1);
+                meet();
+            }
+            if (k + 1 < st.steps) {
+                Product p = st.apply;
+                p.out = st.x[(k + 1) & 1];
+                product<kApply, 64>(q, &maps.p, &maps.x[k & 1], p, nullptr, batch, all0, st.group, all1);
+                meet();
+            } else {
+                product<kResult, 64>(q, &maps.p, &maps.x[k & 1], st.apply, &result, batch, all0, st.group, all1);
+            }
+        }
+    }
+    pipe_close<64>(q);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -979,7 +1039,7 @@ int plane_map(EncodeFn encode, CUtensorMap* map, __half* base, int batch, int ro
 struct Layout {
     int m, n, xp, ap;               // sides (m <= n) and pitches
     int parts;                      // partial norms per matrix: one per 4096 elements
-    size_t part, x0, x1, a, p, bytes;
+    size_t part, arrivals, x0, x1, a, p, bytes;
     long long x_plane, a_plane;     // elements
 
     Layout(int batch, int rows, int cols) {
@@ -998,6 +1058,7 @@ struct Layout {
         const long long want = ((long long)rows * cols + 4095) / 4096;
         parts = want < kMaxParts ? (int)want : kMaxParts;
         part = take((size_t)batch * parts * sizeof(double));
+        arrivals = take((size_t)batch * sizeof(unsigned));
         x0 = take((size_t)x_plane * 4);
         x1 = take((size_t)x_plane * 4);
         a = take((size_t)a_plane * 4);
@@ -1076,16 +1137,16 @@ int launch_chained(const char* what, void (*kernel)(Args...), dim3 grid, int thr
     return fail(CIMEKV_ECUDA, msg);
 }
 
-template <int M, bool kPair>
+template <int M, int kSide>
 int launch_as(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
               cudaStream_t s) {
     const cudaError_t e =
-        cudaFuncSetAttribute(ns_gemm_kernel<M, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
+        cudaFuncSetAttribute(ns_gemm_kernel<M, kSide>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kSide>::kSmem);
     if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
-    constexpr int ranks = kPair ? 2 : 1;
-    const long long tiles = tile_count(M, kTile * ranks, p.rows, p.cols) * batch, most = sms / ranks;
-    return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kPair>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
-                          kGemmThreads, kSmemBytes, ranks, s, l, r, p, result, batch, (int)tiles);
+    constexpr int ranks = Tile<kSide>::kRanks;
+    const long long tiles = tile_count(M, kSide, p.rows, p.cols) * batch, most = sms / ranks;
+    return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kSide>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
+                          Tile<kSide>::kThreads, Tile<kSide>::kSmem, ranks, s, l, r, p, result, batch, (int)tiles);
 }
 
 // Pairs once single tiles would fill every SM anyway: the larger tile halves
@@ -1093,16 +1154,21 @@ int launch_as(const CUtensorMap& l, const CUtensorMap& r, const Product& p, cons
 template <int M>
 int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
                 cudaStream_t s) {
-    return tile_count(M, kTile, p.rows, p.cols) * batch > sms ? launch_as<M, true>(l, r, p, result, batch, sms, s)
-                                                              : launch_as<M, false>(l, r, p, result, batch, sms, s);
+    return tile_count(M, 128, p.rows, p.cols) * batch > sms ? launch_as<M, 256>(l, r, p, result, batch, sms, s)
+                                                            : launch_as<M, 128>(l, r, p, result, batch, sms, s);
 }
 
 // CTAs per matrix when all steps run in one kernel, 0 when each product is its own.
-int steps_cluster(int batch, int m, int n, int sms) {
-    const long long tiles = tile_count(kApply, kTile, m, n);
-    static const char* force = getenv("NS_CLUSTER");
-    if (force) return (int)std::min<long long>(tiles, atoi(force));
-    return 0;
+int steps_group(int batch, int m, int n, int sms) {
+    const long long tiles = tile_count(kApply, 64, m, n), slots = sms;
+    static const char* force = getenv("NS_GROUP");
+    if (force && atoi(force) == 0) return 0;
+    if (force && atoi(force) > 0) return (int)std::min<long long>(tiles, atoi(force));
+    long long most = slots / batch;
+    if (most < 1) most = 1;
+    if (most > tiles) most = tiles;
+    const long long rounds = (tiles + most - 1) / most;
+    return (int)((tiles + rounds - 1) / rounds);
 }
 
 int type_bytes(int type) { return type == CIMEKV_F32 ? 4 : 2; }
@@ -1134,13 +1200,6 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     __half* x[2] = {reinterpret_cast<__half*>(ws + lay.x0), reinterpret_cast<__half*>(ws + lay.x1)};
     __half* am = reinterpret_cast<__half*>(ws + lay.a);
     __half* pm = reinterpret_cast<__half*>(ws + lay.p);
-    StepMaps maps;  // X as rows along K (Gram) and as the right operand whose rows are K (apply)
-    for (int i = 0; i < 2; ++i) {
-        if ((rc = plane_map(encode, &maps.x[i], x[i], batch, lay.m, lay.n, lay.xp, kTile))) return rc;
-        if ((rc = plane_map(encode, &maps.right[i], x[i], batch, lay.m, lay.n, lay.xp, kK))) return rc;
-    }
-    if ((rc = plane_map(encode, &maps.b, am, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
-    if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, kTile))) return rc;
 
     prep.rows = rows;
     prep.cols = cols;
@@ -1149,6 +1208,7 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     prep.plane = lay.x_plane;
     prep.parts = lay.parts;
     prep.part = reinterpret_cast<double*>(ws + lay.part);
+    prep.arrivals = reinterpret_cast<unsigned*>(ws + lay.arrivals);
     prep.x = x[0];
     const bool vec = rows_in_fours(prep.g, batch, cols) && rows_in_fours(prep.mom, batch, cols);
     const bool flat = vec && (prep.g.row_stride == cols || rows == 1);
@@ -1193,21 +1253,45 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     result.transposed = prep.transposed;
     result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
 
-    const int cluster = steps_cluster(batch, lay.m, lay.n, sms);
-    if (cluster) {
-        cudaError_t e = cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-        if (e == cudaSuccess && cluster > 8)
-            e = cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
-        if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
-        return launch_chained("ns_steps_kernel", ns_steps_kernel, dim3((unsigned)batch * cluster), kGemmThreads,
-                              kSmemBytes, cluster, s, maps, st, result, batch);
+    if (const int group = steps_group(batch, lay.m, lay.n, sms)) {
+        StepMaps maps;
+        for (int i = 0; i < 2; ++i)
+            if ((rc = plane_map(encode, &maps.x[i], x[i], batch, lay.m, lay.n, lay.xp, 64))) return rc;
+        if ((rc = plane_map(encode, &maps.b, am, batch, lay.m, lay.m, lay.ap, 64))) return rc;
+        if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, 64))) return rc;
+        cudaError_t e =
+            cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<64>::kSmem);
+        st.arrivals = prep.arrivals;
+        st.group = group;
+        const int most = sms / group;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)(batch < most ? batch : most) * group);
+        cfg.blockDim = dim3(Tile<64>::kThreads);
+        cfg.dynamicSmemBytes = Tile<64>::kSmem;
+        cfg.stream = s;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeCooperative;
+        attr[0].val.cooperative = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, ns_steps_kernel, maps, st, result, batch);
+        if (e == cudaSuccess) return CIMEKV_OK;
+        (void)cudaGetLastError();
+        return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
     }
+    CUtensorMap xleft[2], xright[2], bmap, pmap;  // X as rows along K (Gram) and as the right operand whose rows are K
+    for (int i = 0; i < 2; ++i) {
+        if ((rc = plane_map(encode, &xleft[i], x[i], batch, lay.m, lay.n, lay.xp, 128))) return rc;
+        if ((rc = plane_map(encode, &xright[i], x[i], batch, lay.m, lay.n, lay.xp, kK))) return rc;
+    }
+    if ((rc = plane_map(encode, &bmap, am, batch, lay.m, lay.m, lay.ap, 128))) return rc;
+    if ((rc = plane_map(encode, &pmap, pm, batch, lay.m, lay.m, lay.ap, 128))) return rc;
     for (int k = 0; k < steps; ++k) {
-        if ((rc = launch_gemm<kSymmetric>(maps.x[k & 1], maps.x[k & 1], st.gram, result, batch, sms, s))) return rc;
-        if (squared && (rc = launch_gemm<kSymmetric>(maps.b, maps.b, st.square, result, batch, sms, s))) return rc;
+        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], st.gram, result, batch, sms, s))) return rc;
+        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, st.square, result, batch, sms, s))) return rc;
         st.apply.out = x[(k + 1) & 1];
-        rc = k + 1 < steps ? launch_gemm<kApply>(maps.p, maps.right[k & 1], st.apply, result, batch, sms, s)
-                           : launch_gemm<kResult>(maps.p, maps.right[k & 1], st.apply, result, batch, sms, s);
+        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], st.apply, result, batch, sms, s)
+                           : launch_gemm<kResult>(pmap, xright[k & 1], st.apply, result, batch, sms, s);
         if (rc) return rc;
     }
     return CIMEKV_OK;
