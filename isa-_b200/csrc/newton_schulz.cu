@@ -168,6 +168,20 @@ __device__ __forceinline__ void tma_box(uint32_t dst, const CUtensorMap* map, in
             : "memory");
 }
 
+// A warp's box of 32 columns from its staging place to a plane, and the wait until
+// the place may be written again (all: until the planes are written).
+__device__ __forceinline__ void tma_store(const CUtensorMap* map, uint32_t src, int x, int y, int z) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.global.shared::cta.tile.bulk_group [%0, {%2, %3, %4}], [%1];\n\t"
+        "cp.async.bulk.commit_group;" ::"l"(map), "r"(src), "r"(x), "r"(y), "r"(z)
+        : "memory");
+}
+template <bool kAll>
+__device__ __forceinline__ void tma_store_wait() {
+    if constexpr (kAll) asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+    else asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory");
+}
+
 // One lane of a converged warp.  The copy and product warps run whole, with values
 // that are the same in all lanes, and only issue from one: coordinates and
 // descriptors then live in uniform registers, where these instructions want them
@@ -496,15 +510,14 @@ __global__ void __launch_bounds__(256) ns_prepare_tall_kernel(const __grid_const
 
 // ---------------------------------------------------------------- products --
 
-// kSymmetric: alpha L L^T + beta I, one triangle; kApply: L R; kResult: L R to the caller's matrices.
-enum Mode { kSymmetric = 0, kApply = 1, kResult = 2 };
+// kSymmetric: alpha L L^T + beta I, one triangle and its mirror image; kFull: the same, all
+// tiles; kApply: L R; kResult: L R to the caller's matrices.
+enum Mode { kSymmetric = 0, kFull = 1, kApply = 2, kResult = 3 };
+__host__ __device__ constexpr bool is_square(int mode) { return mode <= kFull; }
 
 // One product of a batch.
 struct Product {
     int rows, cols, depth;
-    __half* out;            // planes of the result (not kResult)
-    long long out_plane;    // elements from hi to lo
-    int out_pitch;
     float alpha, beta;      // on values as the planes hold them
 };
 
@@ -620,13 +633,16 @@ __device__ __forceinline__ void finish_result(const Result& p, int rows, int col
 }
 
 // 32 columns from cb of the warp's kRows rows from row0 of a product that stays in
-// planes, and their mirror image off the diagonal of a symmetric one.  Called by
-// whole warps.
-template <bool kSym, int kRows>
-__device__ __forceinline__ void finish_planes(const Product& p, const float (&v0)[16], const float (&v1)[16], int b,
-                                              int row0, int cb, bool diagonal, uint32_t staging) {
+// planes (kDiagonal: plus beta on the diagonal; kMirror: and their mirror image off
+// it).  Rows of 64 bytes are staged in the 64-byte swizzle of `out` and leave by a
+// bulk copy, which clips them to the matrix and lets the warp go on: ordinary stores of
+// a 256 x 256 tile took 8,000 cycles, in which the products ran out of accumulators.
+// Called by whole warps.
+template <bool kDiagonal, bool kMirror, int kRows>
+__device__ __forceinline__ void finish_planes(const Product& p, const CUtensorMap* out, const float (&v0)[16],
+                                              const float (&v1)[16], int batch, int b, int row0, int cb, bool diagonal,
+                                              uint32_t staging) {
     const int lane = threadIdx.x & 31, r = row0 + lane;
-    __half* matrix = p.out + (long long)b * p.rows * p.out_pitch;
     uint32_t words[2][16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -634,37 +650,42 @@ __device__ __forceinline__ void finish_planes(const Product& p, const float (&v0
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             o[k] = (i < 8 ? v0[(2 * i + k) & 15] : v1[(2 * i + k) & 15]) * p.alpha;
-            if (kSym && diagonal && r == cb + 2 * i + k) o[k] += p.beta;
+            if (kDiagonal && diagonal && r == cb + 2 * i + k) o[k] += p.beta;
         }
         split2(o[0], o[1], words[0][i], words[1][i]);
     }
+    const auto leave = [&](int x, int y, int plane) {
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        __syncwarp();
+        if (lane == 0) tma_store(out, staging, x, y, plane * batch + b);
+    };
+    const auto place_free = [&]() {
+        if (lane == 0) tma_store_wait<false>();
+        __syncwarp();
+    };
+    if (row0 >= p.rows) return;
 #pragma unroll
     for (int plane = 0; plane < 2; ++plane) {
         const uint32_t(&w)[16] = words[plane];
-        uint4 in[4], out[kRows / 8];
+        place_free();
+        if (kRows == 32 || lane < kRows) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) in[k] = make_uint4(w[4 * k], w[4 * k + 1], w[4 * k + 2], w[4 * k + 3]);
-        turn_rows<kRows>(staging, in, out);
-        const int c = cb + (lane & 3) * 8;
-#pragma unroll
-        for (int t = 0; t < kRows / 8; ++t) {
-            const int row = row0 + 8 * t + (lane >> 2);
-            // the pitch is a multiple of 8: a group that begins inside a row ends inside its pitch
-            if (row < p.rows && c < p.cols)
-                *reinterpret_cast<uint4*>(matrix + plane * p.out_plane + (long long)row * p.out_pitch + c) = out[t];
-        }
-        if (kSym && !diagonal) {
-            // lanes 2k and 2k + 1 exchange, so that the even one holds both rows of an
-            // even column and the odd one those of the next: 32-bit stores along rows
-            const int odd = lane & 1, r2 = r & ~1;
-            __half* mirror = matrix + plane * p.out_plane + (long long)(cb + odd) * p.out_pitch + r2;
-            const uint32_t sel = odd ? 0x3276u : 0x5410u;  // halves {mine, its} of the even, {its, mine} of the odd column
-#pragma unroll
-            for (int i = 0; i < 16; ++i) {
-                const uint32_t other = __shfl_xor_sync(0xffffffffu, w[i], 1);
-                if (lane < kRows && r2 < p.rows && cb + 2 * i + odd < p.cols)
-                    *reinterpret_cast<uint32_t*>(mirror + (long long)(2 * i) * p.out_pitch) = __byte_perm(w[i], other, sel);
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = staging + lane * 64 + ((k ^ ((lane >> 1) & 3)) << 4);
+                asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[4 * k]), "r"(w[4 * k + 1]),
+                             "r"(w[4 * k + 2]), "r"(w[4 * k + 3])
+                             : "memory");
             }
+        }
+        leave(cb, row0, plane);
+        if (kMirror && !diagonal) {  // row c of the image: element c of all lanes
+            place_free();
+#pragma unroll
+            for (int c = 0; c < 32; ++c) {
+                const uint32_t at = staging + c * 64 + (((lane >> 3) ^ ((c >> 1) & 3)) << 4) + (lane & 7) * 2;
+                asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"((unsigned short)(w[c / 2] >> (16 * (c & 1)))) : "memory");
+            }
+            leave(row0, cb, plane);
         }
     }
 }
@@ -694,8 +715,8 @@ struct Pipe {
 // them in registers with round-to-nearest while the next ones run.  The same
 // accumulators let the next tile start while the last one is stored.
 template <int M, int kSide>
-__device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right, const Product& p,
-                                        const Result* result, int batch, int first, int step, int tiles) {
+__device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
+                                        const CUtensorMap* out, const Product& p, const Result* result, int batch, int first, int step, int tiles) {
     using T = Tile<kSide>;
     constexpr bool kPair = T::kPair;
     constexpr int kRanks = T::kRanks, kRows = T::kRows, kOperand = T::kOperand, kStageBytes = T::kStageBytes;
@@ -724,7 +745,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
         for (int t = first; t < tiles && q.ok; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
-            const bool same = M == kSymmetric && row0 == col0;  // both operands are the same rows
+            const bool same = is_square(M) && row0 == col0;  // both operands are the same rows
             row0 += (int)q.rank * kRows;
             col0 += (int)q.rank * kRows;
             for (int k = 0; k < ksteps; ++k, ++q.fill) {
@@ -739,7 +760,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                         const uint32_t l = base + plane * kOperand, r = base + (2 + plane) * kOperand;
                         tma_box<kPair>(l, left, k * kK, row0, z, bar);
                         if (same) continue;
-                        if (M == kSymmetric) {
+                        if (is_square(M)) {
                             tma_box<kPair>(r, right, k * kK, col0, z, bar);
                         } else {
                             tma_box<kPair>(r, right, col0, k * kK, z, bar);
@@ -753,12 +774,12 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
     } else if (warp == kWarps + 1) {
         if (q.rank == 0) {
             // D fp32, A and B fp16; right operand along K (0) or along its own axis (1)
-            const uint32_t idesc = 1u << 4 | (M == kSymmetric ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
+            const uint32_t idesc = 1u << 4 | (is_square(M) ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
                                    (uint32_t)(kSide / 16) << 24;
             for (int t = first; t < tiles && q.ok; t += step) {
                 int b, row0, col0;
                 place(t, b, row0, col0);
-                const int r_at = M == kSymmetric && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
+                const int r_at = is_square(M) && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
                 for (int k = 0; k < ksteps && q.ok; ++q.chunk) {
                     const int buf = q.chunk % kBufs;
                     if (q.chunk >= kBufs && !(q.ok = mbar_wait(q.acc_empty + 8 * buf, (q.chunk / kBufs - 1) & 1))) break;
@@ -771,9 +792,9 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                         const uint32_t base = q.stages + s * kStageBytes;
                         // both planes of either operand; a step of 16 along K moves the address alone
                         const uint64_t l0 = operand_desc(base, 16, 1024), l1 = operand_desc(base + kOperand, 16, 1024);
-                        const uint64_t r0 = operand_desc(base + r_at, M == kSymmetric ? 16 : 8192, 1024);
-                        const uint64_t r1 = operand_desc(base + r_at + kOperand, M == kSymmetric ? 16 : 8192, 1024);
-                        constexpr uint64_t kL = 32 >> 4, kR = (M == kSymmetric ? 32 : 2048) >> 4;
+                        const uint64_t r0 = operand_desc(base + r_at, is_square(M) ? 16 : 8192, 1024);
+                        const uint64_t r1 = operand_desc(base + r_at + kOperand, is_square(M) ? 16 : 8192, 1024);
+                        constexpr uint64_t kL = 32 >> 4, kR = (is_square(M) ? 32 : 2048) >> 4;
                         if (elect_one()) {
 #pragma unroll
                             for (uint64_t i = 0; i < kK / 16; ++i) {
@@ -839,10 +860,12 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                 if constexpr (M == kResult)
                     finish_result<T::kWarpRows>(*result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
                 else if (g % 2 == 0)
-                    finish_planes<M == kSymmetric, T::kWarpRows>(p, acc[g], acc[g + 1], b, r0, col0 + g * 16, diagonal, staging);
+                    finish_planes<is_square(M), M == kSymmetric, T::kWarpRows>(p, out, acc[g], acc[g + 1], batch, b, r0, col0 + g * 16, diagonal, staging);
             }
             __syncwarp();
         }
+        if (M != kResult && lane == 0) tma_store_wait<true>();
+        __syncwarp();
     }
 }
 
@@ -910,6 +933,7 @@ __device__ __forceinline__ void pipe_close(Pipe& q) {
 template <int M, int kSide>
 __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
                                                                            const __grid_constant__ CUtensorMap right,
+                                                                           const __grid_constant__ CUtensorMap out,
                                                                            const __grid_constant__ Product p,
                                                                            const __grid_constant__ Result result, int batch,
                                                                            int tiles) {
@@ -920,7 +944,7 @@ __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const
     pipe_open<kSide>(q, bars, &tmem_slot, smem_raw);
     chain();
     constexpr int kRanks = Tile<kSide>::kRanks;
-    product<M, kSide>(q, &left, &right, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
+    product<M, kSide>(q, &left, &right, &out, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
     pipe_close<kSide>(q);
 }
 
@@ -930,12 +954,12 @@ __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const
 // launch, so that all of them are resident while they wait for one another.
 struct Steps {
     Product gram, square, apply;    // square.rows = 0: c = 0, no square
-    __half* x[2];
     unsigned* arrivals;             // per matrix, zeroed by ns_norm_kernel
     int steps, group;
 };
 struct StepMaps {
-    CUtensorMap x[2], b, p;
+    CUtensorMap x[2], b, p;                 // to read from, boxes of 64 rows
+    CUtensorMap x_out[2], b_out, p_out;     // to write to, boxes of a warp's rows
 };
 
 // All CTAs of a matrix have finished a product: planes are written by ordinary
@@ -975,27 +999,26 @@ __global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const _
     Pipe q;
     pipe_open<64>(q, bars, &tmem_slot, smem_raw);
     const int ni = (st.gram.rows + 63) / 64, nj = (st.apply.cols + 63) / 64;
-    const int half = ni * (ni + 1) / 2, all = ni * nj, rank = blockIdx.x % st.group;
-    const int groups = gridDim.x / st.group;
+    const int square = ni * ni, all = ni * nj, rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
     for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
         unsigned target = 0;
         const auto meet = [&]() { group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost); };
-        const int half0 = matrix * half + rank, half1 = (matrix + 1) * half;
+        const int square0 = matrix * square + rank, square1 = (matrix + 1) * square;
         const int all0 = matrix * all + rank, all1 = (matrix + 1) * all;
         for (int k = 0; k < st.steps; ++k) {
-            product<kSymmetric, 64>(q, &maps.x[k & 1], &maps.x[k & 1], st.gram, nullptr, batch, half0, st.group, half1);
+            // all tiles: storing mirror images takes a CTA longer than a tile that another one has time for
+            product<kFull, 64>(q, &maps.x[k & 1], &maps.x[k & 1], st.square.rows ? &maps.b_out : &maps.p_out,
+                                 st.gram, nullptr, batch, square0, st.group, square1);
             meet();
             if (st.square.rows) {
-                product<kSymmetric, 64>(q, &maps.b, &maps.b, st.square, nullptr, batch, half0, st.group, half1);
+                product<kFull, 64>(q, &maps.b, &maps.b, &maps.p_out, st.square, nullptr, batch, square0, st.group, square1);
                 meet();
             }
             if (k + 1 < st.steps) {
-                Product p = st.apply;
-                p.out = st.x[(k + 1) & 1];
-                product<kApply, 64>(q, &maps.p, &maps.x[k & 1], p, nullptr, batch, all0, st.group, all1);
+                product<kApply, 64>(q, &maps.p, &maps.x[k & 1], &maps.x_out[(k + 1) & 1], st.apply, nullptr, batch, all0, st.group, all1);
                 meet();
             } else {
-                product<kResult, 64>(q, &maps.p, &maps.x[k & 1], st.apply, &result, batch, all0, st.group, all1);
+                product<kResult, 64>(q, &maps.p, &maps.x[k & 1], nullptr, st.apply, &result, batch, all0, st.group, all1);
             }
         }
     }
@@ -1024,13 +1047,16 @@ int encoder(EncodeFn* out) {
     return CIMEKV_OK;
 }
 
-// Planes [2 * batch][rows][cols] of a given pitch, boxes of 64 columns, zeros outside.
-int plane_map(EncodeFn encode, CUtensorMap* map, __half* base, int batch, int rows, int cols, int pitch, int box_rows) {
+// Planes [2 * batch][rows][cols] of a given pitch, zeros outside.
+// To read: 64 columns, 128-byte swizzle; to write: 32 columns, 64-byte swizzle.
+int plane_map(EncodeFn encode, CUtensorMap* map, __half* base, int batch, int rows, int cols, int pitch, int box_rows,
+              bool write = false) {
     const cuuint64_t dims[3] = {(cuuint64_t)cols, (cuuint64_t)rows, (cuuint64_t)2 * batch};
     const cuuint64_t strides[2] = {(cuuint64_t)pitch * 2, (cuuint64_t)pitch * 2 * rows};
-    const cuuint32_t box[3] = {64, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
+    const cuuint32_t box[3] = {write ? 32u : 64u, (cuuint32_t)box_rows, 1}, step[3] = {1, 1, 1};
     const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, base, dims, strides, box, step,
-                              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                              CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              write ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? CIMEKV_OK : fail(CIMEKV_ECUDA, "cuTensorMapEncodeTiled refused a plane");
 }
@@ -1138,7 +1164,7 @@ int launch_chained(const char* what, void (*kernel)(Args...), dim3 grid, int thr
 }
 
 template <int M, int kSide>
-int launch_as(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
+int launch_as(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result, int batch, int sms,
               cudaStream_t s) {
     const cudaError_t e =
         cudaFuncSetAttribute(ns_gemm_kernel<M, kSide>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kSide>::kSmem);
@@ -1146,29 +1172,49 @@ int launch_as(const CUtensorMap& l, const CUtensorMap& r, const Product& p, cons
     constexpr int ranks = Tile<kSide>::kRanks;
     const long long tiles = tile_count(M, kSide, p.rows, p.cols) * batch, most = sms / ranks;
     return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kSide>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
-                          Tile<kSide>::kThreads, Tile<kSide>::kSmem, ranks, s, l, r, p, result, batch, (int)tiles);
+                          Tile<kSide>::kThreads, Tile<kSide>::kSmem, ranks, s, l, r, out, p, result, batch, (int)tiles);
 }
 
-// Pairs once single tiles would fill every SM anyway: the larger tile halves
-// the operand traffic; below that the smaller one spreads over more SMs.
+// What a product takes, in cycles: a part that does not depend on its size (launch
+// or meeting, latencies) and the tiles of the busiest SM, so many cycles a stage
+// and a tile.  Fitted to times of single matrices of 64 to 1,280 rows and of
+// batches of 8 to 200 matrices of 64 to 768 (within 15 %).
+struct Cost {
+    double start, stage, tile;
+    double of(long long rounds, int depth) const { return start + rounds * (stage * ((depth + 63) / 64) + tile); }
+};
+constexpr Cost kCost64 = {6000, 900, 300}, kCost128 = {9200, 1420, 500}, kCost256 = {9200, 1600, 3000};
+
+long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
+
+double cost_of(int side, int mode, int rows, int cols, int depth, int batch, int sms) {
+    const Cost& c = side == 256 ? kCost256 : kCost128;
+    return c.of(ceil_div(tile_count(mode, side, rows, cols) * batch, side == 256 ? sms / 2 : sms), depth);
+}
+
 template <int M>
-int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const Product& p, const Result& result, int batch, int sms,
+int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result, int batch, int sms,
                 cudaStream_t s) {
-    return tile_count(M, 128, p.rows, p.cols) * batch > sms ? launch_as<M, 256>(l, r, p, result, batch, sms, s)
-                                                            : launch_as<M, 128>(l, r, p, result, batch, sms, s);
+    const bool pair = cost_of(256, M, p.rows, p.cols, p.depth, batch, sms) < cost_of(128, M, p.rows, p.cols, p.depth, batch, sms);
+    return pair ? launch_as<M, 256>(l, r, out, p, result, batch, sms, s) : launch_as<M, 128>(l, r, out, p, result, batch, sms, s);
 }
 
-// CTAs per matrix when all steps run in one kernel, 0 when each product is its own.
-int steps_group(int batch, int m, int n, int sms) {
-    const long long tiles = tile_count(kApply, 64, m, n), slots = sms;
-    static const char* force = getenv("NS_GROUP");
-    if (force && atoi(force) == 0) return 0;
-    if (force && atoi(force) > 0) return (int)std::min<long long>(tiles, atoi(force));
-    long long most = slots / batch;
-    if (most < 1) most = 1;
-    if (most > tiles) most = tiles;
-    const long long rounds = (tiles + most - 1) / most;
-    return (int)((tiles + rounds - 1) / rounds);
+// CTAs per matrix when all steps run in one kernel, 0 where a kernel for each
+// product costs less.  Measured, one kernel against fifteen: 73 against 114 us for
+// one 192 x 192 matrix, 146 against 214 for 768 x 768, 83 against 95 for 200 of
+// 64 x 64; 283 against 258 for 1024 x 1024, 196 against 161 for 12 of 384 x 384.
+int steps_group(int batch, int m, int n, bool squared, int sms) {
+    const long long tiles = tile_count(kApply, 64, m, n), most = std::max(1LL, std::min<long long>(tiles, sms / batch));
+    const long long group = ceil_div(tiles, ceil_div(tiles, most));  // no more than the rounds need
+    const long long turns = ceil_div(batch, std::max(1LL, sms / group));
+    const long long square = ceil_div(tile_count(kApply, 64, m, m), group);
+    const double together = turns * (kCost64.of(square, n) + (squared ? kCost64.of(square, m) : 0) +
+                                     kCost64.of(ceil_div(tiles, group), m));
+    const auto apart = [&](int mode, int cols, int depth) {
+        return std::min(cost_of(128, mode, m, cols, depth, batch, sms), cost_of(256, mode, m, cols, depth, batch, sms));
+    };
+    const double each = apart(kSymmetric, m, n) + (squared ? apart(kSymmetric, m, m) : 0) + apart(kApply, n, m);
+    return together <= each ? (int)group : 0;
 }
 
 int type_bytes(int type) { return type == CIMEKV_F32 ? 4 : 2; }
@@ -1229,36 +1275,33 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     const bool squared = c != 0.0f;
     Steps st = {};
     st.steps = steps;
-    st.x[0] = x[0];
-    st.x[1] = x[1];
     st.gram.rows = st.gram.cols = lay.m;
     st.gram.depth = lay.n;
-    st.gram.out = squared ? am : pm;
-    st.gram.out_plane = lay.a_plane;
-    st.gram.out_pitch = lay.ap;
     st.gram.alpha = (squared ? 1.0f : b) / kScale;
     st.gram.beta = (squared ? (float)(0.5 * b / c) : a) * kScale;
     if (squared) {
         st.square = st.gram;
         st.square.depth = lay.m;
-        st.square.out = pm;
         st.square.alpha = c / kScale;
         st.square.beta = (float)(a - 0.25 * (double)b * b / c) * kScale;
     }
     st.apply.rows = st.apply.depth = lay.m;
     st.apply.cols = lay.n;
-    st.apply.out_plane = lay.x_plane;
-    st.apply.out_pitch = lay.xp;
     st.apply.alpha = 1.0f / kScale;
     result.transposed = prep.transposed;
     result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
 
-    if (const int group = steps_group(batch, lay.m, lay.n, sms)) {
+    if (const int group = steps_group(batch, lay.m, lay.n, squared, sms)) {
         StepMaps maps;
-        for (int i = 0; i < 2; ++i)
+        constexpr int out_rows = Tile<64>::kWarpRows;
+        for (int i = 0; i < 2; ++i) {
             if ((rc = plane_map(encode, &maps.x[i], x[i], batch, lay.m, lay.n, lay.xp, 64))) return rc;
+            if ((rc = plane_map(encode, &maps.x_out[i], x[i], batch, lay.m, lay.n, lay.xp, out_rows, true))) return rc;
+        }
         if ((rc = plane_map(encode, &maps.b, am, batch, lay.m, lay.m, lay.ap, 64))) return rc;
         if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, 64))) return rc;
+        if ((rc = plane_map(encode, &maps.b_out, am, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
+        if ((rc = plane_map(encode, &maps.p_out, pm, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
         cudaError_t e =
             cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<64>::kSmem);
         st.arrivals = prep.arrivals;
@@ -1279,19 +1322,22 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
         (void)cudaGetLastError();
         return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
     }
-    CUtensorMap xleft[2], xright[2], bmap, pmap;  // X as rows along K (Gram) and as the right operand whose rows are K
+    // X as rows along K (Gram), as the right operand whose rows are K (apply), and to write
+    CUtensorMap xleft[2], xright[2], xout[2], bmap, pmap, bout, pout;
     for (int i = 0; i < 2; ++i) {
         if ((rc = plane_map(encode, &xleft[i], x[i], batch, lay.m, lay.n, lay.xp, 128))) return rc;
         if ((rc = plane_map(encode, &xright[i], x[i], batch, lay.m, lay.n, lay.xp, kK))) return rc;
+        if ((rc = plane_map(encode, &xout[i], x[i], batch, lay.m, lay.n, lay.xp, 32, true))) return rc;
     }
     if ((rc = plane_map(encode, &bmap, am, batch, lay.m, lay.m, lay.ap, 128))) return rc;
     if ((rc = plane_map(encode, &pmap, pm, batch, lay.m, lay.m, lay.ap, 128))) return rc;
+    if ((rc = plane_map(encode, &bout, am, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
+    if ((rc = plane_map(encode, &pout, pm, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
     for (int k = 0; k < steps; ++k) {
-        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], st.gram, result, batch, sms, s))) return rc;
-        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, st.square, result, batch, sms, s))) return rc;
-        st.apply.out = x[(k + 1) & 1];
-        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], st.apply, result, batch, sms, s)
-                           : launch_gemm<kResult>(pmap, xright[k & 1], st.apply, result, batch, sms, s);
+        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], squared ? bout : pout, st.gram, result, batch, sms, s))) return rc;
+        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, pout, st.square, result, batch, sms, s))) return rc;
+        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], xout[(k + 1) & 1], st.apply, result, batch, sms, s)
+                           : launch_gemm<kResult>(pmap, xright[k & 1], xout[0], st.apply, result, batch, sms, s);
         if (rc) return rc;
     }
     return CIMEKV_OK;
