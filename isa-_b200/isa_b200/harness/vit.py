@@ -19,6 +19,7 @@ import torch.nn.functional as F
 
 from isa_b200.device_models.config import make_flash_transistor_ekv_config
 from isa_b200.operators.cim import CIMLinear, PhysicalFFN
+from isa_b200.operators.norm import LayerNorm
 
 
 @dataclass
@@ -31,6 +32,7 @@ class ViTConfig:
     depth: int = 12
     mlp_ratio: float = 4.0
     lut_size: int = 8192  # vision configs pin EKV_LUT_SIZE=8192
+    fused_norm: bool = False  # layer norms and residual sums on this package's kernels
 
 
 class ViTBlock(nn.Module):
@@ -38,17 +40,23 @@ class ViTBlock(nn.Module):
         super().__init__()
         d = cfg.embed_dim
         self.heads = cfg.num_heads
-        self.norm1 = nn.LayerNorm(d)
+        self.fused_norm = cfg.fused_norm
+        norm = LayerNorm if cfg.fused_norm else nn.LayerNorm
+        self.norm1 = norm(d)
         self.qkv = nn.Linear(d, 3 * d)
         self.proj = nn.Linear(d, d)
-        self.norm2 = nn.LayerNorm(d)
+        self.norm2 = norm(d)
         self.mlp = PhysicalFFN(d, int(d * cfg.mlp_ratio), cim_cfg)
 
     def forward(self, x):
         b, t, d = x.shape
         q, k, v = self.qkv(self.norm1(x)).view(b, t, 3, self.heads, d // self.heads).unbind(2)
         a = F.scaled_dot_product_attention(q.transpose(1, 2), k.transpose(1, 2), v.transpose(1, 2))
-        x = x + self.proj(a.transpose(1, 2).reshape(b, t, d))
+        a = self.proj(a.transpose(1, 2).reshape(b, t, d))
+        if self.fused_norm:
+            normed, x = self.norm2.add(x, a)
+            return x + self.mlp(normed)
+        x = x + a
         return x + self.mlp(self.norm2(x))
 
 
@@ -64,7 +72,7 @@ class PhysicalViT(nn.Module):
         nn.init.trunc_normal_(self.pos_embed, std=0.02)
         nn.init.trunc_normal_(self.cls_token, std=0.02)
         self.blocks = nn.ModuleList(ViTBlock(cfg, cim_cfg) for _ in range(cfg.depth))
-        self.norm = nn.LayerNorm(cfg.embed_dim)
+        self.norm = (LayerNorm if cfg.fused_norm else nn.LayerNorm)(cfg.embed_dim)
         self.head = nn.Linear(cfg.embed_dim, cfg.num_classes)
 
     def forward(self, img):

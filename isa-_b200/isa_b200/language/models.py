@@ -20,7 +20,8 @@ keys, so a reference checkpoint loads unchanged:
   tied LM head.
 
 The CIM layers run on this package's sm_100a kernels; everything else is
-plain PyTorch.
+plain PyTorch, or with ``ModelConfig.fused_norm`` has its layer norms, joined with
+the residual sums in front of them, on them as well.
 """
 
 from __future__ import annotations
@@ -34,6 +35,7 @@ import torch.nn.functional as F
 
 from isa_b200.device_models.config import make_flash_transistor_ekv_config
 from isa_b200.operators.cim import CIMLinear, PhysicalFFN, VoltageMapping
+from isa_b200.operators.norm import LayerNorm
 
 # The language experiments pin the table size to 4096 (reference config.py:13;
 # EKV_LUT_SIZE in the environment still overrides it).
@@ -63,6 +65,7 @@ class ModelConfig:
     voltage_max: float = 4.0
     affine_scope: str = "final"
     output_chunk_size: int = 16
+    fused_norm: bool = False  # layer norms and residual sums on this package's kernels (no counterpart there)
 
     @classmethod
     def from_preset(cls, size: str, model_type: str, **kwargs) -> "ModelConfig":
@@ -116,17 +119,19 @@ class GPT2Block(nn.Module):
     """Pre-LayerNorm transformer block: causal attention, then the FFN variant."""
 
     def __init__(self, embed_dim: int, ffn_dim: int, num_heads: int, model_type: str, voltage_max: float = 4.0,
-                 dropout: float = 0.0, physical_config: Optional[Dict] = None):
+                 dropout: float = 0.0, physical_config: Optional[Dict] = None, fused_norm: bool = False):
         super().__init__()
         if embed_dim % num_heads:
             raise ValueError(f"embed_dim={embed_dim} must be divisible by num_heads={num_heads}")
         self.num_heads = num_heads
         self.head_dim = embed_dim // num_heads
-        self.ln1 = nn.LayerNorm(embed_dim)
+        norm = LayerNorm if fused_norm else nn.LayerNorm
+        self.ln1 = norm(embed_dim)
         # parameter container only (in_proj_weight/bias, out_proj); the forward
         # calls scaled_dot_product_attention on these weights directly
         self.attn = nn.MultiheadAttention(embed_dim, num_heads, dropout=dropout, batch_first=True)
-        self.ln2 = nn.LayerNorm(embed_dim)
+        self.ln2 = norm(embed_dim)
+        self.digital_ffn = model_type == "standard"
         if model_type == "standard":
             self.ffn = StandardFFN(embed_dim, ffn_dim, dropout)
         elif model_type == "hybrid":
@@ -137,8 +142,11 @@ class GPT2Block(nn.Module):
             raise ValueError(f"Unknown model_type: {model_type}")
 
     def attention(self, x: torch.Tensor) -> torch.Tensor:
-        b, t, d = x.shape
-        qkv = F.linear(self.ln1(x), self.attn.in_proj_weight, self.attn.in_proj_bias)
+        return self._attend(self.ln1(x))
+
+    def _attend(self, normed: torch.Tensor) -> torch.Tensor:
+        b, t, d = normed.shape
+        qkv = F.linear(normed, self.attn.in_proj_weight, self.attn.in_proj_bias)
         q, k, v = (h.transpose(1, 2) for h in qkv.view(b, t, 3, self.num_heads, self.head_dim).unbind(2))
         p = float(self.attn.dropout) if self.training else 0.0
         y = F.scaled_dot_product_attention(q, k, v, dropout_p=p, is_causal=True)
@@ -153,6 +161,27 @@ class GPT2Block(nn.Module):
         return out
 
 
+    def forward_fused(self, x: torch.Tensor, delta: Optional[torch.Tensor]):
+        """The block on ``x + delta`` (delta: the FFN output of the block before),
+        with both residual sums inside the norms that follow them.  Returns the
+        stream before this block's own FFN output, and that output."""
+        digital = _projection_dtype(x)  # what a norm that feeds a projection hands out
+        if delta is None:
+            normed = self.ln1(x, digital)
+        else:
+            normed, x = self.ln1.add(x, delta, digital)
+        normed, x = self.ln2.add(x, self._attend(normed), digital if self.digital_ffn else None)
+        return x, self.ffn(normed)
+
+
+def _projection_dtype(x: torch.Tensor) -> Optional[torch.dtype]:
+    """The autocast type, where one is on and the stream can hand it out."""
+    if not torch.is_autocast_enabled("cuda"):
+        return None
+    dtype = torch.get_autocast_dtype("cuda")
+    return dtype if x.dtype in (torch.float32, dtype) else None
+
+
 class GPT2Model(nn.Module):
     """GPT-2 with the FFN variant of ``cfg.model_type`` in every block."""
 
@@ -164,9 +193,9 @@ class GPT2Model(nn.Module):
         self.drop = nn.Dropout(cfg.dropout)
         self.blocks = nn.ModuleList(
             GPT2Block(cfg.embed_dim, cfg.ffn_dim, cfg.num_heads, cfg.model_type, cfg.voltage_max, cfg.dropout,
-                      physical_config)
+                      physical_config, cfg.fused_norm)
             for _ in range(cfg.depth))
-        self.ln_f = nn.LayerNorm(cfg.embed_dim)
+        self.ln_f = (LayerNorm if cfg.fused_norm else nn.LayerNorm)(cfg.embed_dim)
         self.lm_head = nn.Linear(cfg.embed_dim, cfg.vocab_size, bias=False)
         self.lm_head.weight = self.token_embedding.weight
         self.register_buffer("pos_ids", torch.arange(cfg.max_seq_len).unsqueeze(0), persistent=False)
@@ -174,6 +203,13 @@ class GPT2Model(nn.Module):
     def forward(self, input_ids: torch.Tensor, need_intermediate: bool = False):
         b, t = input_ids.shape
         x = self.drop(self.token_embedding(input_ids) + self.pos_embedding(self.pos_ids[:, :t].expand(b, -1)))
+        if self.cfg.fused_norm and not need_intermediate:
+            delta = None
+            for blk in self.blocks:
+                x, delta = blk.forward_fused(x, delta)
+            dtype = _projection_dtype(x)
+            normed = self.ln_f(x, dtype) if delta is None else self.ln_f.add(x, delta, dtype)[0]
+            return self.lm_head(normed)
         inter: List[Dict[str, torch.Tensor]] = []
         for blk in self.blocks:
             if need_intermediate:
@@ -198,6 +234,26 @@ class GPT2Model(nn.Module):
             (no_decay if exempt or p.dim() < 2 else decay).append(p)
         return [{"params": decay, "weight_decay": weight_decay, "lr": lr},
                 {"params": no_decay, "weight_decay": 0.0, "lr": lr}]
+
+
+    def configure_muon_groups(self, weight_decay: float, lr: float, muon_weight_decay: float, muon_lr: float):
+        """(groups for ``isa_b200.optim.Muon``, AdamW groups for the rest).  Muon
+        takes the digital matrices of the blocks: attention projections, the fused
+        query / key / value one as three, and the linear layers of a standard or
+        hybrid FFN.  Threshold voltages are device parameters in a narrow window and
+        stay with AdamW, as do embeddings, norms, gains and biases."""
+        fused, single = [], []
+        for blk in self.blocks:
+            fused.append(blk.attn.in_proj_weight)
+            single.append(blk.attn.out_proj.weight)
+            single += [m.weight for m in blk.ffn.modules() if isinstance(m, nn.Linear)]
+        both = dict(weight_decay=muon_weight_decay, lr=muon_lr)
+        muon = [{"params": [p for p in ps if p.requires_grad], "matrices": k, **both} for ps, k in ((fused, 3), (single, 1))]
+        taken = {id(p) for g in muon for p in g["params"]}
+        rest = self.configure_optimizer_groups(weight_decay, lr)
+        for g in rest:
+            g["params"] = [p for p in g["params"] if id(p) not in taken]
+        return [g for g in muon if g["params"]], [g for g in rest if g["params"]]
 
 
 def create_model(cfg: ModelConfig, physical_config: Optional[Dict] = None) -> GPT2Model:

@@ -5,3 +5,4 @@ from isa_b200.operators.cim import (  # noqa: F401
     VoltageMapping,
     clamp_signed,
 )
+from isa_b200.operators.norm import LayerNorm  # noqa: F401
