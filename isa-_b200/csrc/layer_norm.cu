@@ -29,6 +29,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <cstdio>
 #include <initializer_list>
@@ -779,10 +780,18 @@ int layout_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* place
     return pick_shape(cols, 1);
 }
 
-int allow_smem(const void* kernel, size_t bytes) {
+// Lets kernel number `id` use as much shared memory as its layout may ask for, once
+// per device (the attribute stays).
+int allow_smem(const void* kernel, int id, size_t bytes) {
+    static std::atomic<uint64_t> done[4 * kNumShapes];
     if (bytes <= (48 << 10)) return CIMEKV_OK;
-    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
-    return e == cudaSuccess ? CIMEKV_OK : fail(CIMEKV_ECUDA, cudaGetErrorString(e));
+    int dev;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(CIMEKV_ECUDA, "no current device");
+    if (dev < 64 && (done[id].load(std::memory_order_acquire) >> dev & 1)) return CIMEKV_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 220 << 10);
+    if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
+    if (dev < 64) done[id].fetch_or(1ull << dev, std::memory_order_release);
+    return CIMEKV_OK;
 }
 
 int check_sizes(long long rows, int cols) {
@@ -847,7 +856,7 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
     p.stages = ring_stages(kShapes[i], row_bytes, true);
     const Kernel kernel = kernels(i).fwd[delta != nullptr];
     const size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
-    if ((rc = allow_smem((const void*)kernel, smem))) return rc;
+    if ((rc = allow_smem((const void*)kernel, 4 * i + (delta != nullptr), smem))) return rc;
     kernel<<<(unsigned)grid_size(rows, kShapes[i], sms, true), cta_threads(kShapes[i].w), smem, (cudaStream_t)stream>>>(p);
     return launched("norm_fwd_kernel");
 }
@@ -919,7 +928,7 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
         const Kernel kernel = kernels(i).bwd[dh != nullptr];
         size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
         if (cta_rows(kShapes[i].w) > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
-        if ((rc = cimekv_internal_no_pending_error()) || (rc = allow_smem((const void*)kernel, smem))) return rc;
+        if ((rc = cimekv_internal_no_pending_error()) || (rc = allow_smem((const void*)kernel, 4 * i + 2 + (dh != nullptr), smem))) return rc;
         kernel<<<(unsigned)grid, cta_threads(kShapes[i].w), smem, s>>>(p);
         if ((rc = launched("norm_bwd_kernel"))) return rc;
         nparts = (int)grid;

@@ -34,6 +34,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <cstdio>
@@ -85,15 +86,16 @@ struct Tile {
     static constexpr int kWarps = kSide == 64 ? 8 : 16;     // collecting warps
     static constexpr int kWarpCols = kSide / (kWarps / 4);  // result columns of a collecting warp
     static constexpr int kThreads = (kWarps + 2) * 32;      // and a copy warp, a product warp
-    static constexpr int kBufs = kPair ? 2 : 4;             // accumulators in tensor memory
-    static constexpr int kChunk = kPair ? 2 : 1;            // stages summed in one of them
-    static constexpr int kColumns = kBufs * kSide;          // tensor memory columns
+    static constexpr int kBufs = kPair ? 2 : kStages;       // accumulators in tensor memory
+    static constexpr int kChunk = kPair ? 2 : 1;            // stages summed in one of them; where it is one, stage and
+                                                            // accumulator s are filled and done together
+    static constexpr int kColumns = 512;                    // tensor memory columns taken: all
     static constexpr int kStaging = kWarpRows * 64;         // a collecting warp's row segments on their way out
     static constexpr int kSmem = kStages * kStageBytes + kWarps * kStaging + 1024;
 };
 
 constexpr int kMaxTable = CIMEKV_MUON_MAX_MATRICES;
-constexpr int kMaxParts = 256;              // partial norms per matrix, at most
+constexpr int kMaxParts = 512;              // partial norms per matrix, at most
 
 // ------------------------------------------------------------- PTX pieces --
 
@@ -349,24 +351,36 @@ __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ Pr
     if (blockIdx.x == 0 && threadIdx.x == 0) p.arrivals[b] = 0;
     double s = 0.0;
     if constexpr (kFlat) {
-        const long long total = (long long)p.rows * p.cols / 4;
-        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long long)p.parts * 256) {
-            float v[4];
-            load4(g, p.g.type, 4 * i, v);
-            if (mom) {
-                float4 m = *reinterpret_cast<const float4*>(mom + 4 * i);
-                m.x = new_momentum(p, v[0], m.x);
-                m.y = new_momentum(p, v[1], m.y);
-                m.z = new_momentum(p, v[2], m.z);
-                m.w = new_momentum(p, v[3], m.w);
-                *reinterpret_cast<float4*>(mom + 4 * i) = m;
-                v[0] = update_of(p, v[0], m.x);
-                v[1] = update_of(p, v[1], m.y);
-                v[2] = update_of(p, v[2], m.z);
-                v[3] = update_of(p, v[3], m.w);
+        constexpr int kAhead = 4;
+        const long long total = (long long)p.rows * p.cols / 4, step = (long long)p.parts * 256;
+        for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < total; i += kAhead * step) {
+            // loads of several turns first: one after the other they are latency
+            float v[kAhead][4];
+            float4 m[kAhead];
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) {
+                if (i + u * step < total) {
+                    load4(g, p.g.type, 4 * (i + u * step), v[u]);
+                    if (mom) m[u] = *reinterpret_cast<const float4*>(mom + 4 * (i + u * step));
+                }
             }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) s += (double)v[k] * (double)v[k];
+            for (int u = 0; u < kAhead; ++u) {
+                if (i + u * step >= total) break;
+                if (mom) {
+                    m[u].x = new_momentum(p, v[u][0], m[u].x);
+                    m[u].y = new_momentum(p, v[u][1], m[u].y);
+                    m[u].z = new_momentum(p, v[u][2], m[u].z);
+                    m[u].w = new_momentum(p, v[u][3], m[u].w);
+                    *reinterpret_cast<float4*>(mom + 4 * (i + u * step)) = m[u];
+                    v[u][0] = update_of(p, v[u][0], m[u].x);
+                    v[u][1] = update_of(p, v[u][1], m[u].y);
+                    v[u][2] = update_of(p, v[u][2], m[u].z);
+                    v[u][3] = update_of(p, v[u][3], m[u].w);
+                }
+#pragma unroll
+                for (int k = 0; k < 4; ++k) s += (double)v[u][k] * (double)v[u][k];
+            }
         }
     } else {
         for (int r = blockIdx.x; r < p.rows; r += p.parts)
@@ -431,9 +445,10 @@ template <bool kVec>
 __global__ void __launch_bounds__(256) ns_prepare_kernel(const __grid_constant__ PrepParams p) {
     __shared__ float shared;
     chain();
-    const int b = blockIdx.z;
+    // from the end: what ns_norm_kernel touched last is still in L2
+    const int b = gridDim.z - 1 - blockIdx.z;
     const float factor = plane_factor(p, b, &shared);
-    const int r = blockIdx.y * 8 + (threadIdx.x >> 5), c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
+    const int r = (gridDim.y - 1 - blockIdx.y) * 8 + (threadIdx.x >> 5), c = blockIdx.x * 256 + (threadIdx.x & 31) * 8;
     if (r >= p.rows || c >= p.cols) return;
     const void* g = p.g.at(b);
     const float* mom = p.mom.tabled ? static_cast<const float*>(p.mom.table[b]) + (long long)r * p.cols : nullptr;
@@ -478,11 +493,11 @@ __global__ void __launch_bounds__(256) ns_prepare_tall_kernel(const __grid_const
     __shared__ float tile[64][65];
     __shared__ float shared;
     chain();
-    const int b = blockIdx.z;
+    const int b = gridDim.z - 1 - blockIdx.z;
     const float factor = plane_factor(p, b, &shared);
     const void* g = p.g.at(b);
     const float* mom = p.mom.tabled ? static_cast<const float*>(p.mom.table[b]) : nullptr;
-    const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64;
+    const int r0 = (gridDim.y - 1 - blockIdx.y) * 64, c0 = blockIdx.x * 64;
     const int tx = threadIdx.x & 63, ty = threadIdx.x >> 6;
 #pragma unroll 4
     for (int k = ty; k < 64; k += 4) {
@@ -750,7 +765,8 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             col0 += (int)q.rank * kRows;
             for (int k = 0; k < ksteps; ++k, ++q.fill) {
                 const int s = q.fill % kStages;
-                if (q.fill >= kStages && !(q.ok = mbar_wait(q.empty + 8 * s, (q.fill / kStages - 1) & 1))) break;
+                const uint32_t taken = kChunk == 1 ? q.acc_full : q.empty;
+                if (q.fill >= kStages && !(q.ok = mbar_wait(taken + 8 * s, (q.fill / kStages - 1) & 1))) break;
                 const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
                 if (elect_one()) {
                     if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
@@ -803,7 +819,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                             }
 #pragma unroll
                             for (uint64_t i = 0; i < kK / 16; ++i) mma_f16<kPair>(d, l0 + i * kL, r0 + i * kR, idesc, 1);
-                            mma_commit<kPair>(q.empty + 8 * s);
+                            if (kChunk > 1) mma_commit<kPair>(q.empty + 8 * s);
                             if (k + 1 == end) mma_commit<kPair>(q.acc_full + 8 * buf);
                         }
                         __syncwarp();
@@ -878,7 +894,7 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
     q.full = smem_addr(bars);
     q.empty = q.full + 8 * kStages;
     q.acc_full = q.full + 16 * kStages;
-    q.acc_empty = q.acc_full + 32;
+    q.acc_empty = q.acc_full + 8 * kMaxStages;
     q.rank = kPair ? cluster_rank() : 0;
     q.fill = q.chunk = 0;
     q.ok = true;
@@ -891,7 +907,7 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
             mbar_init(q.acc_full + 8 * s, 1);
             mbar_init(q.acc_empty + 8 * s, Tile<kSide>::kWarps * Tile<kSide>::kRanks);
         }
-        mbar_init(q.acc_full + 64, 1);
+        mbar_init(q.acc_empty + 8 * kMaxStages, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
     if ((threadIdx.x >> 5) == Tile<kSide>::kWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), Tile<kSide>::kColumns);
@@ -915,9 +931,9 @@ __device__ __forceinline__ void pipe_close(Pipe& q) {
             if (fills > 0) mbar_wait(q.full + 8 * s, (fills - 1) & 1);
         }
     } else if (warp == kWarps + 1 && q.rank == 0) {
-        if (elect_one()) mma_commit<kPair>(q.acc_full + 64);
+        if (elect_one()) mma_commit<kPair>(q.acc_empty + 8 * kMaxStages);
         __syncwarp();
-        mbar_wait(q.acc_full + 64, 0);
+        mbar_wait(q.acc_empty + 8 * kMaxStages, 0);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -938,7 +954,7 @@ __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const
                                                                            const __grid_constant__ Result result, int batch,
                                                                            int tiles) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 9];
+    __shared__ __align__(8) uint64_t bars[4 * kMaxStages + 1];
     __shared__ uint32_t tmem_slot;
     Pipe q;
     pipe_open<kSide>(q, bars, &tmem_slot, smem_raw);
@@ -992,7 +1008,7 @@ __global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const _
                                                                          const __grid_constant__ Steps st,
                                                                          const __grid_constant__ Result result, int batch) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 9];
+    __shared__ __align__(8) uint64_t bars[4 * kMaxStages + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int lost;
     if (threadIdx.x == 0) lost = 0;
@@ -1133,6 +1149,18 @@ int sm_count(int* sms) {
     return CIMEKV_OK;
 }
 
+// Lets `kernel` use its shared memory, once per device (the attribute stays).
+template <typename Kernel>
+int allow_smem(Kernel kernel, size_t bytes, std::atomic<uint64_t>& done) {
+    int dev;
+    if (cudaGetDevice(&dev) != cudaSuccess) return fail(CIMEKV_ECUDA, "no current device");
+    if (dev < 64 && (done.load(std::memory_order_acquire) >> dev & 1)) return CIMEKV_OK;
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
+    if (dev < 64) done.fetch_or(1ull << dev, std::memory_order_release);
+    return CIMEKV_OK;
+}
+
 long long tile_count(int mode, int side, int rows, int cols) {
     const long long ni = (rows + side - 1) / side, nj = (cols + side - 1) / side;
     return mode == kSymmetric ? ni * (ni + 1) / 2 : ni * nj;
@@ -1166,9 +1194,8 @@ int launch_chained(const char* what, void (*kernel)(Args...), dim3 grid, int thr
 template <int M, int kSide>
 int launch_as(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result, int batch, int sms,
               cudaStream_t s) {
-    const cudaError_t e =
-        cudaFuncSetAttribute(ns_gemm_kernel<M, kSide>, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<kSide>::kSmem);
-    if (e != cudaSuccess) return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
+    static std::atomic<uint64_t> allowed{0};
+    if (int rc = allow_smem(ns_gemm_kernel<M, kSide>, Tile<kSide>::kSmem, allowed)) return rc;
     constexpr int ranks = Tile<kSide>::kRanks;
     const long long tiles = tile_count(M, kSide, p.rows, p.cols) * batch, most = sms / ranks;
     return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kSide>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
@@ -1183,7 +1210,7 @@ struct Cost {
     double start, stage, tile;
     double of(long long rounds, int depth) const { return start + rounds * (stage * ((depth + 63) / 64) + tile); }
 };
-constexpr Cost kCost64 = {6000, 900, 300}, kCost128 = {9200, 1420, 500}, kCost256 = {9200, 1600, 3000};
+constexpr Cost kCost64 = {6000, 900, 300}, kCost128 = {10000, 1420, 500}, kCost256 = {10000, 1600, 3000};
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -1302,8 +1329,8 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
         if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, 64))) return rc;
         if ((rc = plane_map(encode, &maps.b_out, am, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
         if ((rc = plane_map(encode, &maps.p_out, pm, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
-        cudaError_t e =
-            cudaFuncSetAttribute(ns_steps_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Tile<64>::kSmem);
+        static std::atomic<uint64_t> allowed{0};
+        if ((rc = allow_smem(ns_steps_kernel, Tile<64>::kSmem, allowed))) return rc;
         st.arrivals = prep.arrivals;
         st.group = group;
         const int most = sms / group;
@@ -1317,7 +1344,7 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
         attr[0].val.cooperative = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        if (e == cudaSuccess) e = cudaLaunchKernelEx(&cfg, ns_steps_kernel, maps, st, result, batch);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_steps_kernel, maps, st, result, batch);
         if (e == cudaSuccess) return CIMEKV_OK;
         (void)cudaGetLastError();
         return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
