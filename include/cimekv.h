@@ -253,7 +253,8 @@ enum { CIMEKV_F32 = 0, CIMEKV_BF16 = 1, CIMEKV_F16 = 2 };
  * x and delta have rows of contiguous elements `*_stride` elements apart (0
  * repeats a row); h and y are contiguous.  weight and bias [cols] share w_type,
  * either may be NULL.  mean and rstd [rows] are kept for the backward (both may
- * be NULL).  Outputs must not overlap inputs.
+ * be NULL).  Outputs must not overlap inputs.  Rows are read in units of 16 bytes:
+ * what shares a unit with the first or last element of a row is read too.
  */
 int cimekv_layer_norm_forward(const void* x, int x_type, long long x_stride,
                               const void* delta, int delta_type, long long delta_stride,
@@ -309,7 +310,8 @@ int cimekv_orthogonalize(const void* g, int type, long long batch_stride, long l
  *   u  = nesterov ? momentum m + (1 - momentum) g : m
  *   p <- p (1 - lr weight_decay) - lr scale NS(u)   (NS as cimekv_orthogonalize)
  * params, grads and momenta are HOST arrays of device pointers to contiguous
- * [rows][cols] matrices (all distinct); they are read before the call returns.
+ * [rows][cols] matrices; the arrays are read before the call returns.  Parameters and
+ * momenta must not overlap each other (refused) or a gradient.
  * lr_device, when not NULL, is a device scalar read instead of lr, so that a
  * captured graph follows a schedule.  workspace as for cimekv_orthogonalize
  * with batch = count.

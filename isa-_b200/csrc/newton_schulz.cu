@@ -1419,7 +1419,7 @@ extern "C" int cimekv_muon_step(int count, void* const* params, const void* cons
     if (!params || !grads || !momenta) return fail(CIMEKV_EINVAL_SHAPE, "null pointer");
     for (int i = 0; i < count; ++i)
         if (!params[i] || !grads[i] || !momenta[i]) return fail(CIMEKV_EINVAL_SHAPE, "null pointer");
-    // matrices written in one launch must not share memory
+    // matrices written in one launch must not share memory (a gradient may be shared, but not with them)
     std::pair<uintptr_t, uintptr_t> range[2 * kMaxTable];
     const uintptr_t elements = (uintptr_t)rows * (uintptr_t)cols;
     for (int i = 0; i < count; ++i) {

@@ -10,7 +10,9 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <algorithm>
 #include <array>
+#include <cmath>
 #include <map>
 #include <tuple>
 #include <vector>
@@ -298,6 +300,30 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
                         lr_tensor->device() == params[0].device(),
                     "lr must be a float or a one-element float32 tensor on the parameters' device");
     if (params.empty()) return;
+    // What is written must be memory of its own, checked before anything is: a
+    // refused call leaves every parameter as it was.
+    struct Range {
+        uintptr_t begin, end;
+        bool written;
+        bool operator<(const Range& o) const { return begin < o.begin; }
+    };
+    std::vector<Range> ranges;
+    const auto add = [&](const Tensor& t, bool written) {
+        if (t.numel() && (written || t.is_contiguous()))  // other gradients are copied first
+            ranges.push_back({(uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.numel() * t.element_size(), written});
+    };
+    for (size_t i = 0; i < params.size(); ++i) {
+        add(params[i], true);
+        add(momenta[i], true);
+        add(grads[i], false);
+    }
+    std::sort(ranges.begin(), ranges.end());
+    uintptr_t written_to = 0, read_to = 0;  // ends of what was seen so far
+    for (const Range& r : ranges) {
+        TORCH_CHECK(r.begin >= written_to && (!r.written || r.begin >= read_to),
+                    "parameters and momenta must not overlap each other or a gradient");
+        (r.written ? written_to : read_to) = std::max(r.written ? written_to : read_to, r.end);
+    }
     const c10::cuda::CUDAGuard guard(params[0].device());
     for (size_t i = 0; i < params.size(); ++i) {
         const Tensor &p = params[i], &m = momenta[i];

@@ -78,6 +78,8 @@ def _ops():
 # ------------------------------------------------------------- CPU: refusals --
 
 def test_refuses_cpu_tensors():
+    from isa_b200 import build
+    build.build_library()
     layer_norm, add_layer_norm = _ops()
     x = torch.zeros(2, 8)
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -366,6 +368,52 @@ def test_other_stream_and_graph(dev):
             t.fill_(float("nan"))
         g.replay()
         assert all(torch.equal(p, q) for p, q in zip(want, out))
+
+
+@gpu
+def test_offsets_beyond_32_bits(dev):
+    """2.3e9 elements: rows do not depend on one another, so the last ones equal a small call's."""
+    layer_norm, add_layer_norm = _ops()
+    x = torch.empty(140000, 16384, device=dev, dtype=BF16).normal_()
+    w = torch.rand(16384, device=dev, dtype=BF16).requires_grad_(True)
+    leaf = x.requires_grad_(True)
+    y = layer_norm(leaf, w)
+    tail = x.detach()[-5:].clone().requires_grad_(True)
+    small = layer_norm(tail, w)
+    assert torch.equal(y[-5:], small) and torch.equal(y[:5], layer_norm(x.detach()[:5].clone(), w))
+    dy = torch.zeros((), device=dev, dtype=BF16).expand_as(x).clone()
+    dy[-5:] = 1.0
+    gx, gw = torch.autograd.grad(y, (leaf, w), dy)
+    sx, sw = torch.autograd.grad(small, (tail, w), torch.ones_like(small))
+    assert torch.equal(gx[-5:], sx) and not gx[:-5].any()
+    _assert_near(gw, sw.double(), _eta(sw.double(), BF16) * 2, "dw")  # either sum rounded to bf16 once
+
+
+@gpu
+def test_no_memory_is_kept(dev):
+    """Outputs that are dropped without a backward free everything, a saved output among it."""
+    _, add_layer_norm = _ops()
+    x, d, w, b, dy, dh = _case(dev, 500, 256, F32, BF16, F32, F32, seed=7)
+    add_layer_norm(x, d, w, b)
+    before = torch.cuda.memory_allocated()
+    for _ in range(3):
+        add_layer_norm(x, d, w, b)
+        y, h = add_layer_norm(x, d, w, b)
+        torch.autograd.grad((y, h), (x, d), (dy, dh))
+    del y, h
+    assert torch.cuda.memory_allocated() == before
+
+
+@gpu
+def test_changes_behind_its_back_are_noticed(dev):
+    layer_norm, add_layer_norm = _ops()
+    x, w = torch.randn(4, 32, device=dev, requires_grad=True), torch.ones(32, device=dev, requires_grad=True)
+    for change in ("w", "h"):
+        y, h = add_layer_norm(x, x.detach(), w)
+        with torch.no_grad():
+            (w if change == "w" else h).mul_(2.0)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y.sum(), x)
 
 
 @gpu

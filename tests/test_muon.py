@@ -75,6 +75,8 @@ def _update(dev, *shape, seed=0, dtype=F32, scale=1e-3):
 # ------------------------------------------------------------- CPU: refusals --
 
 def test_refuses_cpu_tensors():
+    from isa_b200 import build
+    build.build_library()
     orthogonalize, muon_step = _ops()
     g = torch.ones(4, 4)
     with pytest.raises(RuntimeError, match="CUDA"):
@@ -303,6 +305,18 @@ def test_gpu_refusals(dev):
         muon_step([g, g], [g, g], [m, torch.zeros_like(m)], lr=0.1)
     with pytest.raises(RuntimeError, match="overlap"):
         muon_step([g], [m], [g], lr=0.1)
+    with pytest.raises(RuntimeError, match="overlap"):
+        muon_step([g], [m], [m], lr=0.1)  # a gradient that is its own momentum
+    with pytest.raises(RuntimeError, match="overlap"):
+        muon_step([torch.ones(4, 4, device=dev), g], [torch.ones(4, 4, device=dev), g], [torch.zeros(4, 4, device=dev), m], lr=0.1)
+    p = torch.ones(4, 4, device=dev)
+    with pytest.raises(RuntimeError, match="overlap"):  # nothing of a refused call is carried out
+        muon_step([p, g, g], [torch.ones_like(p), torch.ones_like(g), torch.ones_like(g)],
+                  [torch.zeros_like(p), m, torch.zeros_like(g)], lr=0.1)
+    assert (p == 1).all()
+    muon_step([p, g], [torch.ones(4, 4, device=dev).expand(4, 4)] + [torch.ones_like(g)], [torch.zeros_like(p), m], lr=0.1)
+    both = torch.ones(4, 4, device=dev)
+    muon_step([p, torch.ones_like(p)], [both, both], [torch.zeros_like(p), torch.zeros_like(p)], lr=0.1)  # one gradient twice
     with pytest.raises(RuntimeError, match="one-element"):
         muon_step([g], [m], [m], lr=torch.zeros(2, device=dev))
     with pytest.raises(RuntimeError, match="momentum must be"):
