@@ -7,7 +7,11 @@
 
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
+#include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -144,6 +148,7 @@ public:
     }
 
     static variable_list backward(AutogradContext* ctx, variable_list grads) {
+        check_capture();
         variable_list out(6);
         const Tensor dy = grads[0], dh = grads.size() > 1 ? grads[1] : Tensor();
         if (!dy.defined() && !dh.defined()) return out;
@@ -161,6 +166,27 @@ public:
     }
 
 private:
+    // A captured backward that reaches leaves whose accumulators an eager graph has
+    // made on the default stream would pull that stream into the capture, which
+    // spoils the capture or ends the process.  Refused here while it is still an error.
+    static void check_capture() {
+        if (c10::cuda::currentStreamCaptureStatusMayInitCtx() == c10::cuda::CaptureStatus::None) return;
+        const auto* only = torch::autograd::get_current_graph_task_exec_info();  // autograd.grad(): what it needs
+        const auto node = torch::autograd::get_current_node();
+        if (!node) return;
+        for (const auto& edge : node->next_edges()) {
+            if (!edge.function || !dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+            if (only && !only->empty()) {
+                const auto it = only->find(edge.function.get());
+                if (it == only->end() || !it->second.should_execute()) continue;
+            }
+            const auto made_on = edge.function->stream();
+            TORCH_CHECK(!made_on || *made_on != c10::cuda::getDefaultCUDAStream(made_on->device_index()).unwrap(),
+                        "this backward is being captured while an eager graph of the same parameters is alive (made on the "
+                        "default stream): drop its outputs before the capture, or make it on a side stream");
+        }
+    }
+
     static void run(AutogradContext* ctx, const Tensor& dy, const Tensor& dh, variable_list& out) {
         const auto saved = ctx->get_saved_variables();
         const Tensor &src = saved[0], &weight = saved[1], &stats = saved[2];

@@ -14,8 +14,8 @@ rows and a fixed-order reduction for the weight gradients, so it gives the same
 bits every time; it cannot be differentiated again.
 
 A backward captured into a CUDA graph follows torch's rule: no eager graph of the
-same leaf parameters may be alive during the capture (``del`` the warm-up's
-outputs and losses first).
+same leaf parameters, made on the default stream, may be alive during the capture
+(``del`` the warm-up's outputs and losses first).  Such a capture raises.
 """
 
 from __future__ import annotations

@@ -405,6 +405,48 @@ def test_no_memory_is_kept(dev):
 
 
 @gpu
+@pytest.mark.parametrize("how", ["backward", "grad", "other", "released"])
+def test_capture_while_an_eager_graph_lives(dev, how):
+    """In a process of its own: a capture that would reach the default stream raises, and the process goes on."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"""
+import sys
+sys.path.insert(0, {str(Path(__file__).resolve().parent.parent / 'isa-_b200')!r})
+import torch
+from isa_b200.kernels.transformer_norm import cuda_layer_norm
+how = {how!r}
+x, w = torch.randn(64, 128, device="cuda"), torch.ones(128, device="cuda", requires_grad=True)
+v = torch.ones(128, device="cuda", requires_grad=True)
+eager = cuda_layer_norm(x, w)
+if how == "released":
+    eager.sum().backward()
+    del eager
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+try:
+    with torch.cuda.graph(graph):
+        y = cuda_layer_norm(x, w, v)
+        if how == "grad":
+            torch.autograd.grad(y.sum(), w)
+        elif how == "other":  # only a leaf that no eager graph holds
+            out, = torch.autograd.grad(y.sum(), v)
+        else:
+            y.sum().backward()
+    graph.replay()
+    print("captured")
+except RuntimeError as e:
+    print("refused" if "eager graph" in str(e) else e)
+torch.cuda.synchronize()
+print("alive", float((x * 0 + 1).sum()))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    want = "captured" if how in ("other", "released") else "refused"
+    assert r.returncode == 0 and r.stdout.split() == [want, "alive", "8192.0"], (r.stdout, r.stderr[-2000:])
+
+
+@gpu
 def test_changes_behind_its_back_are_noticed(dev):
     layer_norm, add_layer_norm = _ops()
     x, w = torch.randn(4, 32, device=dev, requires_grad=True), torch.ones(32, device=dev, requires_grad=True)
