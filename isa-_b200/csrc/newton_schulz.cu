@@ -527,8 +527,8 @@ __global__ void __launch_bounds__(256) ns_prepare_tall_kernel(const __grid_const
 
 // kSymmetric: alpha L L^T + beta I, one triangle and its mirror image; kFull: the same, all
 // tiles; kApply: L R; kResult: L R to the caller's matrices.
-enum Mode { kSymmetric = 0, kFull = 1, kApply = 2, kResult = 3 };
-__host__ __device__ constexpr bool is_square(int mode) { return mode <= kFull; }
+// kAny: one of the others, told at run time (all but kSymmetric).
+enum Mode { kSymmetric = 0, kFull = 1, kApply = 2, kResult = 3, kAny = 4 };
 
 // One product of a batch.
 struct Product {
@@ -648,12 +648,12 @@ __device__ __forceinline__ void finish_result(const Result& p, int rows, int col
 }
 
 // 32 columns from cb of the warp's kRows rows from row0 of a product that stays in
-// planes (kDiagonal: plus beta on the diagonal; kMirror: and their mirror image off
-// it).  Rows of 64 bytes are staged in the 64-byte swizzle of `out` and leave by a
+// planes (`diagonal`: a tile on the diagonal, which gets beta there; kMirror: off it,
+// their mirror image too).  Rows of 64 bytes are staged in the 64-byte swizzle of `out` and leave by a
 // bulk copy, which clips them to the matrix and lets the warp go on: ordinary stores of
 // a 256 x 256 tile took 8,000 cycles, in which the products ran out of accumulators.
 // Called by whole warps.
-template <bool kDiagonal, bool kMirror, int kRows>
+template <bool kMirror, int kRows>
 __device__ __forceinline__ void finish_planes(const Product& p, const CUtensorMap* out, const float (&v0)[16],
                                               const float (&v1)[16], int batch, int b, int row0, int cb, bool diagonal,
                                               uint32_t staging) {
@@ -665,7 +665,7 @@ __device__ __forceinline__ void finish_planes(const Product& p, const CUtensorMa
 #pragma unroll
         for (int k = 0; k < 2; ++k) {
             o[k] = (i < 8 ? v0[(2 * i + k) & 15] : v1[(2 * i + k) & 15]) * p.alpha;
-            if (kDiagonal && diagonal && r == cb + 2 * i + k) o[k] += p.beta;
+            if (diagonal && r == cb + 2 * i + k) o[k] += p.beta;
         }
         split2(o[0], o[1], words[0][i], words[1][i]);
     }
@@ -705,16 +705,31 @@ __device__ __forceinline__ void finish_planes(const Product& p, const CUtensorMa
     }
 }
 
+// Place in a ring of barriers and the parity of the phase to wait for there.  (Kept
+// step by step: the divisions of a running number were 250 cycles a stage in the one
+// thread that issues.)
+struct Turn {
+    int at;
+    uint32_t parity;
+    __device__ __forceinline__ void next(int places) {
+        if (++at == places) {
+            at = 0;
+            parity ^= 1;
+        }
+    }
+};
+
 // Shared-memory addresses of a CTA's pipeline, and where each role stands in it.
 struct Pipe {
     uint32_t stages, full, empty, acc_full, acc_empty, tmem;
     uint32_t rank;          // in the pair
-    int fill;               // copy and product warps: stages so far
-    int chunk;              // product and collecting warps: accumulators so far
+    Turn fill;              // copy and product warps: the stage
+    Turn chunk;             // product and collecting warps: the accumulator
     bool ok;                // no wait has run out
 };
 
-// The tiles first, first + step, ... of one product.  Tiles are 128 x 128 by one CTA,
+// The tiles first, first + step, ... of one product: of matrix `matrix`, or (-1) of all
+// matrices in turn.  Tiles are 128 x 128 by one CTA,
 // 256 x 256 by a pair of CTAs whose tensor cores work as one (each stages 128
 // rows of either operand, holds its 128 rows of the result, and the first CTA
 // issues), or 64 x 64 by one CTA.  One warp copies stages ahead, one
@@ -731,7 +746,8 @@ struct Pipe {
 // accumulators let the next tile start while the last one is stored.
 template <int M, int kSide>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
-                                        const CUtensorMap* out, const Product& p, const Result* result, int batch, int first, int step, int tiles) {
+                                        const CUtensorMap* out, const Product& p, const Result& result, int batch, int first, int step, int tiles,
+                                        int mode = M, int matrix = -1) {
     using T = Tile<kSide>;
     constexpr bool kPair = T::kPair;
     constexpr int kRanks = T::kRanks, kRows = T::kRows, kOperand = T::kOperand, kStageBytes = T::kStageBytes;
@@ -741,15 +757,24 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
     const int ni = (p.rows + kSide - 1) / kSide, nj = (p.cols + kSide - 1) / kSide;
     const int per_matrix = M == kSymmetric ? ni * (ni + 1) / 2 : ni * nj;
     const int ksteps = (p.depth + kK - 1) / kK;
+    const bool square = mode <= kFull;  // L L^T: both operands' rows run along K
+    const float per_row = 1.0f / (float)nj;
     const auto place = [&](int t, int& b, int& row0, int& col0) {
-        b = t / per_matrix;
-        const int at = t - b * per_matrix;
+        b = matrix >= 0 ? matrix : t / per_matrix;
+        const int at = matrix >= 0 ? t : t - b * per_matrix;
         int i, j;
         if (M == kSymmetric) {
             triangle(at, i, j);
         } else {
-            i = at / nj;
+            i = (int)((float)at * per_row);  // off by one at most (at < 2^24), mended below
             j = at - i * nj;
+            if (j < 0) {
+                --i;
+                j += nj;
+            } else if (j >= nj) {
+                ++i;
+                j -= nj;
+            }
         }
         row0 = i * kSide;
         col0 = j * kSide;
@@ -760,13 +785,13 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
         for (int t = first; t < tiles && q.ok; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
-            const bool same = is_square(M) && row0 == col0;  // both operands are the same rows
+            const bool same = square && row0 == col0;  // both operands are the same rows
             row0 += (int)q.rank * kRows;
             col0 += (int)q.rank * kRows;
-            for (int k = 0; k < ksteps; ++k, ++q.fill) {
-                const int s = q.fill % kStages;
-                const uint32_t taken = kChunk == 1 ? q.acc_full : q.empty;
-                if (q.fill >= kStages && !(q.ok = mbar_wait(taken + 8 * s, (q.fill / kStages - 1) & 1))) break;
+            for (int k = 0; k < ksteps; ++k, q.fill.next(kStages)) {
+                const int s = q.fill.at;
+                // (the phase before a barrier's first has ended by definition)
+                if (!(q.ok = mbar_wait((kChunk == 1 ? q.acc_full : q.empty) + 8 * s, q.fill.parity ^ 1))) break;
                 const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
                 if (elect_one()) {
                     if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
@@ -776,7 +801,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                         const uint32_t l = base + plane * kOperand, r = base + (2 + plane) * kOperand;
                         tma_box<kPair>(l, left, k * kK, row0, z, bar);
                         if (same) continue;
-                        if (is_square(M)) {
+                        if (square) {
                             tma_box<kPair>(r, right, k * kK, col0, z, bar);
                         } else {
                             tma_box<kPair>(r, right, col0, k * kK, z, bar);
@@ -790,27 +815,27 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
     } else if (warp == kWarps + 1) {
         if (q.rank == 0) {
             // D fp32, A and B fp16; right operand along K (0) or along its own axis (1)
-            const uint32_t idesc = 1u << 4 | (is_square(M) ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
+            const uint32_t idesc = 1u << 4 | (square ? 0u : 1u << 16) | (uint32_t)(kSide / 8) << 17 |
                                    (uint32_t)(kSide / 16) << 24;
             for (int t = first; t < tiles && q.ok; t += step) {
                 int b, row0, col0;
                 place(t, b, row0, col0);
-                const int r_at = is_square(M) && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
-                for (int k = 0; k < ksteps && q.ok; ++q.chunk) {
-                    const int buf = q.chunk % kBufs;
-                    if (q.chunk >= kBufs && !(q.ok = mbar_wait(q.acc_empty + 8 * buf, (q.chunk / kBufs - 1) & 1))) break;
+                const int r_at = square && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
+                for (int k = 0; k < ksteps && q.ok; q.chunk.next(kBufs)) {
+                    const int buf = q.chunk.at;
+                    if (!(q.ok = mbar_wait(q.acc_empty + 8 * buf, q.chunk.parity ^ 1))) break;
                     const uint32_t d = q.tmem + buf * kSide;
                     const int end = min(k + kChunk, ksteps);
-                    for (uint32_t more = 0; k < end; ++k, ++q.fill, more = 1) {
-                        const int s = q.fill % kStages;
-                        if (!(q.ok = mbar_wait(q.full + 8 * s, (q.fill / kStages) & 1))) break;
+                    for (uint32_t more = 0; k < end; ++k, q.fill.next(kStages), more = 1) {
+                        const int s = q.fill.at;
+                        if (!(q.ok = mbar_wait(q.full + 8 * s, q.fill.parity))) break;
                         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                         const uint32_t base = q.stages + s * kStageBytes;
                         // both planes of either operand; a step of 16 along K moves the address alone
                         const uint64_t l0 = operand_desc(base, 16, 1024), l1 = operand_desc(base + kOperand, 16, 1024);
-                        const uint64_t r0 = operand_desc(base + r_at, is_square(M) ? 16 : 8192, 1024);
-                        const uint64_t r1 = operand_desc(base + r_at + kOperand, is_square(M) ? 16 : 8192, 1024);
-                        constexpr uint64_t kL = 32 >> 4, kR = (is_square(M) ? 32 : 2048) >> 4;
+                        const uint64_t r0 = operand_desc(base + r_at, square ? 16 : 8192, 1024);
+                        const uint64_t r1 = operand_desc(base + r_at + kOperand, square ? 16 : 8192, 1024);
+                        const uint64_t kL = 32 >> 4, kR = (square ? 32 : 2048) >> 4;
                         if (elect_one()) {
 #pragma unroll
                             for (uint64_t i = 0; i < kK / 16; ++i) {
@@ -832,23 +857,21 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
         const uint32_t staging = q.stages + kStages * kStageBytes + warp * T::kStaging;
         const uint32_t empty_at = kPair ? cluster_addr(q.acc_empty, 0) : q.acc_empty;
         float lr = 0.0f;
-        if constexpr (M == kResult) {
-            if (result->update) lr = result->lr_dev ? *result->lr_dev : result->lr;
-        }
+        if (mode == kResult && result.update) lr = result.lr_dev ? *result.lr_dev : result.lr;
         for (int t = first; t < tiles; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
             const int r0 = row0 + (int)q.rank * kRows + quarter * T::kWarpRows;
-            const bool diagonal = row0 == col0;
+            const bool diagonal = square && row0 == col0;
             col0 += group * kWarpCols;
             float acc[kWarpCols / 16][16];
 #pragma unroll
             for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
-            for (int k = 0; k < ksteps; k += kChunk, ++q.chunk) {
-                const int buf = q.chunk % kBufs;
-                q.ok = q.ok && mbar_wait(q.acc_full + 8 * buf, (q.chunk / kBufs) & 1);
+            for (int k = 0; k < ksteps; k += kChunk, q.chunk.next(kBufs)) {
+                const int buf = q.chunk.at;
+                q.ok = q.ok && mbar_wait(q.acc_full + 8 * buf, q.chunk.parity);
                 q.ok = __all_sync(0xffffffffu, q.ok);
                 if (!q.ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -873,14 +896,14 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
 #pragma unroll
             for (int g = 0; g < kWarpCols / 16; ++g) {
                 if (col0 + g * 16 >= p.cols) break;
-                if constexpr (M == kResult)
-                    finish_result<T::kWarpRows>(*result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
+                if (mode == kResult)
+                    finish_result<T::kWarpRows>(result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
                 else if (g % 2 == 0)
-                    finish_planes<is_square(M), M == kSymmetric, T::kWarpRows>(p, out, acc[g], acc[g + 1], batch, b, r0, col0 + g * 16, diagonal, staging);
+                    finish_planes<M == kSymmetric, T::kWarpRows>(p, out, acc[g], acc[g + 1], batch, b, r0, col0 + g * 16, diagonal, staging);
             }
             __syncwarp();
         }
-        if (M != kResult && lane == 0) tma_store_wait<true>();
+        if (mode != kResult && lane == 0) tma_store_wait<true>();
         __syncwarp();
     }
 }
@@ -896,7 +919,7 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
     q.acc_full = q.full + 16 * kStages;
     q.acc_empty = q.acc_full + 8 * kMaxStages;
     q.rank = kPair ? cluster_rank() : 0;
-    q.fill = q.chunk = 0;
+    q.fill = q.chunk = {0, 0};
     q.ok = true;
     if (threadIdx.x == 0) {
         for (int s = 0; s < kStages; ++s) {
@@ -926,10 +949,8 @@ __device__ __forceinline__ void pipe_close(Pipe& q) {
     constexpr int kWarps = Tile<kSide>::kWarps, kStages = Tile<kSide>::kStages;
     const int warp = threadIdx.x >> 5;
     if (warp == kWarps && q.rank == 0) {
-        for (int s = 0; s < kStages; ++s) {
-            const int fills = (q.fill - s + kStages - 1) / kStages;
-            if (fills > 0) mbar_wait(q.full + 8 * s, (fills - 1) & 1);
-        }
+        // a stage before the turn was last filled in this phase, the others in the one before
+        for (int s = 0; s < kStages; ++s) mbar_wait(q.full + 8 * s, s < q.fill.at ? q.fill.parity : q.fill.parity ^ 1);
     } else if (warp == kWarps + 1 && q.rank == 0) {
         if (elect_one()) mma_commit<kPair>(q.acc_empty + 8 * kMaxStages);
         __syncwarp();
@@ -960,7 +981,7 @@ __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const
     pipe_open<kSide>(q, bars, &tmem_slot, smem_raw);
     chain();
     constexpr int kRanks = Tile<kSide>::kRanks;
-    product<M, kSide>(q, &left, &right, &out, p, &result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
+    product<M, kSide>(q, &left, &right, &out, p, result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
     pipe_close<kSide>(q);
 }
 
@@ -969,7 +990,8 @@ __global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const
 // a matrix with 64 x 64 tiles and meet between its products.  A cooperative
 // launch, so that all of them are resident while they wait for one another.
 struct Steps {
-    Product gram, square, apply;    // square.rows = 0: c = 0, no square
+    Product product[3];             // X X^T, its square, P X
+    int squared;                    // 0: c = 0, no square
     unsigned* arrivals;             // per matrix, zeroed by ns_norm_kernel
     int steps, group;
 };
@@ -984,8 +1006,7 @@ __device__ __forceinline__ void group_meet(unsigned* arrivals, unsigned target, 
     asm volatile("fence.proxy.async.global;" ::: "memory");
     __syncthreads();
     if (group > 1 && threadIdx.x == 0) {
-        __threadfence();
-        atomicAdd(arrivals, 1u);
+        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrivals) : "memory");
         unsigned long long began = 0;
         for (;;) {
             unsigned seen;
@@ -1014,27 +1035,21 @@ __global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const _
     if (threadIdx.x == 0) lost = 0;
     Pipe q;
     pipe_open<64>(q, bars, &tmem_slot, smem_raw);
-    const int ni = (st.gram.rows + 63) / 64, nj = (st.apply.cols + 63) / 64;
-    const int square = ni * ni, all = ni * nj, rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
+    const int ni = (st.product[0].rows + 63) / 64, nj = (st.product[2].cols + 63) / 64;
+    const int rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
     for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
         unsigned target = 0;
-        const auto meet = [&]() { group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost); };
-        const int square0 = matrix * square + rank, square1 = (matrix + 1) * square;
-        const int all0 = matrix * all + rank, all1 = (matrix + 1) * all;
         for (int k = 0; k < st.steps; ++k) {
-            // all tiles: storing mirror images takes a CTA longer than a tile that another one has time for
-            product<kFull, 64>(q, &maps.x[k & 1], &maps.x[k & 1], st.square.rows ? &maps.b_out : &maps.p_out,
-                                 st.gram, nullptr, batch, square0, st.group, square1);
-            meet();
-            if (st.square.rows) {
-                product<kFull, 64>(q, &maps.b, &maps.b, &maps.p_out, st.square, nullptr, batch, square0, st.group, square1);
-                meet();
-            }
-            if (k + 1 < st.steps) {
-                product<kApply, 64>(q, &maps.p, &maps.x[k & 1], &maps.x_out[(k + 1) & 1], st.apply, nullptr, batch, all0, st.group, all1);
-                meet();
-            } else {
-                product<kResult, 64>(q, &maps.p, &maps.x[k & 1], nullptr, st.apply, &result, batch, all0, st.group, all1);
+            // All tiles of the square products: storing mirror images takes a CTA longer than a tile that
+            // another one has time for.
+            for (int i = 0; i < 3; i += st.squared ? 1 : 2) {
+                const int mode = i < 2 ? kFull : k + 1 < st.steps ? kApply : kResult;
+                const int tiles = ni * (i < 2 ? ni : nj);
+                const CUtensorMap* const x = &maps.x[k & 1];
+                product<kAny, 64>(q, i == 0 ? x : i == 1 ? &maps.b : &maps.p, i == 1 ? &maps.b : x,
+                                  i == 0 && st.squared ? &maps.b_out : i < 2 ? &maps.p_out : &maps.x_out[(k + 1) & 1],
+                                  st.product[i], result, batch, rank, st.group, tiles, mode, matrix);
+                if (mode != kResult) group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost);
             }
         }
     }
@@ -1210,7 +1225,7 @@ struct Cost {
     double start, stage, tile;
     double of(long long rounds, int depth) const { return start + rounds * (stage * ((depth + 63) / 64) + tile); }
 };
-constexpr Cost kCost64 = {6000, 900, 300}, kCost128 = {10000, 1420, 500}, kCost256 = {10000, 1600, 3000};
+constexpr Cost kCost64 = {5000, 900, 300}, kCost128 = {9000, 1425, 500}, kCost256 = {9500, 1600, 3000};
 
 long long ceil_div(long long a, long long b) { return (a + b - 1) / b; }
 
@@ -1227,9 +1242,9 @@ int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& o
 }
 
 // CTAs per matrix when all steps run in one kernel, 0 where a kernel for each
-// product costs less.  Measured, one kernel against fifteen: 73 against 114 us for
-// one 192 x 192 matrix, 146 against 214 for 768 x 768, 83 against 95 for 200 of
-// 64 x 64; 283 against 258 for 1024 x 1024, 196 against 161 for 12 of 384 x 384.
+// product costs less.  Measured a call, one kernel against fifteen: 73 against 112 us
+// for one 192 x 192 matrix, 131 against 202 for 768 x 768, 120 against 135 for 40 of
+// 192 x 192; 252 against 239 for 1024 x 1024, 176 against 159 for 12 of 384 x 384.
 int steps_group(int batch, int m, int n, bool squared, int sms) {
     const long long tiles = tile_count(kApply, 64, m, n), most = std::max(1LL, std::min<long long>(tiles, sms / batch));
     const long long group = ceil_div(tiles, ceil_div(tiles, most));  // no more than the rounds need
@@ -1301,20 +1316,21 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     // sums of products of two planes are 2^24 times the value, planes 2^12 times
     const bool squared = c != 0.0f;
     Steps st = {};
+    Product &gram = st.product[0], &square = st.product[1], &apply = st.product[2];
     st.steps = steps;
-    st.gram.rows = st.gram.cols = lay.m;
-    st.gram.depth = lay.n;
-    st.gram.alpha = (squared ? 1.0f : b) / kScale;
-    st.gram.beta = (squared ? (float)(0.5 * b / c) : a) * kScale;
+    st.squared = squared;
+    gram.rows = gram.cols = lay.m;
+    gram.depth = lay.n;
+    gram.alpha = (squared ? 1.0f : b) / kScale;
+    gram.beta = (squared ? (float)(0.5 * b / c) : a) * kScale;
     if (squared) {
-        st.square = st.gram;
-        st.square.depth = lay.m;
-        st.square.alpha = c / kScale;
-        st.square.beta = (float)(a - 0.25 * (double)b * b / c) * kScale;
+        square.rows = square.cols = square.depth = lay.m;
+        square.alpha = c / kScale;
+        square.beta = (float)(a - 0.25 * (double)b * b / c) * kScale;
     }
-    st.apply.rows = st.apply.depth = lay.m;
-    st.apply.cols = lay.n;
-    st.apply.alpha = 1.0f / kScale;
+    apply.rows = apply.depth = lay.m;
+    apply.cols = lay.n;
+    apply.alpha = 1.0f / kScale;
     result.transposed = prep.transposed;
     result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
 
@@ -1361,10 +1377,10 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     if ((rc = plane_map(encode, &bout, am, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
     if ((rc = plane_map(encode, &pout, pm, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
     for (int k = 0; k < steps; ++k) {
-        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], squared ? bout : pout, st.gram, result, batch, sms, s))) return rc;
-        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, pout, st.square, result, batch, sms, s))) return rc;
-        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], xout[(k + 1) & 1], st.apply, result, batch, sms, s)
-                           : launch_gemm<kResult>(pmap, xright[k & 1], xout[0], st.apply, result, batch, sms, s);
+        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], squared ? bout : pout, gram, result, batch, sms, s))) return rc;
+        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, pout, square, result, batch, sms, s))) return rc;
+        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], xout[(k + 1) & 1], apply, result, batch, sms, s)
+                           : launch_gemm<kResult>(pmap, xright[k & 1], xout[0], apply, result, batch, sms, s);
         if (rc) return rc;
     }
     return CIMEKV_OK;
