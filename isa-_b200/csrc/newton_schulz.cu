@@ -23,7 +23,8 @@
 // checked on the host from the coefficients, so the fixed scale neither overflows
 // nor loses small elements), and a
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
-// tensor core products, closer to the exact result than fp32 FMAs.
+// tensor core products.  fp32 results are off by 0.6 to 1.9 times what products in
+// fp32 give (16 x 16 to 4096 x 4096).
 //
 // B and P are symmetric: only tiles on and below the diagonal are computed, the
 // epilogue stores each tile and its mirror image.
@@ -70,10 +71,10 @@ int launched(const char* what) {
 
 constexpr float kScale = 4096.0f;  // fp16 planes hold value * 2^12
 constexpr int kK = 64;             // depth of one stage: 64 halves = one 128-byte swizzle row
-constexpr int kMaxStages = 6;
+constexpr int kMaxStages = 6, kMaxBufs = 8;
 
-// The three kinds of output tile (see product()), by their side.
-template <int kSide>
+// The three kinds of output tile (see product()), by their side, and how finely they sum.
+template <int kSide, bool kFine>
 struct Tile {
     static constexpr bool kPair = kSide == 256;
     static constexpr int kRanks = kPair ? 2 : 1;
@@ -86,12 +87,14 @@ struct Tile {
     static constexpr int kWarps = kSide == 64 ? 8 : 16;     // collecting warps
     static constexpr int kWarpCols = kSide / (kWarps / 4);  // result columns of a collecting warp
     static constexpr int kThreads = (kWarps + 2) * 32;      // and a copy warp, a product warp
-    static constexpr int kBufs = kPair ? 2 : kStages;       // accumulators in tensor memory
-    static constexpr int kChunk = kPair ? 2 : 1;            // stages summed in one of them; where it is one, stage and
-                                                            // accumulator s are filled and done together
+    static constexpr int kBufs = kSide == 64 ? 8 : kPair ? 2 : 4;   // accumulators in tensor memory
+    // Steps of 16 along K summed in one of them: half a stage or (fast) a stage, of a pair a
+    // stage or (fast) two; the parts of a stage, and the stages, that this makes.
+    static constexpr int kSums = (kPair ? 4 : 2) * (kFine ? 1 : 2);
+    static constexpr int kParts = kSums < 4 ? 4 / kSums : 1, kSpan = kSums > 4 ? kSums / 4 : 1;
     static constexpr int kColumns = 512;                    // tensor memory columns taken: all
     static constexpr int kStaging = kWarpRows * 64;         // a collecting warp's row segments on their way out
-    static constexpr int kSmem = kStages * kStageBytes + kWarps * kStaging + 1024;
+    static constexpr int smem() { return kStages * kStageBytes + kWarps * kStaging + 1024; }
 };
 
 constexpr int kMaxTable = CIMEKV_MUON_MAX_MATRICES;
@@ -738,20 +741,23 @@ struct Pipe {
 // for a pair) feeds only the pair's tensor cores, which is why many tiles go to
 // pairs and few to the tile that spreads them over the most SMs.
 //
-// The tensor core adds into fp32 accumulators by cutting off, not by rounding:
-// over a long depth that is a drift of half a step per addition.  So every stage
-// (4 additions at full size, the small cross products before them; two stages of a
-// pair) goes into a fresh accumulator, one of several, and the collecting warps add
-// them in registers with round-to-nearest while the next ones run.  The same
-// accumulators let the next tile start while the last one is stored.
-template <int M, int kSide>
+// The tensor core aligns the 16 products of a step and the accumulator to the largest
+// of them and cuts off below about 2^-25 of it (a model of that on the CPU gives
+// the errors that are measured), so errors grow with what is already summed and all
+// have one sign.  So a few steps (the small cross products before those at full size) go
+// into a fresh accumulator, one of several, and the collecting warps add them in
+// registers with round-to-nearest while the next ones run.  Fine sums: 192 x 192 is off
+// by 2.0e-6 where fp32 products are by 1.6e-6 (fast: 2.8e-6), 48 of 768 x 768 by 2.3e-6
+// (fp32 products 2.5e-6, fast 4.6e-6), in 1,442 us (fast 1,385), 40 of 192 x 192 in 137
+// (fast 123).  The same accumulators let the next tile start while the last one is stored.
+template <int M, int kSide, bool kFine>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
                                         const CUtensorMap* out, const Product& p, const Result& result, int batch, int first, int step, int tiles,
                                         int mode = M, int matrix = -1) {
-    using T = Tile<kSide>;
+    using T = Tile<kSide, kFine>;
     constexpr bool kPair = T::kPair;
     constexpr int kRanks = T::kRanks, kRows = T::kRows, kOperand = T::kOperand, kStageBytes = T::kStageBytes;
-    constexpr int kWarpCols = T::kWarpCols, kWarps = T::kWarps, kBufs = T::kBufs, kChunk = T::kChunk;
+    constexpr int kWarpCols = T::kWarpCols, kWarps = T::kWarps, kBufs = T::kBufs;
     constexpr int kStages = T::kStages;
     const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;  // known to be uniform
     const int ni = (p.rows + kSide - 1) / kSide, nj = (p.cols + kSide - 1) / kSide;
@@ -791,7 +797,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             for (int k = 0; k < ksteps; ++k, q.fill.next(kStages)) {
                 const int s = q.fill.at;
                 // (the phase before a barrier's first has ended by definition)
-                if (!(q.ok = mbar_wait((kChunk == 1 ? q.acc_full : q.empty) + 8 * s, q.fill.parity ^ 1))) break;
+                if (!(q.ok = mbar_wait(q.empty + 8 * s, q.fill.parity ^ 1))) break;
                 const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
                 if (elect_one()) {
                     if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
@@ -821,33 +827,37 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                 int b, row0, col0;
                 place(t, b, row0, col0);
                 const int r_at = square && row0 == col0 ? 0 : 2 * kOperand;  // on the diagonal L is R
-                for (int k = 0; k < ksteps && q.ok; q.chunk.next(kBufs)) {
-                    const int buf = q.chunk.at;
-                    if (!(q.ok = mbar_wait(q.acc_empty + 8 * buf, q.chunk.parity ^ 1))) break;
-                    const uint32_t d = q.tmem + buf * kSide;
-                    const int end = min(k + kChunk, ksteps);
-                    for (uint32_t more = 0; k < end; ++k, q.fill.next(kStages), more = 1) {
-                        const int s = q.fill.at;
-                        if (!(q.ok = mbar_wait(q.full + 8 * s, q.fill.parity))) break;
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        const uint32_t base = q.stages + s * kStageBytes;
-                        // both planes of either operand; a step of 16 along K moves the address alone
-                        const uint64_t l0 = operand_desc(base, 16, 1024), l1 = operand_desc(base + kOperand, 16, 1024);
-                        const uint64_t r0 = operand_desc(base + r_at, square ? 16 : 8192, 1024);
-                        const uint64_t r1 = operand_desc(base + r_at + kOperand, square ? 16 : 8192, 1024);
-                        const uint64_t kL = 32 >> 4, kR = (square ? 32 : 2048) >> 4;
+                for (int k = 0; k < ksteps && q.ok; ++k, q.fill.next(kStages)) {
+                    const int s = q.fill.at;
+                    if (!(q.ok = mbar_wait(q.full + 8 * s, q.fill.parity))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t base = q.stages + s * kStageBytes;
+                    // both planes of either operand; a step of 16 along K moves the address alone
+                    const uint64_t l0 = operand_desc(base, 16, 1024), l1 = operand_desc(base + kOperand, 16, 1024);
+                    const uint64_t r0 = operand_desc(base + r_at, square ? 16 : 8192, 1024);
+                    const uint64_t r1 = operand_desc(base + r_at + kOperand, square ? 16 : 8192, 1024);
+                    const uint64_t kL = 32 >> 4, kR = (square ? 32 : 2048) >> 4;
+                    constexpr int kHere = kK / 16 / T::kParts;  // steps of a part
+                    const bool fresh = k % T::kSpan == 0, last = (k + 1) % T::kSpan == 0 || k + 1 == ksteps;
+#pragma unroll
+                    for (int part = 0; part < T::kParts; ++part) {
+                        const int buf = q.chunk.at;
+                        if (fresh && !(q.ok = mbar_wait(q.acc_empty + 8 * buf, q.chunk.parity ^ 1))) break;
+                        const uint32_t d = q.tmem + buf * kSide;
                         if (elect_one()) {
 #pragma unroll
-                            for (uint64_t i = 0; i < kK / 16; ++i) {
-                                mma_f16<kPair>(d, l0 + i * kL, r1 + i * kR, idesc, i ? 1u : more);
+                            for (uint64_t i = part * kHere; i < (part + 1) * kHere; ++i) {
+                                mma_f16<kPair>(d, l0 + i * kL, r1 + i * kR, idesc, i != part * kHere || !fresh);
                                 mma_f16<kPair>(d, l1 + i * kL, r0 + i * kR, idesc, 1);
                             }
 #pragma unroll
-                            for (uint64_t i = 0; i < kK / 16; ++i) mma_f16<kPair>(d, l0 + i * kL, r0 + i * kR, idesc, 1);
-                            if (kChunk > 1) mma_commit<kPair>(q.empty + 8 * s);
-                            if (k + 1 == end) mma_commit<kPair>(q.acc_full + 8 * buf);
+                            for (uint64_t i = part * kHere; i < (part + 1) * kHere; ++i)
+                                mma_f16<kPair>(d, l0 + i * kL, r0 + i * kR, idesc, 1);
+                            if (last) mma_commit<kPair>(q.acc_full + 8 * buf);
+                            if (part + 1 == T::kParts) mma_commit<kPair>(q.empty + 8 * s);
                         }
                         __syncwarp();
+                        if (last) q.chunk.next(kBufs);
                     }
                 }
             }
@@ -869,7 +879,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
-            for (int k = 0; k < ksteps; k += kChunk, q.chunk.next(kBufs)) {
+            for (int k = 0; k < ksteps * (kK / 16); k += T::kSums, q.chunk.next(kBufs)) {
                 const int buf = q.chunk.at;
                 q.ok = q.ok && mbar_wait(q.acc_full + 8 * buf, q.chunk.parity);
                 q.ok = __all_sync(0xffffffffu, q.ok);
@@ -909,15 +919,15 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
 }
 
 // Barriers, tensor memory.  All threads.
-template <int kSide>
+template <typename T>
 __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tmem_slot, uint8_t* smem_raw) {
-    constexpr bool kPair = Tile<kSide>::kPair;
-    constexpr int kStages = Tile<kSide>::kStages;
+    constexpr bool kPair = T::kPair;
+    constexpr int kStages = T::kStages;
     q.stages = (smem_addr(smem_raw) + 1023) & ~1023u;
     q.full = smem_addr(bars);
     q.empty = q.full + 8 * kStages;
     q.acc_full = q.full + 16 * kStages;
-    q.acc_empty = q.acc_full + 8 * kMaxStages;
+    q.acc_empty = q.acc_full + 8 * kMaxBufs;
     q.rank = kPair ? cluster_rank() : 0;
     q.fill = q.chunk = {0, 0};
     q.ok = true;
@@ -926,14 +936,14 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
             mbar_init(q.full + 8 * s, 1);
             mbar_init(q.empty + 8 * s, 1);
         }
-        for (int s = 0; s < Tile<kSide>::kBufs; ++s) {
+        for (int s = 0; s < T::kBufs; ++s) {
             mbar_init(q.acc_full + 8 * s, 1);
-            mbar_init(q.acc_empty + 8 * s, Tile<kSide>::kWarps * Tile<kSide>::kRanks);
+            mbar_init(q.acc_empty + 8 * s, T::kWarps * T::kRanks);
         }
-        mbar_init(q.acc_empty + 8 * kMaxStages, 1);
+        mbar_init(q.acc_empty + 8 * kMaxBufs, 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if ((threadIdx.x >> 5) == Tile<kSide>::kWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), Tile<kSide>::kColumns);
+    if ((threadIdx.x >> 5) == T::kWarps + 1) tmem_alloc<kPair>(smem_addr(tmem_slot), T::kColumns);
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
     if constexpr (kPair) cluster_sync();
@@ -943,18 +953,18 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
 
 // Nothing may be in flight when the CTA leaves: copies (a pair's are all
 // counted in the first CTA), products.  All threads.
-template <int kSide>
+template <typename T>
 __device__ __forceinline__ void pipe_close(Pipe& q) {
-    constexpr bool kPair = Tile<kSide>::kPair;
-    constexpr int kWarps = Tile<kSide>::kWarps, kStages = Tile<kSide>::kStages;
+    constexpr bool kPair = T::kPair;
+    constexpr int kWarps = T::kWarps, kStages = T::kStages;
     const int warp = threadIdx.x >> 5;
     if (warp == kWarps && q.rank == 0) {
         // a stage before the turn was last filled in this phase, the others in the one before
         for (int s = 0; s < kStages; ++s) mbar_wait(q.full + 8 * s, s < q.fill.at ? q.fill.parity : q.fill.parity ^ 1);
     } else if (warp == kWarps + 1 && q.rank == 0) {
-        if (elect_one()) mma_commit<kPair>(q.acc_empty + 8 * kMaxStages);
+        if (elect_one()) mma_commit<kPair>(q.acc_empty + 8 * kMaxBufs);
         __syncwarp();
-        mbar_wait(q.acc_empty + 8 * kMaxStages, 0);
+        mbar_wait(q.acc_empty + 8 * kMaxBufs, 0);
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
@@ -962,27 +972,28 @@ __device__ __forceinline__ void pipe_close(Pipe& q) {
     if (warp == kWarps + 1) {
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        tmem_free<kPair>(q.tmem, Tile<kSide>::kColumns);
+        tmem_free<kPair>(q.tmem, T::kColumns);
     }
 }
 
 // One product of all matrices, a persistent loop over its tiles.
-template <int M, int kSide>
-__global__ void __launch_bounds__(Tile<kSide>::kThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
+template <int M, int kSide, bool kFine>
+__global__ void __launch_bounds__(Tile<kSide, kFine>::kThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
                                                                            const __grid_constant__ CUtensorMap right,
                                                                            const __grid_constant__ CUtensorMap out,
                                                                            const __grid_constant__ Product p,
                                                                            const __grid_constant__ Result result, int batch,
                                                                            int tiles) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[4 * kMaxStages + 1];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBufs + 1];
     __shared__ uint32_t tmem_slot;
     Pipe q;
-    pipe_open<kSide>(q, bars, &tmem_slot, smem_raw);
+    using T = Tile<kSide, kFine>;
+    pipe_open<T>(q, bars, &tmem_slot, smem_raw);
     chain();
-    constexpr int kRanks = Tile<kSide>::kRanks;
-    product<M, kSide>(q, &left, &right, &out, p, result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
-    pipe_close<kSide>(q);
+    constexpr int kRanks = T::kRanks;
+    product<M, kSide, kFine>(q, &left, &right, &out, p, result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
+    pipe_close<T>(q);
 }
 
 // All steps in one kernel, for matrices whose products are a few microseconds
@@ -1025,16 +1036,17 @@ __device__ __forceinline__ void group_meet(unsigned* arrivals, unsigned target, 
     asm volatile("fence.proxy.async.global;" ::: "memory");
 }
 
-__global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
+template <bool kFine>
+__global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
                                                                          const __grid_constant__ Steps st,
                                                                          const __grid_constant__ Result result, int batch) {
     extern __shared__ uint8_t smem_raw[];
-    __shared__ __align__(8) uint64_t bars[4 * kMaxStages + 1];
+    __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBufs + 1];
     __shared__ uint32_t tmem_slot;
     __shared__ int lost;
     if (threadIdx.x == 0) lost = 0;
     Pipe q;
-    pipe_open<64>(q, bars, &tmem_slot, smem_raw);
+    pipe_open<Tile<64, kFine>>(q, bars, &tmem_slot, smem_raw);
     const int ni = (st.product[0].rows + 63) / 64, nj = (st.product[2].cols + 63) / 64;
     const int rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
     for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
@@ -1046,14 +1058,14 @@ __global__ void __launch_bounds__(Tile<64>::kThreads, 1) ns_steps_kernel(const _
                 const int mode = i < 2 ? kFull : k + 1 < st.steps ? kApply : kResult;
                 const int tiles = ni * (i < 2 ? ni : nj);
                 const CUtensorMap* const x = &maps.x[k & 1];
-                product<kAny, 64>(q, i == 0 ? x : i == 1 ? &maps.b : &maps.p, i == 1 ? &maps.b : x,
+                product<kAny, 64, kFine>(q, i == 0 ? x : i == 1 ? &maps.b : &maps.p, i == 1 ? &maps.b : x,
                                   i == 0 && st.squared ? &maps.b_out : i < 2 ? &maps.p_out : &maps.x_out[(k + 1) & 1],
                                   st.product[i], result, batch, rank, st.group, tiles, mode, matrix);
                 if (mode != kResult) group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost);
             }
         }
     }
-    pipe_close<64>(q);
+    pipe_close<Tile<64, kFine>>(q);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -1206,15 +1218,16 @@ int launch_chained(const char* what, void (*kernel)(Args...), dim3 grid, int thr
     return fail(CIMEKV_ECUDA, msg);
 }
 
-template <int M, int kSide>
+template <int M, int kSide, bool kFine>
 int launch_as(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result, int batch, int sms,
               cudaStream_t s) {
+    using T = Tile<kSide, kFine>;
     static std::atomic<uint64_t> allowed{0};
-    if (int rc = allow_smem(ns_gemm_kernel<M, kSide>, Tile<kSide>::kSmem, allowed)) return rc;
-    constexpr int ranks = Tile<kSide>::kRanks;
+    if (int rc = allow_smem(ns_gemm_kernel<M, kSide, kFine>, T::smem(), allowed)) return rc;
+    constexpr int ranks = T::kRanks;
     const long long tiles = tile_count(M, kSide, p.rows, p.cols) * batch, most = sms / ranks;
-    return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kSide>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
-                          Tile<kSide>::kThreads, Tile<kSide>::kSmem, ranks, s, l, r, out, p, result, batch, (int)tiles);
+    return launch_chained("ns_gemm_kernel", ns_gemm_kernel<M, kSide, kFine>, dim3((unsigned)(tiles < most ? tiles : most) * ranks),
+                          T::kThreads, T::smem(), ranks, s, l, r, out, p, result, batch, (int)tiles);
 }
 
 // What a product takes, in cycles: a part that does not depend on its size (launch
@@ -1235,10 +1248,14 @@ double cost_of(int side, int mode, int rows, int cols, int depth, int batch, int
 }
 
 template <int M>
-int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result, int batch, int sms,
-                cudaStream_t s) {
+int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result,
+                int batch, int sms, bool fine, cudaStream_t s) {
     const bool pair = cost_of(256, M, p.rows, p.cols, p.depth, batch, sms) < cost_of(128, M, p.rows, p.cols, p.depth, batch, sms);
-    return pair ? launch_as<M, 256>(l, r, out, p, result, batch, sms, s) : launch_as<M, 128>(l, r, out, p, result, batch, sms, s);
+    if (fine)
+        return pair ? launch_as<M, 256, true>(l, r, out, p, result, batch, sms, s)
+                    : launch_as<M, 128, true>(l, r, out, p, result, batch, sms, s);
+    return pair ? launch_as<M, 256, false>(l, r, out, p, result, batch, sms, s)
+                : launch_as<M, 128, false>(l, r, out, p, result, batch, sms, s);
 }
 
 // CTAs per matrix when all steps run in one kernel, 0 where a kernel for each
@@ -1315,6 +1332,9 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
 
     // sums of products of two planes are 2^24 times the value, planes 2^12 times
     const bool squared = c != 0.0f;
+    // Sums as fine as an fp32 result shows.  A 16-bit result's own rounding, or that of
+    // an fp32 parameter that moves by a small part of its size, hides the difference.
+    const bool fine = result.dst.type == CIMEKV_F32 && !result.update;
     Steps st = {};
     Product &gram = st.product[0], &square = st.product[1], &apply = st.product[2];
     st.steps = steps;
@@ -1336,7 +1356,8 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
 
     if (const int group = steps_group(batch, lay.m, lay.n, squared, sms)) {
         StepMaps maps;
-        constexpr int out_rows = Tile<64>::kWarpRows;
+        using T = Tile<64, true>;  // sizes are those of the fast one too
+        constexpr int out_rows = T::kWarpRows;
         for (int i = 0; i < 2; ++i) {
             if ((rc = plane_map(encode, &maps.x[i], x[i], batch, lay.m, lay.n, lay.xp, 64))) return rc;
             if ((rc = plane_map(encode, &maps.x_out[i], x[i], batch, lay.m, lay.n, lay.xp, out_rows, true))) return rc;
@@ -1345,22 +1366,23 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
         if ((rc = plane_map(encode, &maps.p, pm, batch, lay.m, lay.m, lay.ap, 64))) return rc;
         if ((rc = plane_map(encode, &maps.b_out, am, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
         if ((rc = plane_map(encode, &maps.p_out, pm, batch, lay.m, lay.m, lay.ap, out_rows, true))) return rc;
-        static std::atomic<uint64_t> allowed{0};
-        if ((rc = allow_smem(ns_steps_kernel, Tile<64>::kSmem, allowed))) return rc;
+        static std::atomic<uint64_t> allowed[2];
+        const auto kernel = fine ? ns_steps_kernel<true> : ns_steps_kernel<false>;
+        if ((rc = allow_smem(kernel, T::smem(), allowed[fine]))) return rc;
         st.arrivals = prep.arrivals;
         st.group = group;
         const int most = sms / group;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)(batch < most ? batch : most) * group);
-        cfg.blockDim = dim3(Tile<64>::kThreads);
-        cfg.dynamicSmemBytes = Tile<64>::kSmem;
+        cfg.blockDim = dim3(T::kThreads);
+        cfg.dynamicSmemBytes = T::smem();
         cfg.stream = s;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeCooperative;
         attr[0].val.cooperative = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
-        const cudaError_t e = cudaLaunchKernelEx(&cfg, ns_steps_kernel, maps, st, result, batch);
+        const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, maps, st, result, batch);
         if (e == cudaSuccess) return CIMEKV_OK;
         (void)cudaGetLastError();
         return fail(CIMEKV_ECUDA, cudaGetErrorString(e));
@@ -1377,10 +1399,10 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     if ((rc = plane_map(encode, &bout, am, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
     if ((rc = plane_map(encode, &pout, pm, batch, lay.m, lay.m, lay.ap, 32, true))) return rc;
     for (int k = 0; k < steps; ++k) {
-        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], squared ? bout : pout, gram, result, batch, sms, s))) return rc;
-        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, pout, square, result, batch, sms, s))) return rc;
-        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], xout[(k + 1) & 1], apply, result, batch, sms, s)
-                           : launch_gemm<kResult>(pmap, xright[k & 1], xout[0], apply, result, batch, sms, s);
+        if ((rc = launch_gemm<kSymmetric>(xleft[k & 1], xleft[k & 1], squared ? bout : pout, gram, result, batch, sms, fine, s))) return rc;
+        if (squared && (rc = launch_gemm<kSymmetric>(bmap, bmap, pout, square, result, batch, sms, fine, s))) return rc;
+        rc = k + 1 < steps ? launch_gemm<kApply>(pmap, xright[k & 1], xout[(k + 1) & 1], apply, result, batch, sms, fine, s)
+                           : launch_gemm<kResult>(pmap, xright[k & 1], xout[0], apply, result, batch, sms, fine, s);
         if (rc) return rc;
     }
     return CIMEKV_OK;

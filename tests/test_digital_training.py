@@ -185,7 +185,7 @@ def test_muon_optimizer_against_the_formula(dev):
             m = 0.95 * m + 0.05 * p.grad.double()
             u = 0.95 * m + 0.05 * p.grad.double() if p is fused else m
             lr, parts = (0.02, 3) if p is fused else (0.01, 1)
-            o, bound = zip(*(_exact(t) for t in u.chunk(parts)))
+            o, bound = zip(*(_exact(t, fine=False) for t in u.chunk(parts)))
             # fp32 momenta: a relative rounding of 8 u in the update, at most times the growth of five steps
             bounds[p] += lr * (sum(bound) + parts * 8 * U * 3.4445 ** 5) + 4 * U * float(w.norm())
             want[p] = (w * (1 - lr * 0.05) - lr * torch.cat(o), m)  # none of these matrices is tall: s = 1

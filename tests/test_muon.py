@@ -1,9 +1,10 @@
 """Newton-Schulz orthogonalisation and the Muon step against their definitions in 64 bits.
 
 Bound.  u = 2^-24.  An operand held as two fp16 planes is off by 2^-22 of its value (half a step of 11 bits, twice);
-a product of two drops lo x lo, another 2^-22 of |L| |R|, and adds in fp32: at most 16 truncated additions (2 u each) to an
-accumulator, the accumulators rounded:
-e = 3 * 2^-22 + (32 + K / 64) u of |L| |R|, whose norm is at most |L|_F |R|_F.  With A = X X^T, P = a I + b A + c A^2
+a product of two drops lo x lo, another 2^-22 of |L| |R|.  A step of the tensor core (16 products) cuts the products
+and the sum so far off below 2^-25 of the largest: 17 / 2 u.  Of such steps with terms at full size an accumulator takes
+at most 4 for fp32 results and 16 otherwise, and the accumulators are added in fp32, K / 64 of them at most:
+e = 3 * 2^-22 + (34 or 136 + K / 64) u of |L| |R|, whose norm is at most |L|_F |R|_F.  With A = X X^T, P = a I + b A + c A^2
 (computed as c B^2 + ..., B = A + b / 2c I, so |B| <= max(|b / 2c|, |A + b / 2c|)) one step X' = P X adds
 
     dA = e |X|_F^2 + 2^-22 |B|_F,  dP = |c| (2 |B|_2 dA + e |B|_F^2) + 2^-22 |P|_F  (c = 0: dP = |b| dA + 2^-22 |P|_F),
@@ -28,9 +29,10 @@ def _ops():
     return cuda_orthogonalize, cuda_muon_step
 
 
-def _exact(g, steps=5, coefficients=NS, eps=1e-7):
+def _exact(g, steps=5, coefficients=NS, eps=1e-7, fine=None):
     """(result, bound on the Frobenius norm of the error) of one matrix, in 64 bits."""
     a, b, c = coefficients
+    cut = 34 if (g.dtype == F32 if fine is None else fine) else 136
     x = g.double()
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
@@ -44,7 +46,7 @@ def _exact(g, steps=5, coefficients=NS, eps=1e-7):
         new = P @ x
         s = torch.linspace(0, 1, 257, dtype=torch.float64) * float(torch.linalg.matrix_norm(x, 2))
         lip = float(torch.maximum((a + 3 * b * s ** 2 + 5 * c * s ** 4).abs(), (a + b * s ** 2 + c * s ** 4).abs()).max())
-        e = lambda k: 3 * 2.0 ** -22 + (32 + k / 64) * U  # noqa: E731
+        e = lambda k: 3 * 2.0 ** -22 + (cut + k / 64) * U  # noqa: E731
         B = A + (0.5 * b / c if c else 0.0) * eye
         fro, two = (lambda t: float(t.norm())), (lambda t: float(torch.linalg.matrix_norm(t, 2)))  # noqa: E731
         dA = e(n) * fro(x) ** 2 + 2.0 ** -22 * fro(B)
@@ -332,7 +334,7 @@ def _want_step(p, g, m, lr, momentum=0.95, nesterov=True, weight_decay=0.1, matc
     # three roundings of the momentum, and its parameters' own in fp32
     dm = 4 * U * (m0.abs() + g.abs())
     u = momentum * new + (1 - momentum) * g if nesterov else new
-    o, bound = _exact(u)
+    o, bound = _exact(u, fine=False)
     rows, cols = p.shape
     s = 0.2 * math.sqrt(max(rows, cols)) if match_rms else math.sqrt(max(1.0, rows / cols))
     # the update's rounding (4 u of |m| + |g|) enters like the planes' rounding, times the steps' growth a^5
