@@ -294,7 +294,7 @@ int cimekv_layer_norm_backward(const void* dy, int y_type, long long dy_stride,
  * r*row_stride (elements), rows are contiguous; out [batch][rows][cols] is
  * contiguous, of the same type, and does not overlap g.  Products run on the tensor
  * cores with operands of 22 bits and fp32 accumulation.  Coefficients that let
- * a singular value grow beyond 3.9 are refused.  A matrix with a NaN or an
+ * a singular value grow beyond 3.9 are refused, and eps below 1e-30.  A matrix with a NaN or an
  * infinity gives NaN in all its elements and leaves the others alone.
  * workspace: cimekv_orthogonalize_workspace_bytes(batch, rows, cols), 256-byte
  * aligned; its content does not matter.  The result is deterministic.

@@ -1145,7 +1145,8 @@ int check_iteration(int batch, int rows, int cols, int steps, float a, float b, 
     const long long tiles = ((rows + 127LL) / 128) * ((cols + 127LL) / 128) * batch;
     if (tiles > 0x3fffffff) return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: too many elements for one call");
     if (steps < 1 || steps > 64) return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: 1 to 64 steps");
-    if (!(eps > 0.0f)) return fail(CIMEKV_EINVAL_SHAPE, "eps must be > 0");
+    // 2^12 / eps must be finite, or a matrix of zeros would give NaN
+    if (!(eps >= 1e-30f)) return fail(CIMEKV_EINVAL_SHAPE, "eps must be at least 1e-30");
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
         return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: coefficients must be finite");
     // Largest singular values of X, B and P over the steps: they must fit the

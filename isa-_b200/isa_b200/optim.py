@@ -22,7 +22,8 @@ class Muon(torch.optim.Optimizer):
     A group's ``matrices`` is the number of matrices stacked along a parameter's
     rows: 3 for a fused query / key / value projection, whose three parts are
     orthogonalised separately.  ``lr`` may be a one-element fp32 CUDA tensor, which
-    a captured step reads at each replay.  Momenta are fp32.
+    a captured step reads at each replay; the first step, which makes the momenta,
+    cannot be captured.  Momenta are fp32.
     """
 
     def __init__(self, params, lr=1e-3, momentum: float = 0.95, nesterov: bool = True, weight_decay: float = 0.1,
@@ -73,6 +74,8 @@ class Muon(torch.optim.Optimizer):
                     raise RuntimeError("Muon does not take sparse gradients")
                 state = self.state[p]
                 if "momentum_buffer" not in state:
+                    if p.is_cuda and torch.cuda.is_current_stream_capturing():  # every replay would begin with zeros
+                        raise RuntimeError("Muon's first step cannot be captured: take one step before the capture")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 shape = (*p.shape[:-2], k, p.shape[-2] // k, p.shape[-1]) if k > 1 else p.shape
                 params.append(p.view(shape))

@@ -221,6 +221,42 @@ def test_muon_state_dict_round_trip(dev, dtype):
 
 
 @gpu
+def test_muon_captured_step(dev):
+    """The first step makes the momenta and is refused in a capture; a later one replays as the plain step."""
+    from isa_b200.optim import Muon
+    torch.manual_seed(3)
+    a = nn.Parameter(torch.randn(40, 72, device=dev))
+    a.grad = torch.randn_like(a)
+    before = a.detach().clone()
+    opt = Muon([a], lr=0.02)
+    with pytest.raises(RuntimeError, match="first step"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            opt.step()
+    assert torch.equal(a, before)
+    opt.step()
+    b = nn.Parameter(a.detach().clone())
+    b.grad = a.grad.clone()
+    plain = Muon([b], lr=0.02)
+    plain.load_state_dict(opt.state_dict())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    for seed in range(3):
+        a.grad.copy_(torch.randn(40, 72, generator=torch.Generator().manual_seed(seed)))
+        b.grad.copy_(a.grad)
+        graph.replay()
+        plain.step()
+        assert torch.equal(a, b)
+    assert torch.equal(opt.state[a]["momentum_buffer"], plain.state[b]["momentum_buffer"])
+
+
+@gpu
+def test_muon_zero_matrix_at_the_smallest_eps(dev):
+    from isa_b200.kernels.muon import cuda_orthogonalize
+    assert not cuda_orthogonalize(torch.zeros(2, 20, 30, device=dev), eps=1e-30).any()
+
+
+@gpu
 def test_training_steps_of_everything(dev):
     """Fused norms, CIM layers and Muon with AdamW in the package's own training step: it runs, and Muon's matrices
     and the norms move.  (A step of Muon does not depend on the gradient's size; AdamW's does below its eps, where the

@@ -108,6 +108,7 @@ def test_c_entry_refusals_before_any_launch():
     assert orth(batch=65535, rows=32768, cols=32768) == 1 and b"too many" in err()
     assert orth(steps=0) == 1 and orth(steps=65) == 1 and b"steps" in err()
     assert orth(eps=0.0) == 1 and orth(eps=float("nan")) == 1
+    assert orth(eps=1e-38) == 1 and b"at least 1e-30" in err()
     assert orth(c=(float("nan"), 0.0, 0.0)) == 1 and b"finite" in err()
     assert orth(c=(8.0, 0.0, 0.0)) == 1 and b"beyond 3.9" in err()  # grows without bound
     assert orth(c=(1.5, -0.5, 1e-4)) == 1 and b"beyond 15" in err()  # b / 2c does not fit
