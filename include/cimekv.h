@@ -323,6 +323,21 @@ int cimekv_muon_step(int count, void* const* params, const void* const* grads, f
                      void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * Steps of several shapes side by side: small matrices leave most SMs idle.
+ * cimekv_muon_shares gives each of `groups` steps (count matrices of rows x cols) its
+ * share of the `sms` SMs (0: the current device's), so that they end together, or 0
+ * where it is to have all of them, before or after the others.  cimekv_muon_step_on is
+ * cimekv_muon_step on `share` SMs (0: all, otherwise at least 2); steps that
+ * run at the same time need a stream and a workspace each.
+ */
+int cimekv_muon_shares(int groups, const int* counts, const int* rows, const int* cols, float c, int sms, int* shares);
+int cimekv_muon_step_on(int share, int count, void* const* params, const void* const* grads, float* const* momenta,
+                        int p_type, int g_type, int rows, int cols, float lr, const float* lr_device,
+                        float momentum, int nesterov, float weight_decay, float scale,
+                        int steps, float a, float b, float c, float eps,
+                        void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Debug support, no counterpart in the reference.  cimekv_debug_build()
  * returns 1 for the library variant built with CIMEKV_DEBUG_BOUNDS=1
  * (libcimekv_debug.so), whose kernels check every table index against the

@@ -1274,7 +1274,11 @@ int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& o
 // product costs less.  Measured a call, one kernel against fifteen: 73 against 112 us
 // for one 192 x 192 matrix, 131 against 202 for 768 x 768, 120 against 135 for 40 of
 // 192 x 192; 252 against 239 for 1024 x 1024, 176 against 159 for 12 of 384 x 384.
-int steps_group(int batch, int m, int n, bool squared, int sms) {
+struct StepCost {
+    int group;              // CTAs of a matrix in the one kernel
+    double together, each;  // cycles of a step: one kernel, a kernel for each product
+};
+StepCost step_cost(int batch, int m, int n, bool squared, int sms) {
     const long long tiles = tile_count(kApply, 64, m, n), most = std::max(1LL, std::min<long long>(tiles, sms / batch));
     const long long group = ceil_div(tiles, ceil_div(tiles, most));  // no more than the rounds need
     const long long turns = ceil_div(batch, std::max(1LL, sms / group));
@@ -1285,7 +1289,7 @@ int steps_group(int batch, int m, int n, bool squared, int sms) {
         return std::min(cost_of(128, mode, m, cols, depth, batch, sms), cost_of(256, mode, m, cols, depth, batch, sms));
     };
     const double each = apart(kSymmetric, m, n) + (squared ? apart(kSymmetric, m, m) : 0) + apart(kApply, n, m);
-    return together <= each ? (int)group : 0;
+    return {(int)group, together, each};
 }
 
 int type_bytes(int type) { return type == CIMEKV_F32 ? 4 : 2; }
@@ -1307,13 +1311,15 @@ bool rows_in_fours(const Matrices& m, int batch, int cols) {
 }
 
 // Everything after the arguments are checked: norms, X0, the steps, the result.
+// share: the SMs to use, by all steps in one kernel; 0 for all SMs.
 int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int steps, float a, float b, float c,
-        uint8_t* ws, cudaStream_t s) {
+        uint8_t* ws, int share, cudaStream_t s) {
     const Layout lay(batch, rows, cols);
     EncodeFn encode;
     int rc;
     int sms;
     if ((rc = encoder(&encode)) || (rc = sm_count(&sms))) return rc;
+    if (share) sms = std::min(sms, share);
     __half* x[2] = {reinterpret_cast<__half*>(ws + lay.x0), reinterpret_cast<__half*>(ws + lay.x1)};
     __half* am = reinterpret_cast<__half*>(ws + lay.a);
     __half* pm = reinterpret_cast<__half*>(ws + lay.p);
@@ -1366,7 +1372,9 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     result.transposed = prep.transposed;
     result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
 
-    if (const int group = steps_group(batch, lay.m, lay.n, squared, sms)) {
+    const StepCost cost = step_cost(batch, lay.m, lay.n, squared, sms);
+    if (share || cost.together <= cost.each) {
+        const int group = cost.group;
         StepMaps maps;
         using T = Tile<64, true>;  // sizes are those of the fast one too
         constexpr int out_rows = T::kWarpRows;
@@ -1452,16 +1460,76 @@ extern "C" int cimekv_orthogonalize(const void* g, int type, long long batch_str
     last.dst.base = out;
     last.dst.batch_stride = (long long)rows * cols;
     last.dst.type = type;
-    return run(prep, last, batch, rows, cols, steps, a, b, c, static_cast<uint8_t*>(workspace), (cudaStream_t)stream);
+    return run(prep, last, batch, rows, cols, steps, a, b, c, static_cast<uint8_t*>(workspace), 0, (cudaStream_t)stream);
 }
 
 extern "C" int cimekv_muon_step(int count, void* const* params, const void* const* grads, float* const* momenta,
                                 int p_type, int g_type, int rows, int cols, float lr, const float* lr_device,
                                 float momentum, int nesterov, float weight_decay, float scale, int steps, float a,
                                 float b, float c, float eps, void* workspace, size_t workspace_bytes, void* stream) {
+    return cimekv_muon_step_on(0, count, params, grads, momenta, p_type, g_type, rows, cols, lr, lr_device, momentum,
+                               nesterov, weight_decay, scale, steps, a, b, c, eps, workspace, workspace_bytes, stream);
+}
+
+// Which steps run side by side: those of small matrices, whose products are latency
+// and leave SMs idle, and which run in one kernel (or nearly would; large ones fill the
+// chip either way, and would hold their workspaces at the same time).  Every SM goes
+// to the step that then takes longest.  Measured: 40 of 192 x 192 with 10 of 192 x 768 in
+// 182 us a call, one after the other in 244.
+extern "C" int cimekv_muon_shares(int groups, const int* counts, const int* rows, const int* cols, float c, int sms,
+                                  int* shares) {
+    int rc = cimekv_internal_begin_call();
+    if (rc) return rc;
+    if (groups < 0 || (groups && (!counts || !rows || !cols || !shares)))
+        return fail(CIMEKV_EINVAL_SHAPE, "muon shares: null pointer or negative count");
+    for (int i = 0; i < groups; ++i) {
+        if (counts[i] < 0 || rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxSide || cols[i] > kMaxSide)
+            return fail(CIMEKV_EINVAL_SHAPE, "muon shares: bad size");
+        shares[i] = 0;
+    }
+    if (sms < 0) return fail(CIMEKV_EINVAL_SHAPE, "muon shares: negative number of SMs");
+    if (!sms && (rc = sm_count(&sms))) return rc;
+    constexpr int kMost = 16;  // side by side
+    int at[kMost], n = 0, left = sms;
+    double alone[kMost], cost[kMost], all = 0.0;
+    const auto of = [&](int i, int share) {
+        const int batch = std::min(counts[i], kMaxTable);
+        return step_cost(batch, std::min(rows[i], cols[i]), std::max(rows[i], cols[i]), c != 0.0f, share);
+    };
+    const auto calls = [&](int i) { return (double)ceil_div(counts[i], kMaxTable); };
+    for (int i = 0; i < groups && n < kMost && sms >= 2 * kMost; ++i) {
+        if (!counts[i] || !rows[i] || !cols[i]) continue;
+        const StepCost one = of(i, sms);
+        if (one.together > 1.25 * one.each) continue;
+        all += alone[n] = calls(i) * std::min(one.together, one.each);
+        at[n++] = i;
+    }
+    for (int k = 0; k < n; ++k) {  // half of the SMs by the times alone
+        shares[at[k]] = std::max(2, (int)(0.5 * sms * alone[k] / all));
+        left -= shares[at[k]];
+        cost[k] = calls(at[k]) * of(at[k], shares[at[k]]).together;
+    }
+    double longest = 0.0;
+    for (; n > 1; --left) {
+        const int k = (int)(std::max_element(cost, cost + n) - cost);
+        longest = cost[k];
+        if (left <= 0) break;
+        cost[k] = calls(at[k]) * of(at[k], ++shares[at[k]]).together;
+    }
+    // streams and events are about 10 us of the host's: a tenth has to be gained
+    if (n < 2 || longest > 0.9 * all) std::fill(shares, shares + groups, 0);
+    return CIMEKV_OK;
+}
+
+extern "C" int cimekv_muon_step_on(int share, int count, void* const* params, const void* const* grads,
+                                   float* const* momenta, int p_type, int g_type, int rows, int cols, float lr,
+                                   const float* lr_device, float momentum, int nesterov, float weight_decay, float scale,
+                                   int steps, float a, float b, float c, float eps, void* workspace,
+                                   size_t workspace_bytes, void* stream) {
     NvtxRange nvtx_range("cimekv_muon_step");
     int rc = cimekv_internal_begin_call();
     if (rc || (rc = check_iteration(count, rows, cols, steps, a, b, c, eps))) return rc;
+    if (share < 0 || share == 1) return fail(CIMEKV_EINVAL_SHAPE, "muon step: a share is 0 (all) or at least 2 SMs");
     if (count > kMaxTable) return fail(CIMEKV_EINVAL_SHAPE, "muon step: too many matrices for one call");
     if (!valid_type(p_type) || !valid_type(g_type)) return fail(CIMEKV_EINVAL_SHAPE, "unknown element type");
     if (!(momentum >= 0.0f && momentum <= 1.0f)) return fail(CIMEKV_EINVAL_SHAPE, "momentum must be in [0, 1]");
@@ -1503,5 +1571,5 @@ extern "C" int cimekv_muon_step(int count, void* const* params, const void* cons
     last.lr_dev = lr_device;
     last.decay = weight_decay;
     last.scale = scale;
-    return run(prep, last, count, rows, cols, steps, a, b, c, static_cast<uint8_t*>(workspace), (cudaStream_t)stream);
+    return run(prep, last, count, rows, cols, steps, a, b, c, static_cast<uint8_t*>(workspace), share, (cudaStream_t)stream);
 }

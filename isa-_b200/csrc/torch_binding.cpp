@@ -5,6 +5,7 @@
 // interpreter.  The library's entry points are handed over by address (bind), so
 // this module works with whichever build of the library is loaded.
 
+#include <ATen/cuda/CUDAEvent.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -37,7 +38,8 @@ struct Library {
     decltype(&cimekv_layer_norm_workspace_bytes) norm_workspace = nullptr;
     decltype(&cimekv_orthogonalize) orthogonalize = nullptr;
     decltype(&cimekv_orthogonalize_workspace_bytes) orthogonalize_workspace = nullptr;
-    decltype(&cimekv_muon_step) muon_step = nullptr;
+    decltype(&cimekv_muon_shares) muon_shares = nullptr;
+    decltype(&cimekv_muon_step_on) muon_step_on = nullptr;
 } lib;
 
 void bind(const std::map<std::string, uintptr_t>& at) {
@@ -48,7 +50,8 @@ void bind(const std::map<std::string, uintptr_t>& at) {
     get(lib.norm_workspace, "cimekv_layer_norm_workspace_bytes");
     get(lib.orthogonalize, "cimekv_orthogonalize");
     get(lib.orthogonalize_workspace, "cimekv_orthogonalize_workspace_bytes");
-    get(lib.muon_step, "cimekv_muon_step");
+    get(lib.muon_shares, "cimekv_muon_shares");
+    get(lib.muon_step_on, "cimekv_muon_step_on");
 }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (status ", rc, "): ", lib.last_error()); }
@@ -297,7 +300,39 @@ struct Group {
     std::vector<float*> momenta;
 };
 
-// scales: per shape, computed by the caller from (rows, cols).
+// Streams beside the current one: they begin after what it has been given so far, and
+// join() (or the end, if a launch failed) lets it wait for them.
+class Beside {
+public:
+    explicit Beside(c10::DeviceIndex device) : main_(c10::cuda::getCurrentCUDAStream(device)) { begin_.record(main_); }
+    ~Beside() {
+        try {
+            join();
+        } catch (...) {
+        }
+    }
+    c10::cuda::CUDAStream next() {
+        const auto s = c10::cuda::getStreamFromPool(false, main_.device_index());
+        begin_.block(s);
+        sides_.push_back(s);
+        return s;
+    }
+    void join() {
+        while (!sides_.empty()) {
+            const auto s = sides_.back();
+            sides_.pop_back();
+            at::cuda::CUDAEvent end;
+            end.record(s);
+            end.block(main_);
+        }
+    }
+
+private:
+    c10::cuda::CUDAStream main_;
+    at::cuda::CUDAEvent begin_;
+    std::vector<c10::cuda::CUDAStream> sides_;
+};
+
 void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& grads, const std::vector<Tensor>& momenta,
                double lr, const OptTensor& lr_tensor, double momentum, bool nesterov, double weight_decay, int64_t steps,
                std::array<double, 3> c, double eps, bool match_rms) {
@@ -369,19 +404,49 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
         }
     }
     const int64_t most = CIMEKV_MUON_MAX_MATRICES;
-    for (const auto& [key, group] : groups) {
+    const auto step = [&](const std::pair<Key, Group>& of, const Tensor& ws, int share, void* on) {
+        const auto& [key, group] = of;
         const auto& [rows, cols, p_type, g_type] = key;
         const double scale = match_rms ? 0.2 * std::sqrt((double)std::max(rows, cols))
                                        : std::sqrt(std::max(1.0, (double)rows / (double)cols));
         const int64_t count = (int64_t)group.params.size();
-        const Tensor ws = workspace(params[0], std::min(count, most), rows, cols);
         for (int64_t i = 0; i < count; i += most)
-            check(lib.muon_step((int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
-                                group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
-                                lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum, nesterov,
-                                (float)weight_decay, (float)scale, (int)steps, (float)c[0], (float)c[1], (float)c[2],
-                                (float)eps, ws.data_ptr(), (size_t)ws.numel(), stream()),
+            check(lib.muon_step_on(share, (int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
+                                   group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
+                                   lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum, nesterov,
+                                   (float)weight_decay, (float)scale, (int)steps, (float)c[0], (float)c[1], (float)c[2],
+                                   (float)eps, ws.data_ptr(), (size_t)ws.numel(), on),
                   "cimekv_muon_step");
+    };
+    const auto room = [&](const std::pair<Key, Group>& of) {
+        return workspace(params[0], std::min<int64_t>(of.second.params.size(), most), std::get<0>(of.first),
+                         std::get<1>(of.first));
+    };
+    // small matrices of several shapes run side by side, each on its share of the SMs
+    std::vector<int> counts, rows, cols, shares(groups.size(), 0);
+    if (groups.size() > 1) {
+        for (const auto& [key, group] : groups) {
+            counts.push_back((int)group.params.size());
+            rows.push_back((int)std::get<0>(key));
+            cols.push_back((int)std::get<1>(key));
+        }
+        check(lib.muon_shares((int)groups.size(), counts.data(), rows.data(), cols.data(), (float)c[2], 0, shares.data()),
+              "cimekv_muon_shares");
+    }
+    std::vector<Tensor> rooms;  // of those side by side, until the streams have joined
+    for (size_t k = 0; k < groups.size(); ++k) {
+        if (shares[k]) rooms.push_back(room(groups[k]));
+        else step(groups[k], room(groups[k]), 0, stream());
+    }
+    if (!rooms.empty()) {
+        Beside beside(params[0].device().index());
+        size_t used = 0;
+        for (size_t k = 0; k < groups.size(); ++k) {
+            if (!shares[k]) continue;
+            void* on = used ? (void*)beside.next().stream() : stream();
+            step(groups[k], rooms[used++], shares[k], on);
+        }
+        beside.join();
     }
     // autograd must see that these were written
     for (const auto* list : {&params, &momenta})

@@ -53,8 +53,8 @@ def cuda_muon_step(params: List[torch.Tensor], grads: List[torch.Tensor], moment
     ``"match_rms_adamw"`` (all shapes move by AdamW's typical RMS).
 
     ``lr`` may be a one-element fp32 CUDA tensor, which a captured graph reads at
-    each replay.  Matrices of one shape and type run together; parameters and
-    momenta must not overlap.
+    each replay.  Matrices of one shape and type run together, small ones of several
+    shapes side by side; parameters and momenta must not overlap.
     """
     if adjust_lr not in ("original", "match_rms_adamw"):
         raise ValueError(f"unknown adjust_lr {adjust_lr!r}")

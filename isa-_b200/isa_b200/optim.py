@@ -64,8 +64,11 @@ class Muon(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
+        # groups of one device that differ in `matrices` alone make one call, so that their shapes run side by side
+        calls = {}
         for group in self.param_groups:
-            params, grads, momenta = [], [], []
+            options = {k: group[k] for k in ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps",
+                                             "adjust_lr")}
             k = group["matrices"]
             for p in group["params"]:
                 if p.grad is None:
@@ -78,11 +81,11 @@ class Muon(torch.optim.Optimizer):
                         raise RuntimeError("Muon's first step cannot be captured: take one step before the capture")
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
                 shape = (*p.shape[:-2], k, p.shape[-2] // k, p.shape[-1]) if k > 1 else p.shape
+                key = (p.device, *(id(v) if isinstance(v, torch.Tensor) else repr(v) for v in options.values()))
+                params, grads, momenta, _ = calls.setdefault(key, ([], [], [], options))
                 params.append(p.view(shape))
                 grads.append(p.grad.reshape(shape))
                 momenta.append(state["momentum_buffer"].view(shape))
-            if params:
-                cuda_muon_step(params, grads, momenta, lr=group["lr"], momentum=group["momentum"],
-                               nesterov=group["nesterov"], weight_decay=group["weight_decay"], steps=group["steps"],
-                               coefficients=group["coefficients"], eps=group["eps"], adjust_lr=group["adjust_lr"])
+        for params, grads, momenta, options in calls.values():
+            cuda_muon_step(params, grads, momenta, **options)
         return loss

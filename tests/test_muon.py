@@ -13,6 +13,8 @@ e = 3 * 2^-22 + (34 or 136 + K / 64) u of |L| |R|, whose norm is at most |L|_F |
 and an error before a step is multiplied by at most L = max(|p'(s)|, |p(s) / s|) over the singular values there.
 """
 
+import array
+import ctypes
 import math
 
 import pytest
@@ -387,6 +389,94 @@ def test_muon_many_matrices(dev):
         want, bound, _, _ = _want_step(torch.zeros(24, 24, device=dev), grads[i][k], torch.zeros(24, 24, device=dev), 1.0,
                                        weight_decay=0.0)
         _assert_near(params[i][k], want, bound, f"{i} {k}")
+
+
+def test_muon_shares():
+    """How steps of several shapes share the SMs (no GPU: their number is given)."""
+    from isa_b200 import _lib
+    lib = _lib.load()
+
+    def shares(*groups, sms=148, c=2.0):
+        counts, rows, cols = (array.array("i", v) for v in zip(*groups))
+        out = array.array("i", [-1] * len(groups))
+        at = lambda a: a.buffer_info()[0]  # noqa: E731
+        assert lib.cimekv_muon_shares(len(groups), at(counts), at(rows), at(cols), c, sms, at(out)) == 0
+        return list(out)
+
+    for c in (0.0, 2.0):
+        for groups in ([(40, 192, 192), (10, 192, 768)], [(1, 64, 64), (1, 64, 65), (1, 65, 64)], [(3, 200, 100)] * 4):
+            got = shares(*groups, c=c)
+            assert all(s >= 2 for s in got) and sum(got) <= 148, got
+    big = [(48, 768, 768), (1, 4096, 4096)]
+    assert shares(*big) == [0, 0]  # each fills the chip
+    got = shares(*big, (1, 64, 64), (1, 64, 256))
+    assert got[:2] == [0, 0] and all(s >= 2 for s in got[2:])
+    assert shares((5, 64, 64)) == [0]
+    assert shares((0, 64, 64), (5, 0, 64), (5, 64, 64)) == [0, 0, 0]
+    assert shares((1, 64, 64), (1, 64, 65), sms=3) == [0, 0]
+    many = shares(*[(1, 32, 32 + i) for i in range(40)])
+    assert sum(many) <= 148 and sum(s > 0 for s in many) == 16
+    assert lib.cimekv_muon_shares(1, None, None, None, 2.0, 148, None) == 1
+    one, bad = array.array("i", [1]), array.array("i", [40000])
+    a, b = one.buffer_info()[0], bad.buffer_info()[0]
+    assert lib.cimekv_muon_shares(1, a, b, a, 2.0, 148, a) == 1 and lib.cimekv_muon_shares(1, a, a, a, 2.0, -1, a) == 1
+    assert lib.cimekv_muon_shares(0, None, None, None, 2.0, 148, None) == 0
+    t = (ctypes.c_void_p * 1)(256)
+    for share in (1, -1):
+        assert lib.cimekv_muon_step_on(share, 1, t, t, t, 0, 0, 8, 8, 0.1, None, 0.9, 1, 0.0, 1.0, 5, *NS, 1e-7, 256,
+                                       1 << 40, None) == 1
+        assert b"share" in lib.cimekv_last_error()
+
+
+SEVERAL = [(6, 192, 192), (3, 192, 768), (2, 100, 37), (1, 300, 300), (2, 33, 500)]
+
+
+@gpu
+@pytest.mark.parametrize("c", [NS, CUBIC])
+def test_muon_several_shapes_side_by_side(dev, c):
+    """Small matrices of several shapes, a large one among them, in one call: on another stream and from two graphs too."""
+    _, muon_step = _ops()
+    shapes = SEVERAL + [(1, 1500, 1300)]
+    p0 = [torch.randn(s, device=dev) for s in shapes]
+    m0 = [_update(dev, *s, seed=i) for i, s in enumerate(shapes)]
+    g = [_update(dev, *s, seed=50 + i) for i, s in enumerate(shapes)]
+    g[2] = g[2].transpose(1, 2).contiguous().transpose(1, 2)  # copied first
+
+    def call(p, m):
+        muon_step(p, g, m, lr=0.02, coefficients=c, weight_decay=0.1)
+
+    def fresh():
+        return [t.clone() for t in p0], [t.clone() for t in m0]
+
+    p, m = fresh()
+    call(p, m)
+    if c == NS:
+        for i, s in enumerate(shapes):
+            for k in range(s[0]):
+                want_p, bound_p, want_m, bound_m = _want_step(p0[i][k], g[i][k], m0[i][k], 0.02)
+                _assert_near(p[i][k], want_p, bound_p, f"{s} {k}")
+    side = torch.cuda.Stream()
+    sets = [fresh() for _ in range(6)]
+    torch.cuda.synchronize()
+    for k, (q, n) in enumerate(sets):  # on two streams at the same time; workspaces are freed and taken again
+        with torch.cuda.stream(side if k % 2 else torch.cuda.current_stream()):
+            call(q, n)
+    torch.cuda.synchronize()
+    for q, n in sets:
+        assert all(map(torch.equal, q, p)) and all(map(torch.equal, n, m))
+    graphs = []
+    for q, n in sets[:2]:
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            call(q, n)
+        graphs.append(graph)
+    for round_ in range(2):
+        for (q, n), graph in zip(sets, graphs):
+            for t, u in zip(q + n, p0 + m0):
+                t.copy_(u)
+            graph.replay()
+        for q, n in sets[:2]:
+            assert all(map(torch.equal, q, p)) and all(map(torch.equal, n, m))
 
 
 @gpu
