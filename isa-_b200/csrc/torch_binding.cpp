@@ -311,11 +311,17 @@ public:
         } catch (...) {
         }
     }
+    // (the current stream itself if all of the pool's are taken)
     c10::cuda::CUDAStream next() {
-        const auto s = c10::cuda::getStreamFromPool(false, main_.device_index());
-        begin_.block(s);
-        sides_.push_back(s);
-        return s;
+        for (int i = 0; i < 32; ++i) {
+            const auto s = c10::cuda::getStreamFromPool(false, main_.device_index());
+            const auto theirs = capture_of(s);
+            if (theirs && theirs != capture_of(main_)) continue;  // part of somebody else's capture
+            begin_.block(s);
+            sides_.push_back(s);
+            return s;
+        }
+        return main_;
     }
     void join() {
         while (!sides_.empty()) {
@@ -328,6 +334,14 @@ public:
     }
 
 private:
+    // The capture that a stream is part of; 0: none.
+    static unsigned long long capture_of(const c10::cuda::CUDAStream& s) {
+        cudaStreamCaptureStatus status;
+        unsigned long long id = 0;
+        C10_CUDA_CHECK(cudaStreamGetCaptureInfo(s.stream(), &status, &id));
+        return status == cudaStreamCaptureStatusNone ? 0 : id;
+    }
+
     c10::cuda::CUDAStream main_;
     at::cuda::CUDAEvent begin_;
     std::vector<c10::cuda::CUDAStream> sides_;

@@ -480,6 +480,40 @@ def test_muon_several_shapes_side_by_side(dev, c):
 
 
 @gpu
+def test_muon_several_shapes_during_another_capture(dev):
+    """Calls outside a capture that goes on meanwhile stay out of it, whichever of torch's streams it has taken."""
+    _, muon_step = _ops()
+    shapes = SEVERAL[:2]
+    g = [_update(dev, *s, seed=i) for i, s in enumerate(shapes)]
+
+    def fresh():
+        return [torch.ones(s, device=dev) for s in shapes], [torch.zeros(s, device=dev) for s in shapes]
+
+    want = fresh()
+    muon_step(want[0], g, want[1], lr=0.02)
+    inside, outside = fresh(), [fresh() for _ in range(40)]
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, capture_error_mode="relaxed"):
+        muon_step(inside[0], g, inside[1], lr=0.02)
+        for _ in range(8):  # a stream of ours that the capture has not taken
+            other = torch.cuda.Stream()
+            with torch.cuda.stream(other):
+                if not torch.cuda.is_current_stream_capturing():
+                    break
+        with torch.cuda.stream(other):
+            for p, m in outside:
+                muon_step(p, g, m, lr=0.02)
+    torch.cuda.synchronize()
+    for p, m in outside:
+        assert all(map(torch.equal, p, want[0])) and all(map(torch.equal, m, want[1]))
+    assert not any(m.any() for m in inside[1])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert all(map(torch.equal, inside[0], want[0])) and all(map(torch.equal, inside[1], want[1]))
+
+
+@gpu
 def test_muon_learning_rate_on_the_device_and_graph(dev):
     _, muon_step = _ops()
     p0, g, m0 = torch.randn(96, 80, device=dev), _update(dev, 96, 80), _update(dev, 96, 80, seed=1)
