@@ -733,6 +733,55 @@ struct Pipe {
     bool ok;                // no wait has run out
 };
 
+// Where the CTAs of a matrix meet between the products of ns_steps_kernel: a
+// collecting warp counts itself in when its part of the result is in memory, and
+// only what depends on the others waits: the copy warp, before it asks for their results.
+struct Meet {
+    unsigned* arrivals;     // of the matrix, zeroed by ns_norm_kernel
+    unsigned target;        // CTAs' arrivals until the last product's end; 0: nothing to wait for
+    uint32_t own;           // barrier of a CTA that has a matrix alone; 0: it has not
+    uint32_t counted;       // warps of the CTA that have counted themselves in; the last one counts for all
+    volatile int* lost;     // set when a wait has run out: from then on none is waited for and all results are NaN
+};
+template <int kWarps>
+__device__ __forceinline__ void meet_arrive(const Meet& m) {
+    asm volatile("fence.proxy.async.global;" ::: "memory");  // planes are written and read by copies
+    if (m.own) {
+        asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(m.own) : "memory");
+        return;
+    }
+    unsigned before;
+    asm volatile("atom.acq_rel.cta.shared::cta.add.u32 %0, [%1], 1;" : "=r"(before) : "r"(m.counted) : "memory");
+    if (before % kWarps == kWarps - 1) asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(m.arrivals) : "memory");
+}
+// Called by whole warps.  For two seconds at most.
+__device__ __forceinline__ void meet_wait(const Meet& m) {
+    bool ok = true;
+    if (*m.lost) return;
+    if (m.target && m.own) {
+        ok = mbar_wait(m.own, (m.target - 1) & 1);
+    } else if (m.target) {
+        unsigned long long began = 0;
+        for (;;) {
+            unsigned seen;
+            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(m.arrivals) : "memory");
+            if (seen >= m.target) break;
+            const unsigned long long now = wall_ns();
+            if (!began) began = now;
+            else if (now - began > 2000000000ull) {
+                ok = false;
+                break;
+            }
+        }
+    }
+    if (!ok) {
+        *m.lost = 1;
+        __threadfence_block();
+    }
+    asm volatile("fence.proxy.async.global;" ::: "memory");
+    __syncwarp();
+}
+
 // The tiles first, first + step, ... of one product: of matrix `matrix`, or (-1) of all
 // matrices in turn.  Tiles are 128 x 128 by one CTA,
 // 256 x 256 by a pair of CTAs whose tensor cores work as one (each stages 128
@@ -755,7 +804,7 @@ struct Pipe {
 template <int M, int kSide, bool kFine>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
                                         const CUtensorMap* out, const Product& p, const Result& result, int batch, int first, int step, int tiles,
-                                        int mode = M, int matrix = -1) {
+                                        int mode = M, int matrix = -1, const Meet& meet = Meet()) {
     using T = Tile<kSide, kFine>;
     constexpr bool kPair = T::kPair;
     constexpr int kRanks = T::kRanks, kRows = T::kRows, kOperand = T::kOperand, kStageBytes = T::kStageBytes;
@@ -790,6 +839,26 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
 
     if (warp == kWarps) {
         const uint32_t count_at = kPair ? cluster_addr(q.full, 0) : q.full;
+        int ahead = 0;  // stages of the first tile that have their right operand on the way
+        if constexpr (M == kAny) {
+            if (!square && first < tiles) {  // X stands since the step before: it need not wait for the others
+                int b, row0, col0;
+                place(first, b, row0, col0);
+                Turn fill = q.fill;
+                for (; ahead < ksteps && ahead < kStages; ++ahead, fill.next(kStages)) {
+                    if (!(q.ok = q.ok && mbar_wait(q.empty + 8 * fill.at, fill.parity ^ 1))) break;
+                    if (elect_one()) {
+                        mbar_expect(q.full + 8 * fill.at, kStageBytes);
+#pragma unroll
+                        for (int plane = 0; plane < 2; ++plane)
+                            tma_box<kPair>(q.stages + fill.at * kStageBytes + (2 + plane) * kOperand, right, col0, ahead * kK,
+                                           plane * batch + b, q.full + 8 * fill.at);
+                    }
+                    __syncwarp();
+                }
+            }
+            meet_wait(meet);
+        }
         for (int t = first; t < tiles && q.ok; t += step) {
             int b, row0, col0;
             place(t, b, row0, col0);
@@ -799,16 +868,17 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             for (int k = 0; k < ksteps; ++k, q.fill.next(kStages)) {
                 const int s = q.fill.at;
                 // (the phase before a barrier's first has ended by definition)
-                if (!(q.ok = mbar_wait(q.empty + 8 * s, q.fill.parity ^ 1))) break;
+                const bool asked = M == kAny && t == first && k < ahead;
+                if (!asked && !(q.ok = mbar_wait(q.empty + 8 * s, q.fill.parity ^ 1))) break;
                 const uint32_t base = q.stages + s * kStageBytes, bar = count_at + 8 * s;
                 if (elect_one()) {
-                    if (q.rank == 0) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
+                    if (q.rank == 0 && !asked) mbar_expect(q.full + 8 * s, kRanks * (same ? kStageBytes / 2 : kStageBytes));
 #pragma unroll
                     for (int plane = 0; plane < 2; ++plane) {
                         const int z = plane * batch + b;
                         const uint32_t l = base + plane * kOperand, r = base + (2 + plane) * kOperand;
                         tma_box<kPair>(l, left, k * kK, row0, z, bar);
-                        if (same) continue;
+                        if (same || asked) continue;
                         if (square) {
                             tma_box<kPair>(r, right, k * kK, col0, z, bar);
                         } else {
@@ -899,7 +969,9 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                 __syncwarp();
                 if (lane == 0) mbar_arrive_cluster(empty_at + 8 * buf);
             }
-            if (!q.ok) {  // a lost copy or product shows as NaN, it never passes for a result
+            bool good = q.ok;
+            if constexpr (M == kAny) good = __all_sync(0xffffffffu, good && !*meet.lost);
+            if (!good) {  // a lost copy, product or meeting shows as NaN, it never passes for a result
 #pragma unroll
                 for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
@@ -916,6 +988,11 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             __syncwarp();
         }
         if (mode != kResult && lane == 0) tma_store_wait<true>();
+        if (M == kAny && mode != kResult) {
+            // without a tile nothing has held this warp back: its next arrival must not stand for another's last one
+            if (first >= tiles) meet_wait(meet);
+            if (lane == 0) meet_arrive<kWarps>(meet);
+        }
         __syncwarp();
     }
 }
@@ -1018,31 +1095,6 @@ struct StepMaps {
     CUtensorMap x_out[2], b_out, p_out;     // to write to, boxes of a warp's rows
 };
 
-// All CTAs of a matrix have finished a product: planes are written by ordinary
-// stores and read by copies of the other CTAs.  For two seconds at most.
-__device__ __forceinline__ void group_meet(unsigned* arrivals, unsigned target, unsigned group, Pipe& q, int* lost) {
-    asm volatile("fence.proxy.async.global;" ::: "memory");
-    __syncthreads();
-    if (group > 1 && threadIdx.x == 0) {
-        asm volatile("red.release.gpu.global.add.u32 [%0], 1;" ::"l"(arrivals) : "memory");
-        unsigned long long began = 0;
-        for (;;) {
-            unsigned seen;
-            asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(arrivals) : "memory");
-            if (seen >= target) break;
-            const unsigned long long now = wall_ns();
-            if (!began) began = now;
-            else if (now - began > 2000000000ull) {
-                *lost = 1;
-                break;
-            }
-        }
-    }
-    __syncthreads();
-    if (*lost) q.ok = false;
-    asm volatile("fence.proxy.async.global;" ::: "memory");
-}
-
 // All steps of matrices whose tiles fit the SMs, a group of CTAs to a matrix that meet
 // after each product.  Bound by latency: a product of one 192 x 192 matrix is 65 us / 15 =
 // 4.4 us, of which the meeting is 1 us, the first copy 0.4, a stage 0.45 each (three), the
@@ -1053,15 +1105,25 @@ __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(
                                                                          const __grid_constant__ Result result, int batch) {
     extern __shared__ uint8_t smem_raw[];
     __shared__ __align__(8) uint64_t bars[2 * kMaxStages + 2 * kMaxBufs + 1];
-    __shared__ uint32_t tmem_slot;
+    __shared__ __align__(8) uint64_t own;
     __shared__ int lost;
-    if (threadIdx.x == 0) lost = 0;
+    __shared__ unsigned counted;
+    __shared__ uint32_t tmem_slot;
+    constexpr int kWarps = Tile<64, kFine>::kWarps;
+    if (threadIdx.x == 0) {  // made known by pipe_open
+        mbar_init(smem_addr(&own), kWarps);
+        lost = 0;
+        counted = 0;
+    }
     Pipe q;
     pipe_open<Tile<64, kFine>>(q, bars, &tmem_slot, smem_raw);
     const int ni = (st.product[0].rows + 63) / 64, nj = (st.product[2].cols + 63) / 64;
     const int rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
+    Meet meet = {nullptr, 0, st.group > 1 ? 0 : smem_addr(&own), smem_addr(&counted), &lost};
+    unsigned met = 0;  // phases of `own` that earlier matrices have ended
     for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
-        unsigned target = 0;
+        meet.arrivals = st.arrivals + matrix;
+        unsigned count = 0;
         for (int k = 0; k < st.steps; ++k) {
             // All tiles of the square products: storing mirror images takes a CTA longer than a tile that
             // another one has time for.
@@ -1071,10 +1133,13 @@ __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(
                 const CUtensorMap* const x = &maps.x[k & 1];
                 product<kAny, 64, kFine>(q, i == 0 ? x : i == 1 ? &maps.b : &maps.p, i == 1 ? &maps.b : x,
                                   i == 0 && st.squared ? &maps.b_out : i < 2 ? &maps.p_out : &maps.x_out[(k + 1) & 1],
-                                  st.product[i], result, batch, rank, st.group, tiles, mode, matrix);
-                if (mode != kResult) group_meet(st.arrivals + matrix, target += st.group, st.group, q, &lost);
+                                  st.product[i], result, batch, rank, st.group, tiles, mode, matrix, meet);
+                if (mode != kResult) count += st.group;
+                meet.target = count ? (meet.own ? met : 0) + count : 0;
             }
         }
+        meet.target = 0;  // the next matrix begins with what ns_prepare_kernel left
+        met += count;
     }
     pipe_close<Tile<64, kFine>>(q);
 }
