@@ -1096,9 +1096,9 @@ struct StepMaps {
 };
 
 // All steps of matrices whose tiles fit the SMs, a group of CTAs to a matrix that meet
-// after each product.  Bound by latency: a product of one 192 x 192 matrix is 65 us / 15 =
-// 4.4 us, of which the meeting is 1 us, the first copy 0.4, a stage 0.45 each (three), the
-// way out 0.75; 40 of 192 x 192 take 116 us, 10 of 192 x 768 take 103, 2 of 257 x 1001 116.
+// after each product.  Bound by latency: a product of one 192 x 192 matrix is 63 us / 15 =
+// 4.2 us, of which the meeting is about 1 us, the first copy 0.4, a stage 0.45 each (three),
+// the way out 0.75; 40 of 192 x 192 take 115 us, 10 of 192 x 768 take 102, 2 of 257 x 1001 112.
 template <bool kFine>
 __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
                                                                          const __grid_constant__ Steps st,
