@@ -1335,8 +1335,8 @@ int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& o
                 : launch_as<M, 128, false>(l, r, out, p, result, batch, sms, s);
 }
 
-// CTAs per matrix when all steps run in one kernel, 0 where a kernel for each
-// product costs less.  Measured a call, one kernel against fifteen: 73 against 112 us
+// What a step takes when all steps run in one kernel and when each product is a kernel;
+// the cheaper way is taken.  Measured a call, one kernel against fifteen: 73 against 112 us
 // for one 192 x 192 matrix, 131 against 202 for 768 x 768, 120 against 135 for 40 of
 // 192 x 192; 252 against 239 for 1024 x 1024, 176 against 159 for 12 of 384 x 384.
 struct StepCost {
