@@ -12,8 +12,10 @@
 //   B = X X^T + (b / 2c) I,   P = c B B + (a - b^2 / 4c) I,   X <- P X
 //
 // all three are one product each with an epilogue alpha D + beta I, so none of
-// them reads anything but its operands.  (c = 0: P = b X X^T + a I is the first
-// product's, and the second falls away.)
+// them reads anything but its operands.  For fp32 results P is formed as it stands,
+// b A read by the second product's epilogue: the square's completion rounds A at the
+// size of b / 2c (42 x 47: 1.6e-6 off, where products in fp32 are by 0.95e-6, and 0.97e-6
+// as it stands; 192 x 192: 2.0e-6 and 1.3e-6, for 2 us of 74).  (c = 0: P = b X X^T + a I is the first product's, and the second falls away.)
 //
 // Precision.  A singular value far below the largest grows by up to a per step
 // (x 485 in five steps), and so does any rounding noise in its direction: with
@@ -23,8 +25,8 @@
 // checked on the host from the coefficients, so the fixed scale neither overflows
 // nor loses small elements), and a
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
-// tensor core products.  fp32 results are off by 0.6 to 1.9 times what products in
-// fp32 give (16 x 16 to 4096 x 4096).
+// tensor core products.  fp32 results are off by 0.4 to 1.2 times what products in
+// fp32 give (4096 x 4096 to 16 x 16).
 //
 // B and P are symmetric: only tiles on and below the diagonal are computed, the
 // epilogue stores each tile and its mirror image.
@@ -539,6 +541,10 @@ enum Mode { kSymmetric = 0, kFull = 1, kApply = 2, kResult = 3, kAny = 4 };
 struct Product {
     int rows, cols, depth;
     float alpha, beta;      // on values as the planes hold them
+    const __half* add;      // planes of which gamma times the value is added to the sum, or null (fine sums only)
+    long long add_plane;
+    int add_pitch;
+    float gamma;
 };
 
 // Where the last product goes.
@@ -649,6 +655,37 @@ __device__ __forceinline__ void finish_result(const Result& p, int rows, int col
                     store_float(dst, type, at + k,
                                 result_of(p, x[k], p.update ? load_as_float(dst, type, at + k) : 0.0f, lr));
         }
+    }
+}
+
+// 32 columns from cb of a lane's row of the planes that a product adds to.
+struct Addend {
+    uint4 plane[2][4];
+};
+template <int kRows>
+__device__ __forceinline__ void load_addend(const Product& p, int b, int row0, int cb, Addend& more) {
+    const int lane = threadIdx.x & 31, r = row0 + lane;
+    if (lane >= kRows || r >= p.rows) return;
+    const __half* at = p.add + ((long long)b * p.rows + r) * p.add_pitch + cb;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+        if (cb + 8 * q >= p.cols) break;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)  // written by other SMs while this kernel runs: not from L1
+            more.plane[i][q] = __ldcg(reinterpret_cast<const uint4*>(at + i * p.add_plane + 8 * q));
+    }
+}
+
+__device__ __forceinline__ void add_addend(float gamma, const Addend& more, float (&v0)[16], float (&v1)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const auto word = [&](const uint4& u) { return i % 4 == 0 ? u.x : i % 4 == 1 ? u.y : i % 4 == 2 ? u.z : u.w; };
+        const uint32_t wh = word(more.plane[0][i / 4]), wl = word(more.plane[1][i / 4]);
+        const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&wh));
+        const float2 l = __half22float2(*reinterpret_cast<const __half2*>(&wl));
+        float* v = i < 8 ? &v0[2 * i] : &v1[2 * i - 16];
+        v[0] = fmaf(gamma, h.x + l.x, v[0]);
+        v[1] = fmaf(gamma, h.y + l.y, v[1]);
     }
 }
 
@@ -798,9 +835,9 @@ __device__ __forceinline__ void meet_wait(const Meet& m) {
 // have one sign.  So a few steps (the small cross products before those at full size) go
 // into a fresh accumulator, one of several, and the collecting warps add them in
 // registers with round-to-nearest while the next ones run.  Fine sums: 192 x 192 is off
-// by 2.0e-6 where fp32 products are by 1.6e-6 (fast: 2.8e-6), 48 of 768 x 768 by 2.3e-6
-// (fp32 products 2.5e-6, fast 4.6e-6), in 1,442 us (fast 1,385), 40 of 192 x 192 in 137
-// (fast 123).  The same accumulators let the next tile start while the last one is stored.
+// by 2.0e-6 where fp32 products are by 1.6e-6 (fast: 2.8e-6; both with the square
+// completed), 48 of 768 x 768 by 2.3e-6 (fp32 products 2.5e-6, fast 4.6e-6), in 1,442 us
+// (fast 1,385), 40 of 192 x 192 in 137 (fast 123).  The same accumulators let the next tile start while the last one is stored.
 template <int M, int kSide, bool kFine>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
                                         const CUtensorMap* out, const Product& p, const Result& result, int batch, int first, int step, int tiles,
@@ -951,9 +988,14 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
             for (int g = 0; g < kWarpCols / 16; ++g)
 #pragma unroll
                 for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
+            // a 64 x 64 tile's addend is asked for once its first sums are there (A stands by then) and
+            // comes while the next ones run
+            constexpr bool kAdd = kFine && (M == kSymmetric || M == kAny), kEarly = kAdd && kSide == 64;
+            Addend more = {};
             for (int k = 0; k < ksteps * (kK / 16); k += T::kSums, q.chunk.next(kBufs)) {
                 const int buf = q.chunk.at;
                 q.ok = q.ok && mbar_wait(q.acc_full + 8 * buf, q.chunk.parity);
+                if (kEarly && k == 0 && p.add) load_addend<T::kWarpRows>(p, b, r0, col0, more);
                 q.ok = __all_sync(0xffffffffu, q.ok);
                 if (!q.ok) continue;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -982,8 +1024,14 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                 if (col0 + g * 16 >= p.cols) break;
                 if (mode == kResult)
                     finish_result<T::kWarpRows>(result, p.rows, p.cols, acc[g], b, r0, col0 + g * 16, lr, staging);
-                else if (g % 2 == 0)
-                    finish_planes<M == kSymmetric, T::kWarpRows>(p, out, acc[g], acc[g + 1], batch, b, r0, col0 + g * 16, diagonal, staging);
+                else if (g % 2 == 0) {
+                    if (kAdd && p.add) {
+                        if (!kEarly) load_addend<T::kWarpRows>(p, b, r0, col0 + g * 16, more);
+                        add_addend(p.gamma, more, acc[g], acc[g + 1]);
+                    }
+                    finish_planes<M == kSymmetric, T::kWarpRows>(p, out, acc[g], acc[g + 1], batch, b, r0, col0 + g * 16,
+                                                                 diagonal, staging);
+                }
             }
             __syncwarp();
         }
@@ -1425,11 +1473,17 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     gram.rows = gram.cols = lay.m;
     gram.depth = lay.n;
     gram.alpha = (squared ? 1.0f : b) / kScale;
-    gram.beta = (squared ? (float)(0.5 * b / c) : a) * kScale;
+    gram.beta = (squared ? fine ? 0.0f : (float)(0.5 * b / c) : a) * kScale;
     if (squared) {
         square.rows = square.cols = square.depth = lay.m;
         square.alpha = c / kScale;
-        square.beta = (float)(a - 0.25 * (double)b * b / c) * kScale;
+        square.beta = (fine ? a : (float)(a - 0.25 * (double)b * b / c)) * kScale;
+    }
+    if (squared && fine) {
+        square.add = am;
+        square.add_plane = lay.a_plane;
+        square.add_pitch = lay.ap;
+        square.gamma = b / square.alpha;
     }
     apply.rows = apply.depth = lay.m;
     apply.cols = lay.n;

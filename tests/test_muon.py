@@ -10,6 +10,11 @@ e = 3 * 2^-22 + (34 or 136 + K / 64) u of |L| |R|, whose norm is at most |L|_F |
     dA = e |X|_F^2 + 2^-22 |B|_F,  dP = |c| (2 |B|_2 dA + e |B|_F^2) + 2^-22 |P|_F  (c = 0: dP = |b| dA + 2^-22 |P|_F),
     d  = dP |X|_2 + e |P|_F |X|_F + 2^-22 |X'|_F
 
+fp32 results form P as it stands: S = A in place of B where it is stored and multiplied (not in |B|_2, the derivative of P
+by A is c (B dA + dA B) either way), and four roundings of its sum, 4 u (|c| |A|_F^2 + |b| |A|_F).  For others S = B:
+
+    dA = e |X|_F^2 + 2^-22 |S|_F,  dP = |c| (2 |B|_2 dA + e |S|_F^2) + 2^-22 |P|_F
+
 and an error before a step is multiplied by at most L = max(|p'(s)|, |p(s) / s|) over the singular values there.
 """
 
@@ -34,7 +39,8 @@ def _ops():
 def _exact(g, steps=5, coefficients=NS, eps=1e-7, fine=None):
     """(result, bound on the Frobenius norm of the error) of one matrix, in 64 bits."""
     a, b, c = coefficients
-    cut = 34 if (g.dtype == F32 if fine is None else fine) else 136
+    fine = g.dtype == F32 if fine is None else fine
+    cut = 34 if fine else 136
     x = g.double()
     tall = x.shape[0] > x.shape[1]
     x = x.T if tall else x
@@ -51,8 +57,11 @@ def _exact(g, steps=5, coefficients=NS, eps=1e-7, fine=None):
         e = lambda k: 3 * 2.0 ** -22 + (cut + k / 64) * U  # noqa: E731
         B = A + (0.5 * b / c if c else 0.0) * eye
         fro, two = (lambda t: float(t.norm())), (lambda t: float(torch.linalg.matrix_norm(t, 2)))  # noqa: E731
-        dA = e(n) * fro(x) ** 2 + 2.0 ** -22 * fro(B)
-        dP = (abs(c) * (2 * two(B) * dA + e(m) * fro(B) ** 2) if c else abs(b) * dA) + 2.0 ** -22 * fro(P)
+        S = A if fine else B
+        dA = e(n) * fro(x) ** 2 + 2.0 ** -22 * fro(S)
+        dP = (abs(c) * (2 * two(B) * dA + e(m) * fro(S) ** 2) if c else abs(b) * dA) + 2.0 ** -22 * fro(P)
+        if fine and c:
+            dP += 4 * U * (abs(c) * fro(A) ** 2 + abs(b) * fro(A))
         err = lip * err + dP * two(x) + e(m) * fro(P) * fro(x) + 2.0 ** -22 * fro(new)
         x = new
     return (x.T if tall else x), err
