@@ -12,10 +12,10 @@
 //   B = X X^T + (b / 2c) I,   P = c B B + (a - b^2 / 4c) I,   X <- P X
 //
 // all three are one product each with an epilogue alpha D + beta I, so none of
-// them reads anything but its operands.  For fp32 results P is formed as it stands,
-// b A read by the second product's epilogue: the square's completion rounds A at the
-// size of b / 2c (42 x 47: 1.6e-6 off, where products in fp32 are by 0.95e-6, and 0.97e-6
-// as it stands; 192 x 192: 2.0e-6 and 1.3e-6, for 2 us of 74).  (c = 0: P = b X X^T + a I is the first product's, and the second falls away.)
+// them reads anything but its operands.  For fp32 results of small matrices P is formed as it
+// stands, b A read by the second product's epilogue: the square's completion rounds A at
+// the size of b / 2c (42 x 47: 1.6e-6 off, where products in fp32 are by 0.95e-6, and
+// 0.97e-6 as it stands).  (c = 0: P = b X X^T + a I is the first product's, and the second falls away.)
 //
 // Precision.  A singular value far below the largest grows by up to a per step
 // (x 485 in five steps), and so does any rounding noise in its direction: with
@@ -25,8 +25,8 @@
 // checked on the host from the coefficients, so the fixed scale neither overflows
 // nor loses small elements), and a
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
-// tensor core products.  fp32 results are off by 0.4 to 1.2 times what products in
-// fp32 give (4096 x 4096 to 16 x 16).
+// tensor core products.  fp32 results are off by 0.6 to 1.3 times what products in
+// fp32 give (4096 x 4096 to 192 x 192).
 //
 // B and P are symmetric: only tiles on and below the diagonal are computed, the
 // epilogue stores each tile and its mirror image.
@@ -541,7 +541,8 @@ enum Mode { kSymmetric = 0, kFull = 1, kApply = 2, kResult = 3, kAny = 4 };
 struct Product {
     int rows, cols, depth;
     float alpha, beta;      // on values as the planes hold them
-    const __half* add;      // planes of which gamma times the value is added to the sum, or null (fine sums only)
+    const __half* add;      // planes of which gamma times the value is added to the sum, or null (fine sums of
+                            // ns_steps_kernel and 128 x 128 tiles only)
     long long add_plane;
     int add_pitch;
     float gamma;
@@ -990,7 +991,7 @@ __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const 
                 for (int i = 0; i < 16; ++i) acc[g][i] = 0.0f;
             // a 64 x 64 tile's addend is asked for once its first sums are there (A stands by then) and
             // comes while the next ones run
-            constexpr bool kAdd = kFine && (M == kSymmetric || M == kAny), kEarly = kAdd && kSide == 64;
+            constexpr bool kAdd = kFine && (M == kAny || (M == kSymmetric && kSide == 128)), kEarly = kAdd && kSide == 64;
             Addend more = {};
             for (int k = 0; k < ksteps * (kK / 16); k += T::kSums, q.chunk.next(kBufs)) {
                 const int buf = q.chunk.at;
@@ -1375,7 +1376,7 @@ double cost_of(int side, int mode, int rows, int cols, int depth, int batch, int
 template <int M>
 int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& out, const Product& p, const Result& result,
                 int batch, int sms, bool fine, cudaStream_t s) {
-    const bool pair = cost_of(256, M, p.rows, p.cols, p.depth, batch, sms) < cost_of(128, M, p.rows, p.cols, p.depth, batch, sms);
+    const bool pair = !p.add && cost_of(256, M, p.rows, p.cols, p.depth, batch, sms) < cost_of(128, M, p.rows, p.cols, p.depth, batch, sms);
     if (fine)
         return pair ? launch_as<M, 256, true>(l, r, out, p, result, batch, sms, s)
                     : launch_as<M, 128, true>(l, r, out, p, result, batch, sms, s);
@@ -1466,6 +1467,11 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     // Sums as fine as an fp32 result shows.  A 16-bit result's own rounding, or that of
     // an fp32 parameter that moves by a small part of its size, hides the difference.
     const bool fine = result.dst.type == CIMEKV_F32 && !result.update;
+    // Short sums leave products in fp32 so exact that the completed square's rounding shows:
+    // 64 x 128 is off by 1.72e-6 with it, 1.05e-6 without, fp32 products by 1.05e-6; from
+    // 192 rows on it costs more than it gives (192 x 192: 2.0e-6, 1.3e-6 and 1.65e-6, in 67
+    // and 74 us; 48 of 768 x 768: 2.3e-6, 1.5e-6 and 2.45e-6, in 1,442 and 1,643 us).
+    const bool plain = fine && squared && lay.m <= 160;
     Steps st = {};
     Product &gram = st.product[0], &square = st.product[1], &apply = st.product[2];
     st.steps = steps;
@@ -1473,13 +1479,13 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     gram.rows = gram.cols = lay.m;
     gram.depth = lay.n;
     gram.alpha = (squared ? 1.0f : b) / kScale;
-    gram.beta = (squared ? fine ? 0.0f : (float)(0.5 * b / c) : a) * kScale;
+    gram.beta = (squared ? plain ? 0.0f : (float)(0.5 * b / c) : a) * kScale;
     if (squared) {
         square.rows = square.cols = square.depth = lay.m;
         square.alpha = c / kScale;
-        square.beta = (fine ? a : (float)(a - 0.25 * (double)b * b / c)) * kScale;
+        square.beta = (plain ? a : (float)(a - 0.25 * (double)b * b / c)) * kScale;
     }
-    if (squared && fine) {
+    if (plain) {
         square.add = am;
         square.add_plane = lay.a_plane;
         square.add_pitch = lay.ap;

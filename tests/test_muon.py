@@ -10,7 +10,7 @@ e = 3 * 2^-22 + (34 or 136 + K / 64) u of |L| |R|, whose norm is at most |L|_F |
     dA = e |X|_F^2 + 2^-22 |B|_F,  dP = |c| (2 |B|_2 dA + e |B|_F^2) + 2^-22 |P|_F  (c = 0: dP = |b| dA + 2^-22 |P|_F),
     d  = dP |X|_2 + e |P|_F |X|_F + 2^-22 |X'|_F
 
-fp32 results form P as it stands: S = A in place of B where it is stored and multiplied (not in |B|_2, the derivative of P
+fp32 results of at most 160 rows form P as it stands: S = A in place of B where it is stored and multiplied (not in |B|_2, the derivative of P
 by A is c (B dA + dA B) either way), and four roundings of its sum, 4 u (|c| |A|_F^2 + |b| |A|_F).  For others S = B:
 
     dA = e |X|_F^2 + 2^-22 |S|_F,  dP = |c| (2 |B|_2 dA + e |S|_F^2) + 2^-22 |P|_F
@@ -57,10 +57,10 @@ def _exact(g, steps=5, coefficients=NS, eps=1e-7, fine=None):
         e = lambda k: 3 * 2.0 ** -22 + (cut + k / 64) * U  # noqa: E731
         B = A + (0.5 * b / c if c else 0.0) * eye
         fro, two = (lambda t: float(t.norm())), (lambda t: float(torch.linalg.matrix_norm(t, 2)))  # noqa: E731
-        S = A if fine else B
+        S = A if fine and m <= 160 else B
         dA = e(n) * fro(x) ** 2 + 2.0 ** -22 * fro(S)
         dP = (abs(c) * (2 * two(B) * dA + e(m) * fro(S) ** 2) if c else abs(b) * dA) + 2.0 ** -22 * fro(P)
-        if fine and c:
+        if fine and m <= 160 and c:
             dP += 4 * U * (abs(c) * fro(A) ** 2 + abs(b) * fro(A))
         err = lip * err + dP * two(x) + e(m) * fro(P) * fro(x) + 2.0 ** -22 * fro(new)
         x = new
@@ -173,6 +173,20 @@ def test_orthogonalize_shapes(dev, shape, dtype):
     got = orthogonalize(g)
     assert got.shape == g.shape and got.dtype == dtype
     _assert_near(got, *_exact(g), f"{shape} {dtype}")
+
+
+@gpu
+@pytest.mark.parametrize("shape", [(64, 130, 600), (64, 600, 130), (150, 150, 150), (100, 160, 161), (100, 161, 161), (3, 160, 160)])
+@pytest.mark.parametrize("c", [NS, CUBIC])
+def test_both_forms_of_the_polynomial(dev, shape, c):
+    """fp32 results on both sides of 160 rows, from the kernels of single products and from the one of all steps."""
+    orthogonalize, _ = _ops()
+    g = _update(dev, *shape, seed=3)
+    got = orthogonalize(g, coefficients=c)
+    assert torch.equal(orthogonalize(g, coefficients=c), got)
+    for k in (0, shape[0] // 2, shape[0] - 1):
+        _assert_near(got[k], *_exact(g[k], coefficients=c), f"{shape} {k}")
+    assert torch.isfinite(got).all()
 
 
 @gpu
