@@ -15,7 +15,6 @@ from pathlib import Path
 import torch
 
 own = False
-_PACKAGE = str(Path(__file__).resolve().parent.parent / "isa-_b200")
 
 _DTYPES = {"fp32": torch.float32, "bf16": torch.bfloat16, "fp16": torch.float16}
 _EPS = 1e-5
@@ -232,6 +231,12 @@ def _by_shape(s):
     return groups.values()
 
 
+def _package():
+    root = str(Path(__file__).resolve().parent.parent / "isa-_b200")
+    if root not in sys.path:
+        sys.path.insert(0, root)
+
+
 def run(state):
     op = state["op"]
     if own:
@@ -248,8 +253,7 @@ def run(state):
 
 
 def _run_own(s):
-    if _PACKAGE not in sys.path:
-        sys.path.insert(0, _PACKAGE)
+    _package()
     if s["op"] == "norm":
         from isa_b200.kernels.transformer_norm import cuda_layer_norm
 
