@@ -704,10 +704,11 @@ constexpr Shape kShapes[] = {{4, 1, 1}, {4, 2, 1}, {4, 3, 1}, {4, 4, 1}, {4, 3, 
                              {1, 8, 1}, {1, 8, 4}, {1, 16, 8}, {1, 32, 16}};
 constexpr int kNumShapes = sizeof(kShapes) / sizeof(kShapes[0]);
 
-int pick_shape(int cols, int v) {
+// inside: rows begin inside a vector, by their strides whatever their width: room for one
+// vector more.
+int pick_shape(int cols, int v, bool inside) {
     for (int i = 0; i < kNumShapes; ++i)
-        // rows that begin inside a vector need room for one more
-        if (kShapes[i].v == v && kShapes[i].capacity() >= cols + (cols % v ? v - 1 : 0)) return i;
+        if (kShapes[i].v == v && kShapes[i].capacity() >= cols + (inside || cols % v ? v - 1 : 0)) return i;
     return -1;
 }
 
@@ -779,12 +780,19 @@ bool vectors_fit(int v, std::initializer_list<Tensor> ts, int* places) {
 // The layout for a call's tensors.  16-bit rows take vectors of eight, or of four
 // where those leave fewer threads idle (384 columns: 384 places against 512).
 int layout_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* places) {
-    const int four = pick_shape(cols, 4), eight = x_type == CIMEKV_F32 ? -1 : pick_shape(cols, 8);
-    if (eight >= 0 && (four < 0 || kShapes[eight].capacity() <= kShapes[four].capacity()) && vectors_fit(8, ts, places))
-        return eight;
-    if (four >= 0 && vectors_fit(4, ts, places)) return four;
+    const bool fours = vectors_fit(4, ts, places);
+    const int four = fours ? pick_shape(cols, 4, *places != 0) : -1;
+    int places8;
+    if (x_type != CIMEKV_F32 && vectors_fit(8, ts, &places8)) {
+        const int eight = pick_shape(cols, 8, places8 != 0);
+        if (eight >= 0 && (four < 0 || kShapes[eight].capacity() <= kShapes[four].capacity())) {
+            *places = places8;
+            return eight;
+        }
+    }
+    if (four >= 0) return four;
     *places = 0;
-    return pick_shape(cols, 1);
+    return pick_shape(cols, 1, false);
 }
 
 // Lets kernel number `id` use as much shared memory as its layout may ask for, once
@@ -876,9 +884,11 @@ extern "C" size_t cimekv_layer_norm_workspace_bytes(long long rows, int cols) {
     if (sm_count(&sms)) return 0;
     long long most = 0;
     for (const int v : {1, 4, 8}) {
-        const int i = pick_shape(cols, v);
-        const long long g = i < 0 ? 0 : grid_size(rows, kShapes[i], sms, false);
-        if (g > most) most = g;
+        for (const bool inside : {false, true}) {
+            const int i = pick_shape(cols, v, inside);
+            const long long g = i < 0 ? 0 : grid_size(rows, kShapes[i], sms, false);
+            if (g > most) most = g;
+        }
     }
     return (size_t)most * 2 * (size_t)cols * sizeof(float);
 }

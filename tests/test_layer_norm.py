@@ -493,3 +493,28 @@ def test_double_backward_refused(dev):
     g, = torch.autograd.grad(layer_norm(x).sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):
         g.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("add", [False, True])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(1001, 384), (333, 768), (1, 384), (700, 4096), (40, 16384), (500, 257)])
+def test_weight_gradients_alone_of_strided_rows(dev, rows, cols, dtype, add):
+    """Rows one to seven elements further apart than they are wide, in the input and in the gradient that arrives, and
+    no gradient of the input: nothing of the call begins every row at the same place of a vector."""
+    layer_norm, add_layer_norm = _ops()
+    gen = torch.Generator(device=dev).manual_seed(rows + cols)
+    for apart in (1, 2, 4, 7):
+        wide = lambda: torch.randn(rows, cols + apart, device=dev, generator=gen).to(dtype)[:, :cols]  # noqa: E731
+        x, d, dy, dh = wide(), wide(), wide(), wide()
+        w = (1 + 0.3 * torch.randn(cols, device=dev, generator=gen)).to(dtype).requires_grad_(True)
+        b = torch.zeros(cols, device=dev, dtype=dtype, requires_grad=True)
+        want = _plain(x, d if add else None, w.detach(), b.detach(), 1e-5, dy, dh if add else None)
+        if add:
+            gw, gb = torch.autograd.grad(add_layer_norm(x, d, w, b), (w, b), (dy, dh))
+        else:
+            gw, gb = torch.autograd.grad(layer_norm(x, w, b), (w, b), dy)
+        _assert_near(gw, *want["dw"], f"dw, {apart} apart")
+        _assert_near(gb, *want["db"], f"db, {apart} apart")
+        gw, = torch.autograd.grad(layer_norm(x, w), w, dy)
+        _assert_near(gw, *_plain(x, None, w.detach(), None, 1e-5, dy, None)["dw"], f"dw alone, {apart} apart")
