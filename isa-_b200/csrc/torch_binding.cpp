@@ -6,6 +6,8 @@
 // this module works with whichever build of the library is loaded.
 
 #include <ATen/cuda/CUDAEvent.h>
+#include <c10/core/AutogradState.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAGraphsC10Utils.h>
@@ -13,6 +15,7 @@
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/graph_task.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/extension.h>
 
 #include <algorithm>
@@ -59,6 +62,23 @@ void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (stat
 bool available(at::ScalarType t) { return t == at::kFloat || t == at::kBFloat16 || t == at::kHalf; }
 int code(at::ScalarType t) { return t == at::kFloat ? CIMEKV_F32 : t == at::kBFloat16 ? CIMEKV_BF16 : CIMEKV_F16; }
 void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
+// The kernels get addresses, so whatever follows a call by its tensors alone sees only the outputs'
+// allocation.  A trace would hand out memory that nothing writes.
+void check_not_traced(const char* what) {
+    TORCH_CHECK(!torch::jit::tracer::isTracing() &&
+                    !c10::impl::TorchDispatchModeTLS::get_mode(c10::impl::TorchDispatchModeKey::PROXY),
+                what, " cannot be traced: a trace would miss its kernels");
+}
+// A forward-mode tangent would be lost, and read as zero; a subclass that carries its values itself has no
+// memory of its own to hand over.
+void check_plain(const Tensor& t, const char* name, const char* what) {
+    TORCH_CHECK(!t._fw_grad(0).defined() || !c10::AutogradState::get_tls_state().get_fw_grad_mode(), name,
+                " has a forward-mode tangent: ", what, " has no forward-mode derivative");
+    TORCH_CHECK(!t.unsafeGetTensorImpl()->is_python_dispatch(), name, " is a tensor subclass with its own dispatch: ", what,
+                " takes plain tensors");
+}
+
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 // ------------------------------------------------------------- layer norm ---
@@ -77,6 +97,11 @@ Rows rows_of(const Tensor& t, int64_t cols) {
 
 void check_norm(const Tensor& x, const OptTensor& delta, const OptTensor& weight, const OptTensor& bias, double eps,
                 at::ScalarType out) {
+    check_not_traced("layer norm");
+    check_plain(x, "x", "layer norm");
+    if (delta) check_plain(*delta, "delta", "layer norm");
+    if (weight) check_plain(*weight, "weight", "layer norm");
+    if (bias) check_plain(*bias, "bias", "layer norm");
     TORCH_CHECK(x.is_cuda(), "x must be a CUDA tensor: the layer norm kernels have no CPU implementation");
     TORCH_CHECK(x.dim() >= 1, "x must have at least one axis");
     TORCH_CHECK(available(x.scalar_type()), "x must be float32, bfloat16 or float16, got ", x.scalar_type());
@@ -277,6 +302,8 @@ Tensor workspace(const Tensor& like, int64_t batch, int64_t rows, int64_t cols) 
 
 Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, double eps) {
     const at::NoGradGuard no_grad;
+    check_not_traced("orthogonalize");
+    check_plain(g, "g", "orthogonalize");
     check_matrix(g, "g");
     const int64_t rows = g.size(-2), cols = g.size(-1);
     Tensor out = at::empty(g.sizes(), g.options());
@@ -354,12 +381,16 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     TORCH_CHECK(params.size() == grads.size() && params.size() == momenta.size(),
                 "expected as many gradients and momenta as parameters, got ", params.size(), ", ", grads.size(), ", ",
                 momenta.size());
+    check_not_traced("the Muon step");
     using Key = std::tuple<int64_t, int64_t, at::ScalarType, at::ScalarType>;
     std::vector<std::pair<Key, Group>> groups;
     std::vector<Tensor> keep;  // contiguous copies of gradients, alive until the launches
     for (size_t i = 0; i < params.size(); ++i) {
         const Tensor &p = params[i], &m = momenta[i];
         Tensor g = grads[i];
+        check_plain(p, "parameter", "the Muon step");
+        check_plain(g, "gradient", "the Muon step");
+        check_plain(m, "momentum", "the Muon step");
         check_matrix(p, "parameter");
         TORCH_CHECK(g.sizes() == p.sizes() && m.sizes() == p.sizes(), "shape mismatch: parameter ", p.sizes(), ", gradient ",
                     g.sizes(), ", momentum ", m.sizes());

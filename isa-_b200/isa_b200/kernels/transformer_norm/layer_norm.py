@@ -11,7 +11,9 @@ other layouts are copied).  Statistics and sums are fp32, results are rounded
 once.  ``out_dtype`` is the type of ``y``: fp32 streams may hand out any of the
 three, 16-bit streams their own type or fp32.  The backward is one pass over the
 rows and a fixed-order reduction for the weight gradients, so it gives the same
-bits every time; it cannot be differentiated again.
+bits every time; it cannot be differentiated again.  There is no forward-mode
+derivative, and a trace (``torch.jit.trace``, ``make_fx``) would miss the kernels:
+both are refused, with and without gradients recorded.
 
 A backward captured into a CUDA graph follows torch's rule: no eager graph of the
 same leaf parameters, made on the default stream, may be alive during the capture

@@ -12,7 +12,8 @@ from isa_b200.kernels.transformer_norm import cuda_add_layer_norm, cuda_layer_no
 
 class LayerNorm(nn.LayerNorm):
     """``nn.LayerNorm`` over the last axis: same constructor, parameters and state
-    dict, CUDA inputs only.
+    dict, CUDA inputs only.  Forward-mode tangents and traces, which ``nn.LayerNorm``
+    takes, raise.
 
     ``out_dtype`` is the type handed out.  None keeps ``nn.LayerNorm``'s own: the
     input's, or fp32 under CUDA autocast.  A norm that feeds an autocast
