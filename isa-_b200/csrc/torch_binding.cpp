@@ -79,6 +79,9 @@ void check_plain(const Tensor& t, const char* name, const char* what) {
                 " takes plain tensors");
 }
 
+// The values that memory holds for a tensor: a view with its negative bit set is written out.
+Tensor values(const Tensor& t) { return t.is_neg() ? t.resolve_neg() : t; }
+
 void* stream() { return c10::cuda::getCurrentCUDAStream().stream(); }
 
 // ------------------------------------------------------------- layer norm ---
@@ -88,7 +91,8 @@ struct Rows {
     Tensor t;
     int64_t stride;
 };
-Rows rows_of(const Tensor& t, int64_t cols) {
+Rows rows_of(const Tensor& view, int64_t cols) {
+    const Tensor t = values(view);
     if (t.is_contiguous()) return {t, cols};
     Tensor r = t.dim() == 2 ? t : t.reshape({-1, cols});
     if (cols > 1 && r.stride(1) != 1) r = r.contiguous();
@@ -141,8 +145,8 @@ Normed norm_forward(const Tensor& x, const OptTensor& delta, const OptTensor& we
     const Rows x2 = rows_of(x, cols);
     const Rows d2 = delta ? rows_of(*delta, cols) : Rows{Tensor(), 0};
     Normed r;
-    r.weight = weight ? weight->contiguous() : Tensor();
-    const Tensor b = bias ? bias->contiguous() : Tensor();
+    r.weight = weight ? values(*weight).contiguous() : Tensor();
+    const Tensor b = bias ? values(*bias).contiguous() : Tensor();
     r.y = at::empty(x.sizes(), x.options().dtype(out));
     if (delta) r.h = at::empty(x.sizes(), x.options());
     if (keep) r.stats = at::empty({2, rows}, x.options().dtype(at::kFloat));
@@ -308,7 +312,8 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, do
     const int64_t rows = g.size(-2), cols = g.size(-1);
     Tensor out = at::empty(g.sizes(), g.options());
     if (g.numel() == 0) return out;
-    Tensor g3 = g.dim() == 3 ? g : g.reshape({-1, rows, cols});
+    Tensor g3 = values(g);
+    if (g3.dim() != 3) g3 = g3.reshape({-1, rows, cols});
     if (cols > 1 && g3.stride(2) != 1) g3 = g3.contiguous();
     const int64_t batch = g3.size(0);
     TORCH_CHECK(batch <= 65535, "orthogonalize takes at most 65535 matrices, got ", batch);
@@ -398,8 +403,8 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
                     "parameters, gradients and momenta must be on one device");
         TORCH_CHECK(available(g.scalar_type()), "gradient must be float32, bfloat16 or float16, got ", g.scalar_type());
         TORCH_CHECK(m.scalar_type() == at::kFloat, "momentum must be float32, got ", m.scalar_type());
-        TORCH_CHECK(p.is_contiguous() && m.is_contiguous(),
-                    "parameters and momenta are updated in place and must be contiguous");
+        TORCH_CHECK(p.is_contiguous() && m.is_contiguous() && !p.is_neg() && !m.is_neg(),
+                    "parameters and momenta are updated in place and must be contiguous, without a negative bit");
     }
     if (lr_tensor)
         TORCH_CHECK(lr_tensor->numel() == 1 && lr_tensor->scalar_type() == at::kFloat && !params.empty() &&
@@ -415,7 +420,7 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     };
     std::vector<Range> ranges;
     const auto add = [&](const Tensor& t, bool written) {
-        if (t.numel() && (written || t.is_contiguous()))  // other gradients are copied first
+        if (t.numel() && (written || (t.is_contiguous() && !t.is_neg())))  // other gradients are copied first
             ranges.push_back({(uintptr_t)t.data_ptr(), (uintptr_t)t.data_ptr() + t.numel() * t.element_size(), written});
     };
     for (size_t i = 0; i < params.size(); ++i) {
@@ -435,7 +440,7 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
         const Tensor &p = params[i], &m = momenta[i];
         if (p.numel() == 0) continue;
         Tensor g = grads[i];
-        if (!g.is_contiguous()) keep.push_back(g = g.contiguous());
+        if (!g.is_contiguous() || g.is_neg()) keep.push_back(g = values(g).contiguous());
         const Key key{p.size(-2), p.size(-1), p.scalar_type(), g.scalar_type()};
         size_t k = 0;
         while (k < groups.size() && groups[k].first != key) ++k;

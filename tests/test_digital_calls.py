@@ -99,3 +99,47 @@ def test_dispatch_modes_that_only_look_on(norms):
     assert torch.equal(got, want) and torch.equal(g, torch.autograd.grad(want.sum(), x)[0])
     again = torch.utils.checkpoint.checkpoint(layer_norm, x, use_reentrant=False)
     assert torch.equal(torch.autograd.grad(again.sum(), x)[0], g)
+
+
+# ------------------------------------------------------------------------ views --
+
+@gpu
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_norm_of_negative_views(norms, dtype):
+    """Memory that holds the negatives of a tensor's values (the imaginary part of a conjugate is one)."""
+    layer_norm, add_layer_norm = norms
+    neg = torch._neg_view
+    x, d, dy, dh = (torch.randn(9, 40, device="cuda").to(dtype) for _ in range(4))
+    w, b = torch.randn(40, device="cuda").to(dtype), torch.randn(40, device="cuda").to(dtype)
+    leaves = [t.clone().requires_grad_(True) for t in (x, d, w, b)]
+    want = add_layer_norm(*leaves)
+    want += torch.autograd.grad(want, leaves, (dy, dh))
+    others = [(-t).requires_grad_(True) for t in (x, d, w, b)]
+    got = add_layer_norm(*(neg(t) for t in others))
+    got += tuple(-g for g in torch.autograd.grad(got, others, (neg(-dy), neg(-dh))))
+    assert all(torch.equal(p, q) for p, q in zip(want, got))
+    assert torch.equal(layer_norm(neg(x), neg(w), neg(b)), layer_norm(-x, -w, -b))
+    z = torch.complex(torch.randn(6, 40, device="cuda"), torch.randn(6, 40, device="cuda"))
+    assert z.conj().imag.is_neg() and torch.equal(layer_norm(z.conj().imag), layer_norm(-z.imag))
+
+
+@gpu
+def test_muon_of_negative_views(muons):
+    orthogonalize, muon_step = muons
+    neg = torch._neg_view
+    g = torch.randn(3, 30, 20, device="cuda")
+    assert torch.equal(orthogonalize(neg(g)), orthogonalize(-g))
+    p, m = torch.randn_like(g), torch.randn_like(g)
+    want = p.clone(), m.clone()
+    muon_step([want[0]], [-g], [want[1]], lr=0.1)
+    got = p.clone(), m.clone()
+    for bad in (([neg(got[0])], [g], [got[1]]), ([got[0]], [g], [neg(got[1])])):
+        with pytest.raises(RuntimeError, match="negative bit"):
+            muon_step(*bad, lr=0.1)
+    muon_step([got[0]], [neg(g)], [got[1]], lr=0.1)
+    assert all(torch.equal(a, c) for a, c in zip(want, got))
+    # a gradient that is its momentum's negative is written out first, so nothing overlaps
+    a, c = (p.clone(), m.clone()), (p.clone(), m.clone())
+    muon_step([a[0]], [neg(a[1])], [a[1]], lr=0.1)
+    muon_step([c[0]], [-c[1]], [c[1]], lr=0.1)
+    assert all(torch.equal(s, t) for s, t in zip(a, c))
