@@ -20,6 +20,7 @@
 
 #include <algorithm>
 #include <array>
+#include <climits>
 #include <cmath>
 #include <map>
 #include <tuple>
@@ -56,6 +57,9 @@ void bind(const std::map<std::string, uintptr_t>& at) {
     get(lib.muon_shares, "cimekv_muon_shares");
     get(lib.muon_step_on, "cimekv_muon_step_on");
 }
+
+// A number of steps as the library's int; one that does not fit is none that it takes.
+int steps_of(int64_t steps) { return (int)std::clamp<int64_t>(steps, -1, INT_MAX); }
 
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, what, " failed (status ", rc, "): ", lib.last_error()); }
 
@@ -320,7 +324,7 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, do
     const c10::cuda::CUDAGuard guard(g.device());
     const Tensor ws = workspace(g, batch, rows, cols);
     check(lib.orthogonalize(g3.data_ptr(), code(g.scalar_type()), g3.stride(0), g3.stride(1), (int)batch, (int)rows, (int)cols,
-                            (int)steps, (float)c[0], (float)c[1], (float)c[2], (float)eps, out.data_ptr(), ws.data_ptr(),
+                            steps_of(steps), (float)c[0], (float)c[1], (float)c[2], (float)eps, out.data_ptr(), ws.data_ptr(),
                             (size_t)ws.numel(), stream()),
           "cimekv_orthogonalize");
     return out;
@@ -464,7 +468,7 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
             check(lib.muon_step_on(share, (int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
                                    group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
                                    lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum, nesterov,
-                                   (float)weight_decay, (float)scale, (int)steps, (float)c[0], (float)c[1], (float)c[2],
+                                   (float)weight_decay, (float)scale, steps_of(steps), (float)c[0], (float)c[1], (float)c[2],
                                    (float)eps, ws.data_ptr(), (size_t)ws.numel(), on),
                   "cimekv_muon_step");
     };

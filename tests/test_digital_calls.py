@@ -143,3 +143,19 @@ def test_muon_of_negative_views(muons):
     muon_step([a[0]], [neg(a[1])], [a[1]], lr=0.1)
     muon_step([c[0]], [-c[1]], [c[1]], lr=0.1)
     assert all(torch.equal(s, t) for s, t in zip(a, c))
+
+
+# ----------------------------------------------------------------------- numbers --
+
+@gpu
+def test_steps_beyond_an_int(muons):
+    """2^32 + 5 steps are refused, not taken for 5."""
+    orthogonalize, muon_step = muons
+    g = torch.randn(8, 8, device="cuda")
+    p, m = torch.ones_like(g), torch.zeros_like(g)
+    for steps in (2 ** 32 + 5, -2 ** 32 + 5, 2 ** 31, 65, 0, -1):
+        with pytest.raises(RuntimeError, match="1 to 64 steps"):
+            orthogonalize(g, steps=steps)
+        with pytest.raises(RuntimeError, match="1 to 64 steps"):
+            muon_step([p], [g], [m], lr=0.1, steps=steps)
+    assert (p == 1).all() and not m.any()
