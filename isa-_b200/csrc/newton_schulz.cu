@@ -1275,15 +1275,29 @@ int check_iteration(int batch, int rows, int cols, int steps, float a, float b, 
     if (!std::isfinite(a) || !std::isfinite(b) || !std::isfinite(c))
         return fail(CIMEKV_EINVAL_SHAPE, "orthogonalize: coefficients must be finite");
     // Largest singular values of X, B and P over the steps: they must fit the
-    // planes' fixed scale (2^16 / 2^12).
-    const double shift = c != 0.0f ? 0.5 * b / c : 0.0;
+    // planes' fixed scale (2^16 / 2^12).  For a singular value t of X, u = t^2, these are
+    // t |p(u)|, |u + b / 2c| and |p(u)|, p(u) = a + b u + c u^2: largest at an end or where a derivative
+    // vanishes (a + 3 b u + 5 c u^2 = 0, b + 2 c u = 0).  1 us for five steps.
+    const double da = a, db = b, dc = c, shift = c != 0.0f ? 0.5 * db / dc : 0.0;
+    double at[5] = {0.0, 0.0, 0.0, 0.0, 0.0};  // last: the end, s^2
+    if (c != 0.0f) {
+        const double d = 9.0 * db * db - 20.0 * da * dc;
+        const double q = d >= 0.0 ? -0.5 * (3.0 * db + std::copysign(std::sqrt(d), db)) : 0.0;
+        at[1] = q / (5.0 * dc);
+        at[2] = q != 0.0 ? da / q : 0.0;
+        at[3] = -shift;
+    } else if (b != 0.0f) {
+        at[1] = -da / (3.0 * db);
+    }
     double s = 1.001;
     for (int k = 0; k < steps; ++k) {
-        double next = 0.0, most = std::fabs(shift);
-        for (int i = 0; i <= 1024; ++i) {
-            const double t = s * i / 1024.0, q = a + (b + c * t * t) * t * t;
-            next = std::fmax(next, std::fabs(t * q));
-            most = std::fmax(most, std::fmax(std::fabs(q), std::fabs(t * t + shift)));
+        double next = 0.0, most = 0.0;
+        at[4] = s * s;
+        for (const double u : at) {
+            if (!(u >= 0.0 && u <= at[4])) continue;
+            const double p = std::fabs(da + (db + dc * u) * u);
+            next = std::fmax(next, std::sqrt(u) * p);
+            most = std::fmax(most, std::fmax(p, std::fabs(u + shift)));
         }
         s = next * 1.001;
         if (!(s <= 3.9 && most <= 15.0))

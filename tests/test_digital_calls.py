@@ -159,3 +159,53 @@ def test_steps_beyond_an_int(muons):
         with pytest.raises(RuntimeError, match="1 to 64 steps"):
             muon_step([p], [g], [m], lr=0.1, steps=steps)
     assert (p == 1).all() and not m.any()
+
+
+def _accepted(lib, steps, a, b, c):
+    rc = lib.cimekv_orthogonalize(None, 0, 0, 0, 0, 8, 8, steps, a, b, c, 1e-7, None, None, 0, None)  # of no matrices
+    assert rc in (0, 1) and (rc == 0 or b"beyond" in lib.cimekv_last_error())
+    return rc == 0
+
+
+def test_coefficients_by_what_they_let_grow():
+    """Accepted are those whose singular values stay below 3.9 and whose factors stay below 15, by dense sampling."""
+    import numpy as np
+    from isa_b200 import _lib
+    lib = _lib.load()
+    rng = np.random.default_rng(0)
+    seen = set()
+    for k in range(3000):
+        a, b, c = (float(np.float32(v)) for v in rng.normal(size=3) * rng.choice([0.3, 2.0, 6.0], 3))
+        if k % 5 == 0:
+            c = 0.0
+        if k % 7 == 0:
+            b = 0.0
+        steps = int(rng.integers(1, 7))
+        s, shift, size, sure = 1.001, 0.5 * b / c if c else 0.0, 0.0, True
+        for _ in range(steps):
+            t = np.linspace(0.0, s, 20001)
+            q = a + (b + c * t * t) * t * t
+            s = np.abs(t * q).max() * 1.001
+            size = max(size, s / 3.9, np.abs(q).max() / 15.0, np.abs(t * t + shift).max() / 15.0, abs(shift) / 15.0)
+            if size > 1e6:
+                break
+        if abs(size - 1.0) > 1e-4:  # on either side of the limit by more than the sampling
+            assert _accepted(lib, steps, a, b, c) == (size < 1.0), (steps, a, b, c, size)
+            seen.add(size < 1.0)
+    assert seen == {True, False}
+    for known in ((3.4445, -4.7750, 2.0315), (1.5, -0.5, 0.0), (1.875, -1.25, 0.375), (2.0, -1.5, 0.5), (1.0, 0.0, 0.0)):
+        assert _accepted(lib, 5, *known)
+
+
+def test_checking_coefficients_takes_no_time():
+    """The checks before a launch are a few microseconds of the host's (sampling the polynomial took 50)."""
+    import time
+    from isa_b200 import _lib
+    lib = _lib.load()
+    times = []
+    for _ in range(7):
+        began = time.process_time()
+        for _ in range(500):
+            _accepted(lib, 5, 3.4445, -4.7750, 2.0315)
+        times.append((time.process_time() - began) / 500)
+    assert min(times) < 20e-6, min(times)
