@@ -338,6 +338,16 @@ int cimekv_muon_step_on(int share, int count, void* const* params, const void* c
                         void* workspace, size_t workspace_bytes, void* stream);
 
 /*
+ * cimekv_muon_step_on with the gradient's weight given: m <- momentum m + gain g, u likewise.  The other two form
+ * 1 - momentum from a momentum that is rounded already: off by 2.4e-7 of itself at 0.95, by 1.3e-5 at 0.999.
+ */
+int cimekv_muon_step_weighted(int share, int count, void* const* params, const void* const* grads, float* const* momenta,
+                              int p_type, int g_type, int rows, int cols, float lr, const float* lr_device,
+                              float momentum, float gain, int nesterov, float weight_decay, float scale,
+                              int steps, float a, float b, float c, float eps,
+                              void* workspace, size_t workspace_bytes, void* stream);
+
+/*
  * Debug support, no counterpart in the reference.  cimekv_debug_build()
  * returns 1 for the library variant built with CIMEKV_DEBUG_BOUNDS=1
  * (libcimekv_debug.so), whose kernels check every table index against the

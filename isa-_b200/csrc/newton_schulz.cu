@@ -297,7 +297,7 @@ struct Matrices {
 struct PrepParams {
     Matrices g;
     Matrices mom;       // momenta (fp32, contiguous), table only; tabled = 0: none
-    float beta;
+    float beta, gain;   // of the momentum and of the gradient
     int nesterov;
     int rows, cols;     // of G
     int transposed;     // rows > cols
@@ -317,12 +317,10 @@ __device__ __forceinline__ void chain() {
 }
 
 // The update before orthogonalisation: G itself, or the (Nesterov) momentum after
-// its own update m <- beta m + (1 - beta) g.
-__device__ __forceinline__ float new_momentum(const PrepParams& p, float g, float m) {
-    return fmaf(p.beta, m, (1.0f - p.beta) * g);
-}
+// its own update m <- beta m + gain g.
+__device__ __forceinline__ float new_momentum(const PrepParams& p, float g, float m) { return fmaf(p.beta, m, p.gain * g); }
 __device__ __forceinline__ float update_of(const PrepParams& p, float g, float m) {
-    return p.nesterov ? fmaf(p.beta, m, (1.0f - p.beta) * g) : m;
+    return p.nesterov ? fmaf(p.beta, m, p.gain * g) : m;
 }
 
 // Four neighbours from an address that is a multiple of four elements.
@@ -1665,6 +1663,16 @@ extern "C" int cimekv_muon_step_on(int share, int count, void* const* params, co
                                    const float* lr_device, float momentum, int nesterov, float weight_decay, float scale,
                                    int steps, float a, float b, float c, float eps, void* workspace,
                                    size_t workspace_bytes, void* stream) {
+    return cimekv_muon_step_weighted(share, count, params, grads, momenta, p_type, g_type, rows, cols, lr, lr_device,
+                                     momentum, 1.0f - momentum, nesterov, weight_decay, scale, steps, a, b, c, eps, workspace,
+                                     workspace_bytes, stream);
+}
+
+extern "C" int cimekv_muon_step_weighted(int share, int count, void* const* params, const void* const* grads,
+                                         float* const* momenta, int p_type, int g_type, int rows, int cols, float lr,
+                                         const float* lr_device, float momentum, float gain, int nesterov,
+                                         float weight_decay, float scale, int steps, float a, float b, float c, float eps,
+                                         void* workspace, size_t workspace_bytes, void* stream) {
     NvtxRange nvtx_range("cimekv_muon_step");
     int rc = cimekv_internal_begin_call();
     if (rc || (rc = check_iteration(count, rows, cols, steps, a, b, c, eps))) return rc;
@@ -1672,6 +1680,7 @@ extern "C" int cimekv_muon_step_on(int share, int count, void* const* params, co
     if (count > kMaxTable) return fail(CIMEKV_EINVAL_SHAPE, "muon step: too many matrices for one call");
     if (!valid_type(p_type) || !valid_type(g_type)) return fail(CIMEKV_EINVAL_SHAPE, "unknown element type");
     if (!(momentum >= 0.0f && momentum <= 1.0f)) return fail(CIMEKV_EINVAL_SHAPE, "momentum must be in [0, 1]");
+    if (!std::isfinite(gain)) return fail(CIMEKV_EINVAL_SHAPE, "the gradient's weight must be finite");
     if (count == 0 || rows == 0 || cols == 0) return CIMEKV_OK;
     if (!params || !grads || !momenta) return fail(CIMEKV_EINVAL_SHAPE, "null pointer");
     for (int i = 0; i < count; ++i)
@@ -1703,6 +1712,7 @@ extern "C" int cimekv_muon_step_on(int share, int count, void* const* params, co
         last.dst.table[i] = params[i];
     }
     prep.beta = momentum;
+    prep.gain = gain;
     prep.nesterov = nesterov;
     prep.eps = eps;
     last.update = 1;

@@ -43,7 +43,7 @@ struct Library {
     decltype(&cimekv_orthogonalize) orthogonalize = nullptr;
     decltype(&cimekv_orthogonalize_workspace_bytes) orthogonalize_workspace = nullptr;
     decltype(&cimekv_muon_shares) muon_shares = nullptr;
-    decltype(&cimekv_muon_step_on) muon_step_on = nullptr;
+    decltype(&cimekv_muon_step_weighted) muon_step = nullptr;
 } lib;
 
 void bind(const std::map<std::string, uintptr_t>& at) {
@@ -55,7 +55,7 @@ void bind(const std::map<std::string, uintptr_t>& at) {
     get(lib.orthogonalize, "cimekv_orthogonalize");
     get(lib.orthogonalize_workspace, "cimekv_orthogonalize_workspace_bytes");
     get(lib.muon_shares, "cimekv_muon_shares");
-    get(lib.muon_step_on, "cimekv_muon_step_on");
+    get(lib.muon_step, "cimekv_muon_step_weighted");
 }
 
 // A number of steps as the library's int; one that does not fit is none that it takes.
@@ -465,11 +465,11 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
                                        : std::sqrt(std::max(1.0, (double)rows / (double)cols));
         const int64_t count = (int64_t)group.params.size();
         for (int64_t i = 0; i < count; i += most)
-            check(lib.muon_step_on(share, (int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
-                                   group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
-                                   lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum, nesterov,
-                                   (float)weight_decay, (float)scale, steps_of(steps), (float)c[0], (float)c[1], (float)c[2],
-                                   (float)eps, ws.data_ptr(), (size_t)ws.numel(), on),
+            check(lib.muon_step(share, (int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
+                                group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
+                                lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum,
+                                (float)(1.0 - momentum), nesterov, (float)weight_decay, (float)scale, steps_of(steps),
+                                (float)c[0], (float)c[1], (float)c[2], (float)eps, ws.data_ptr(), (size_t)ws.numel(), on),
                   "cimekv_muon_step");
     };
     const auto room = [&](const std::pair<Key, Group>& of) {

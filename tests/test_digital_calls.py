@@ -209,3 +209,16 @@ def test_checking_coefficients_takes_no_time():
             _accepted(lib, 5, 3.4445, -4.7750, 2.0315)
         times.append((time.process_time() - began) / 500)
     assert min(times) < 20e-6, min(times)
+
+
+@gpu
+@pytest.mark.parametrize("momentum", [0.0, 0.5, 0.9, 0.95, 0.999, 0.99999, 1.0])
+def test_weight_of_the_gradient(muons, momentum):
+    """From zeros the momentum is (1 - momentum) g: one rounding of the weight and one of the product, each half of 2^-23
+    (a weight formed from the rounded momentum is off by up to 2^-25 / (1 - momentum) of itself)."""
+    _, muon_step = muons
+    g = torch.randn(70, 90, device="cuda")
+    m = torch.zeros_like(g)
+    muon_step([torch.zeros_like(g)], [g], [m], lr=0.1, momentum=momentum)
+    want = (1.0 - momentum) * g.double()
+    assert ((m.double() - want).abs() <= 2.01 * 2.0 ** -24 * want.abs()).all()
