@@ -303,6 +303,16 @@ void check_matrix(const Tensor& t, const char* name) {
                 " must have sides of at most ", CIMEKV_ORTHOGONALIZE_MAX_SIDE, ", got shape ", t.sizes());
 }
 
+// Matrices of one launch: at most `most`, and no more than `room` bytes of workspace hold (one matrix takes what it
+// takes), in launches of about one size.  Matrices this large fill the chip by themselves: 16 of 4,096 x 4,096
+// take 3,490 us each in one launch (4 GB of workspace) and 3,460 in two.
+constexpr int64_t kRoom = 2ll << 30;
+int64_t at_once(int64_t count, int64_t rows, int64_t cols, int64_t most, int64_t room = kRoom) {
+    const int64_t one = std::max<int64_t>(1, (int64_t)lib.orthogonalize_workspace(1, (int)rows, (int)cols));
+    const int64_t fit = std::clamp<int64_t>(room / one, 1, most), calls = (count + fit - 1) / fit;
+    return (count + calls - 1) / calls;
+}
+
 Tensor workspace(const Tensor& like, int64_t batch, int64_t rows, int64_t cols) {
     const size_t bytes = lib.orthogonalize_workspace((int)batch, (int)rows, (int)cols);
     return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
@@ -322,11 +332,15 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, do
     const int64_t batch = g3.size(0);
     TORCH_CHECK(batch <= 65535, "orthogonalize takes at most 65535 matrices, got ", batch);
     const c10::cuda::CUDAGuard guard(g.device());
-    const Tensor ws = workspace(g, batch, rows, cols);
-    check(lib.orthogonalize(g3.data_ptr(), code(g.scalar_type()), g3.stride(0), g3.stride(1), (int)batch, (int)rows, (int)cols,
-                            steps_of(steps), (float)c[0], (float)c[1], (float)c[2], (float)eps, out.data_ptr(), ws.data_ptr(),
-                            (size_t)ws.numel(), stream()),
-          "cimekv_orthogonalize");
+    const int64_t each = at_once(batch, rows, cols, batch), size = g.element_size();
+    const Tensor ws = workspace(g, each, rows, cols);
+    for (int64_t i = 0; i < batch; i += each)
+        check(lib.orthogonalize(static_cast<const char*>(g3.data_ptr()) + i * g3.stride(0) * size, code(g.scalar_type()),
+                                g3.stride(0), g3.stride(1), (int)std::min(each, batch - i), (int)rows, (int)cols,
+                                steps_of(steps), (float)c[0], (float)c[1], (float)c[2], (float)eps,
+                                static_cast<char*>(out.data_ptr()) + i * rows * cols * size, ws.data_ptr(),
+                                (size_t)ws.numel(), stream()),
+              "cimekv_orthogonalize");
     return out;
 }
 
@@ -457,24 +471,29 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
             to.momenta.push_back(m.data_ptr<float>() + at);
         }
     }
-    const int64_t most = CIMEKV_MUON_MAX_MATRICES;
-    const auto step = [&](const std::pair<Key, Group>& of, const Tensor& ws, int share, void* on) {
+    struct Room {
+        Tensor ws;
+        int64_t each;  // matrices of a launch
+    };
+    const auto step = [&](const std::pair<Key, Group>& of, const Room& room, int share, void* on) {
         const auto& [key, group] = of;
         const auto& [rows, cols, p_type, g_type] = key;
         const double scale = match_rms ? 0.2 * std::sqrt((double)std::max(rows, cols))
                                        : std::sqrt(std::max(1.0, (double)rows / (double)cols));
         const int64_t count = (int64_t)group.params.size();
-        for (int64_t i = 0; i < count; i += most)
-            check(lib.muon_step(share, (int)std::min(most, count - i), group.params.data() + i, group.grads.data() + i,
+        for (int64_t i = 0; i < count; i += room.each)
+            check(lib.muon_step(share, (int)std::min(room.each, count - i), group.params.data() + i, group.grads.data() + i,
                                 group.momenta.data() + i, code(p_type), code(g_type), (int)rows, (int)cols, (float)lr,
                                 lr_tensor ? lr_tensor->data_ptr<float>() : nullptr, (float)momentum,
                                 (float)(1.0 - momentum), nesterov, (float)weight_decay, (float)scale, steps_of(steps),
-                                (float)c[0], (float)c[1], (float)c[2], (float)eps, ws.data_ptr(), (size_t)ws.numel(), on),
+                                (float)c[0], (float)c[1], (float)c[2], (float)eps, room.ws.data_ptr(),
+                                (size_t)room.ws.numel(), on),
                   "cimekv_muon_step");
     };
-    const auto room = [&](const std::pair<Key, Group>& of) {
-        return workspace(params[0], std::min<int64_t>(of.second.params.size(), most), std::get<0>(of.first),
-                         std::get<1>(of.first));
+    const auto room = [&](const std::pair<Key, Group>& of, int64_t beside) {
+        const int64_t rows = std::get<0>(of.first), cols = std::get<1>(of.first);
+        const int64_t each = at_once((int64_t)of.second.params.size(), rows, cols, CIMEKV_MUON_MAX_MATRICES, kRoom / beside);
+        return Room{workspace(params[0], each, rows, cols), each};
     };
     // small matrices of several shapes run side by side, each on its share of the SMs
     std::vector<int> counts, rows, cols, shares(groups.size(), 0);
@@ -487,10 +506,11 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
         check(lib.muon_shares((int)groups.size(), counts.data(), rows.data(), cols.data(), (float)c[2], 0, shares.data()),
               "cimekv_muon_shares");
     }
-    std::vector<Tensor> rooms;  // of those side by side, until the streams have joined
+    const int64_t beside = groups.size() - std::count(shares.begin(), shares.end(), 0);
+    std::vector<Room> rooms;  // of those side by side, until the streams have joined
     for (size_t k = 0; k < groups.size(); ++k) {
-        if (shares[k]) rooms.push_back(room(groups[k]));
-        else step(groups[k], room(groups[k]), 0, stream());
+        if (shares[k]) rooms.push_back(room(groups[k], beside));
+        else step(groups[k], room(groups[k], 1), 0, stream());
     }
     if (!rooms.empty()) {
         Beside beside(params[0].device().index());

@@ -222,3 +222,36 @@ def test_weight_of_the_gradient(muons, momentum):
     muon_step([torch.zeros_like(g)], [g], [m], lr=0.1, momentum=momentum)
     want = (1.0 - momentum) * g.double()
     assert ((m.double() - want).abs() <= 2.01 * 2.0 ** -24 * want.abs()).all()
+
+
+# ------------------------------------------------------------------------ memory --
+
+def _peak(call):
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    call()
+    return torch.cuda.max_memory_allocated() - before
+
+
+@gpu
+def test_workspace_does_not_grow_with_the_number_of_matrices(muons):
+    """16 bytes an element held at once for 200 matrices of 1,024 x 1,024 would be 3.4 GB: 2 GiB are the limit, and the
+    launches that this makes get each matrix right."""
+    from tests.test_muon import _assert_near, _exact, _update, _want_step
+    orthogonalize, muon_step = muons
+    g = torch.cat([_update("cuda", 50, 1024, 1024, seed=i, dtype=BF16) for i in range(4)])
+    out = []
+    assert _peak(lambda: out.append(orthogonalize(g))) < (2 << 30) + 2 * g.numel() + (1 << 20)
+    out = out[0]
+    for i in (0, 99, 100, 199):
+        _assert_near(out[i], *_exact(g[i]), f"matrix {i}")
+    wide = g[::2].transpose(1, 2)[:, :, :900]  # rows and matrices further apart than they are large
+    assert torch.equal(orthogonalize(wide), orthogonalize(wide.contiguous()))
+    del out
+    p, m = torch.zeros(200, 1024, 1024, device="cuda"), torch.zeros(200, 1024, 1024, device="cuda")
+    assert _peak(lambda: muon_step([p], [g], [m], lr=1.0, weight_decay=0.0)) < (2 << 30) + (1 << 20)
+    zero = torch.zeros(1024, 1024, device="cuda")
+    for i in (0, 99, 100, 127, 128, 199):
+        want, bound, _, _ = _want_step(zero, g[i], zero, 1.0, weight_decay=0.0)
+        _assert_near(p[i], want, bound, f"matrix {i}")
