@@ -313,10 +313,7 @@ int64_t at_once(int64_t count, int64_t rows, int64_t cols, int64_t most, int64_t
     return (count + calls - 1) / calls;
 }
 
-Tensor workspace(const Tensor& like, int64_t batch, int64_t rows, int64_t cols) {
-    const size_t bytes = lib.orthogonalize_workspace((int)batch, (int)rows, (int)cols);
-    return at::empty({(int64_t)bytes}, like.options().dtype(at::kByte));
-}
+Tensor workspace(const Tensor& like, int64_t bytes) { return at::empty({bytes}, like.options().dtype(at::kByte)); }
 
 Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, double eps) {
     const at::NoGradGuard no_grad;
@@ -333,7 +330,7 @@ Tensor orthogonalize(const Tensor& g, int64_t steps, std::array<double, 3> c, do
     TORCH_CHECK(batch <= 65535, "orthogonalize takes at most 65535 matrices, got ", batch);
     const c10::cuda::CUDAGuard guard(g.device());
     const int64_t each = at_once(batch, rows, cols, batch), size = g.element_size();
-    const Tensor ws = workspace(g, each, rows, cols);
+    const Tensor ws = workspace(g, (int64_t)lib.orthogonalize_workspace((int)each, (int)rows, (int)cols));
     for (int64_t i = 0; i < batch; i += each)
         check(lib.orthogonalize(static_cast<const char*>(g3.data_ptr()) + i * g3.stride(0) * size, code(g.scalar_type()),
                                 g3.stride(0), g3.stride(1), (int)std::min(each, batch - i), (int)rows, (int)cols,
@@ -473,7 +470,7 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     }
     struct Room {
         Tensor ws;
-        int64_t each;  // matrices of a launch
+        int64_t each, bytes;  // matrices of a launch, and what these take
     };
     const auto step = [&](const std::pair<Key, Group>& of, const Room& room, int share, void* on) {
         const auto& [key, group] = of;
@@ -493,7 +490,7 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
     const auto room = [&](const std::pair<Key, Group>& of, int64_t beside) {
         const int64_t rows = std::get<0>(of.first), cols = std::get<1>(of.first);
         const int64_t each = at_once((int64_t)of.second.params.size(), rows, cols, CIMEKV_MUON_MAX_MATRICES, kRoom / beside);
-        return Room{workspace(params[0], each, rows, cols), each};
+        return Room{Tensor(), each, (int64_t)lib.orthogonalize_workspace((int)each, (int)rows, (int)cols)};
     };
     // small matrices of several shapes run side by side, each on its share of the SMs
     std::vector<int> counts, rows, cols, shares(groups.size(), 0);
@@ -506,21 +503,34 @@ void muon_step(const std::vector<Tensor>& params, const std::vector<Tensor>& gra
         check(lib.muon_shares((int)groups.size(), counts.data(), rows.data(), cols.data(), (float)c[2], 0, shares.data()),
               "cimekv_muon_shares");
     }
-    const int64_t beside = groups.size() - std::count(shares.begin(), shares.end(), 0);
-    std::vector<Room> rooms;  // of those side by side, until the streams have joined
+    // All memory is asked for before anything is written: a call that it fails leaves every parameter as it was.
+    const int64_t apart = std::count(shares.begin(), shares.end(), 0), beside = (int64_t)groups.size() - apart;
+    std::vector<Room> rooms;  // those side by side have one each, until the streams have joined
+    Tensor shared;            // for the others, one after the other
     for (size_t k = 0; k < groups.size(); ++k) {
-        if (shares[k]) rooms.push_back(room(groups[k], beside));
-        else step(groups[k], room(groups[k], 1), 0, stream());
+        rooms.push_back(room(groups[k], shares[k] ? beside : 1));
+        Room& r = rooms.back();
+        if (!shares[k] && r.bytes > (shared.defined() ? shared.numel() : 0)) {
+            shared = Tensor();
+            shared = workspace(params[0], r.bytes);
+        }
+        if (shares[k]) r.ws = workspace(params[0], r.bytes);
     }
-    if (!rooms.empty()) {
-        Beside beside(params[0].device().index());
-        size_t used = 0;
+    for (size_t k = 0; k < groups.size(); ++k) {
+        if (shares[k]) continue;
+        rooms[k].ws = shared;
+        step(groups[k], rooms[k], 0, stream());
+    }
+    if (beside) {
+        Beside sides(params[0].device().index());
+        bool first = true;
         for (size_t k = 0; k < groups.size(); ++k) {
             if (!shares[k]) continue;
-            void* on = used ? (void*)beside.next().stream() : stream();
-            step(groups[k], rooms[used++], shares[k], on);
+            void* on = first ? stream() : (void*)sides.next().stream();
+            first = false;
+            step(groups[k], rooms[k], shares[k], on);
         }
-        beside.join();
+        sides.join();
     }
     // autograd must see that these were written
     for (const auto* list : {&params, &momenta})

@@ -255,3 +255,23 @@ def test_workspace_does_not_grow_with_the_number_of_matrices(muons):
     for i in (0, 99, 100, 127, 128, 199):
         want, bound, _, _ = _want_step(zero, g[i], zero, 1.0, weight_decay=0.0)
         _assert_near(p[i], want, bound, f"matrix {i}")
+
+
+@gpu
+@pytest.mark.parametrize("shapes", [[(1500, 1300), (4096, 4096)], [(64, 64), (64, 96), (4096, 4096)]])
+def test_muon_step_without_memory_leaves_everything_as_it_was(muons, shapes):
+    """Room for the first shape's workspace and not for the last one's: nothing of the call is carried out."""
+    _, muon_step = muons
+    p, g, m = ([torch.full(s, v, device="cuda", dtype=t) for s in shapes] for v, t in ((1.0, BF16), (2.0, BF16), (0.0, F32)))
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    total = torch.cuda.get_device_properties(0).total_memory
+    torch.cuda.set_per_process_memory_fraction((torch.cuda.memory_reserved() + (150 << 20)) / total)
+    try:
+        with pytest.raises(torch.OutOfMemoryError):
+            muon_step(p, g, m, lr=0.1)
+    finally:
+        torch.cuda.set_per_process_memory_fraction(1.0)
+    assert all((t == 1.0).all() for t in p) and not any(t.any() for t in m)
+    muon_step(p, g, m, lr=0.1)
+    assert all(t.any() for t in m)
