@@ -29,7 +29,8 @@ enum {
     CIMEKV_EINVAL_SHAPE = 1,    /* bad sizes, null or misaligned pointers  */
     CIMEKV_ELUT_TOO_LARGE = 2,  /* table or tile does not fit shared memory */
     CIMEKV_ECUDA = 3,           /* a CUDA runtime call or launch failed     */
-    CIMEKV_EWORKSPACE = 4       /* backward workspace too small             */
+    CIMEKV_EWORKSPACE = 4,      /* backward workspace too small             */
+    CIMEKV_ELOST = 5            /* an earlier launch gave up a wait         */
 };
 
 /* Largest LUT_DELTA_SIZE the kernels accept. */
@@ -346,6 +347,16 @@ int cimekv_muon_step_weighted(int share, int count, void* const* params, const v
                               float momentum, float gain, int nesterov, float weight_decay, float scale,
                               int steps, float a, float b, float c, float eps,
                               void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * The kernels of layer norm and of the Newton-Schulz products wait inside for copies, products and one another, two
+ * seconds at most.  A launch that gives up a wait hands out NaN in place of what was lost (a Muon step has updated its
+ * momenta by then) and marks a word in host memory; the next of these calls returns CIMEKV_ELOST, once, and launches
+ * nothing.  cimekv_lost_waits(reset) tells without a call: bit 0 layer norm, bit 1 products; it does not wait, so
+ * synchronise first.  cimekv_debug_lose_wait launches a kernel whose one wait is given up after so many milliseconds.
+ */
+unsigned int cimekv_lost_waits(int reset);
+int cimekv_debug_lose_wait(int kind, float milliseconds, void* stream);
 
 /*
  * Debug support, no counterpart in the reference.  cimekv_debug_build()

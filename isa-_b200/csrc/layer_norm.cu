@@ -36,6 +36,7 @@
 #include <utility>
 
 #include "cimekv.h"
+#include "device_wait.cuh"
 #include <nvtx3/nvToolsExt.h>
 
 int cimekv_internal_begin_call();
@@ -62,32 +63,6 @@ __host__ __device__ inline int type_bytes(int type) { return type == CIMEKV_F32 
 // ------------------------------------------------------------- PTX pieces --
 
 __device__ __forceinline__ uint32_t smem_addr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-__device__ __forceinline__ unsigned long long wall_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Waits for the phase of `parity` to end, for two seconds at most.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    unsigned long long began = 0;
-    for (int i = 0; i < (1 << 28); ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-        const unsigned long long now = wall_ns();
-        if (!began) began = now;
-        else if (now - began > 2000000000ull) return false;
-    }
-    return false;
-}
-
 // Copies the 16-byte units that hold `bytes` from `src` (the units before and
 // after belong to the same allocation: they hold some of the row).
 __device__ __forceinline__ uint32_t units(uintptr_t src, uint32_t bytes) {
@@ -380,6 +355,7 @@ struct NormParams {
     float* mean;
     float* rstd;
     float* part;
+    unsigned* lost;  // marked when a wait has run out
     long long rows, x_stride, d_stride, dy_stride, dh_stride;
     int cols, x_type, d_type, w_type, y_type;
     int stages;  // rows under way per row group
@@ -563,6 +539,7 @@ __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) n
             set2(h, k, fma2(mul2(get2(h, k), both(rstd)), get2(w, k), get2(b, k)));
         store_row<V, E>(h, row_of(p.y, p.y_type, row, p.cols), p.y_type, col0, kStep, p.cols);
     }
+    if (!ring.ok) mark_lost(p.lost);
 }
 
 // kSum: the sum's own gradient dh is added to dx.  p.part: the CTA's column sums
@@ -634,7 +611,10 @@ __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, false)) 
             if (p.dx) store_row<V, E>(g, row_of(p.dx, p.x_type, row, p.cols), p.x_type, col0, kStep, p.cols);
             if (p.dd) store_row<V, E>(g, row_of(p.dd, p.d_type, row, p.cols), p.d_type, col0, kStep, p.cols);
         }
-        if (!ring.ok) dw[0][0] = db[0][0] = __int_as_float(0x7fffffff);
+        if (!ring.ok) {
+            dw[0][0] = db[0][0] = __int_as_float(0x7fffffff);
+            mark_lost(p.lost);
+        }
     }
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (!p.part) return;
@@ -866,7 +846,7 @@ extern "C" int cimekv_layer_norm_forward(const void* x, int x_type, long long x_
     p.y_type = y_type;
     p.places = places;
     p.eps = eps;
-    if ((rc = cimekv_internal_no_pending_error())) return rc;
+    if ((rc = cimekv_internal_no_pending_error()) || (rc = cimekv_internal_wait_word(CIMEKV_WAIT_NORM, &p.lost))) return rc;
     const size_t row_bytes = row_room(cols, x_type) + (delta ? row_room(cols, delta_type) : 0);
     p.stages = ring_stages(kShapes[i], row_bytes, true);
     const Kernel kernel = kernels(i).fwd[delta != nullptr];
@@ -945,7 +925,9 @@ extern "C" int cimekv_layer_norm_backward(const void* dy, int y_type, long long 
         const Kernel kernel = kernels(i).bwd[dh != nullptr];
         size_t smem = row_bytes * p.stages * cta_rows(kShapes[i].w);
         if (cta_rows(kShapes[i].w) > 1 && smem < (size_t)2 * cols * sizeof(float)) smem = (size_t)2 * cols * sizeof(float);
-        if ((rc = cimekv_internal_no_pending_error()) || (rc = allow_smem((const void*)kernel, 4 * i + 2 + (dh != nullptr), smem))) return rc;
+        if ((rc = cimekv_internal_no_pending_error()) || (rc = cimekv_internal_wait_word(CIMEKV_WAIT_NORM, &p.lost)) ||
+            (rc = allow_smem((const void*)kernel, 4 * i + 2 + (dh != nullptr), smem)))
+            return rc;
         kernel<<<(unsigned)grid, cta_threads(kShapes[i].w), smem, s>>>(p);
         if ((rc = launched("norm_bwd_kernel"))) return rc;
         nparts = (int)grid;

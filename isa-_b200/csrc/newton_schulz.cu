@@ -45,6 +45,7 @@
 #include <utility>
 
 #include "cimekv.h"
+#include "device_wait.cuh"
 #include <nvtx3/nvToolsExt.h>
 
 int cimekv_internal_begin_call();
@@ -111,33 +112,6 @@ __device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
 }
 __device__ __forceinline__ void mbar_expect(uint32_t bar, uint32_t bytes) {
     asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-
-__device__ __forceinline__ unsigned long long wall_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-
-// Waits for the phase of `parity` to end, for two seconds at most: a wait
-// that runs out means a lost copy, and its tile is poisoned instead of hanging.
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity) {
-    unsigned long long began = 0;
-    for (int i = 0; i < (1 << 28); ++i) {
-        uint32_t done;
-        asm volatile(
-            "{\n\t.reg .pred p;\n\t"
-            "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-            "selp.u32 %0, 1, 0, p;\n\t}"
-            : "=r"(done)
-            : "r"(bar), "r"(parity)
-            : "memory");
-        if (done) return true;
-        const unsigned long long now = wall_ns();
-        if (!began) began = now;
-        else if (now - began > 2000000000ull) return false;
-    }
-    return false;
 }
 
 // Address of the same shared variable in CTA `rank` of the cluster.
@@ -554,6 +528,7 @@ struct Result {
     int update;             // parameters: p <- p (1 - lr decay) - lr scale X
     float lr, decay, scale;
     const float* lr_dev;
+    unsigned* lost;         // marked when a wait has run out (by any product, not the last alone)
 };
 
 // Tile (i, j) of the lower triangle, row by row.
@@ -778,6 +753,7 @@ struct Meet {
     uint32_t own;           // barrier of a CTA that has a matrix alone; 0: it has not
     uint32_t counted;       // warps of the CTA that have counted themselves in; the last one counts for all
     volatile int* lost;     // set when a wait has run out: from then on none is waited for and all results are NaN
+    unsigned* word;         // and what tells the host
 };
 template <int kWarps>
 __device__ __forceinline__ void meet_arrive(const Meet& m) {
@@ -797,14 +773,12 @@ __device__ __forceinline__ void meet_wait(const Meet& m) {
     if (m.target && m.own) {
         ok = mbar_wait(m.own, (m.target - 1) & 1);
     } else if (m.target) {
-        unsigned long long began = 0;
+        Patience patience;
         for (;;) {
             unsigned seen;
             asm volatile("ld.acquire.gpu.global.u32 %0, [%1];" : "=r"(seen) : "l"(m.arrivals) : "memory");
             if (seen >= m.target) break;
-            const unsigned long long now = wall_ns();
-            if (!began) began = now;
-            else if (now - began > 2000000000ull) {
+            if (!patience.left()) {
                 ok = false;
                 break;
             }
@@ -813,6 +787,7 @@ __device__ __forceinline__ void meet_wait(const Meet& m) {
     if (!ok) {
         *m.lost = 1;
         __threadfence_block();
+        mark_lost(m.word);
     }
     asm volatile("fence.proxy.async.global;" ::: "memory");
     __syncwarp();
@@ -1080,7 +1055,8 @@ __device__ __forceinline__ void pipe_open(Pipe& q, uint64_t* bars, uint32_t* tme
 // Nothing may be in flight when the CTA leaves: copies (a pair's are all
 // counted in the first CTA), products.  All threads.
 template <typename T>
-__device__ __forceinline__ void pipe_close(Pipe& q) {
+__device__ __forceinline__ void pipe_close(Pipe& q, unsigned* word) {
+    if (!q.ok) mark_lost(word);
     constexpr bool kPair = T::kPair;
     constexpr int kWarps = T::kWarps, kStages = T::kStages;
     const int warp = threadIdx.x >> 5;
@@ -1124,7 +1100,7 @@ __global__ void __launch_bounds__(Tile<kSide, kFine>::kThreads, 1) ns_gemm_kerne
     chain();
     constexpr int kRanks = T::kRanks;
     product<M, kSide, kFine>(q, &left, &right, &out, p, result, batch, blockIdx.x / kRanks, gridDim.x / kRanks, tiles);
-    pipe_close<T>(q);
+    pipe_close<T>(q, result.lost);
 }
 
 // All steps in one kernel, for matrices whose products are a few microseconds
@@ -1166,7 +1142,7 @@ __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(
     pipe_open<Tile<64, kFine>>(q, bars, &tmem_slot, smem_raw);
     const int ni = (st.product[0].rows + 63) / 64, nj = (st.product[2].cols + 63) / 64;
     const int rank = blockIdx.x % st.group, groups = gridDim.x / st.group;
-    Meet meet = {nullptr, 0, st.group > 1 ? 0 : smem_addr(&own), smem_addr(&counted), &lost};
+    Meet meet = {nullptr, 0, st.group > 1 ? 0 : smem_addr(&own), smem_addr(&counted), &lost, result.lost};
     unsigned met = 0;  // phases of `own` that earlier matrices have ended
     for (int matrix = blockIdx.x / st.group; matrix < batch; matrix += groups) {
         meet.arrivals = st.arrivals + matrix;
@@ -1188,7 +1164,7 @@ __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(
         meet.target = 0;  // the next matrix begins with what ns_prepare_kernel left
         met += count;
     }
-    pipe_close<Tile<64, kFine>>(q);
+    pipe_close<Tile<64, kFine>>(q, result.lost);
 }
 
 // ------------------------------------------------------------------ host ----
@@ -1461,7 +1437,8 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     prep.x = x[0];
     const bool vec = rows_in_fours(prep.g, batch, cols) && rows_in_fours(prep.mom, batch, cols);
     const bool flat = vec && (prep.g.row_stride == cols || rows == 1);
-    if ((rc = cimekv_internal_no_pending_error())) return rc;
+    if ((rc = cimekv_internal_no_pending_error()) || (rc = cimekv_internal_wait_word(CIMEKV_WAIT_PRODUCT, &result.lost)))
+        return rc;
     const dim3 norm_grid(lay.parts, batch);
     if (flat) ns_norm_kernel<true><<<norm_grid, 256, 0, s>>>(prep);
     else ns_norm_kernel<false><<<norm_grid, 256, 0, s>>>(prep);

@@ -69,6 +69,8 @@ SIGNATURES = {
     "cimekv_muon_step_weighted": (_c_int, [_c_int, _c_int, _vp, _vp, _vp, _c_int, _c_int, _c_int, _c_int, _c_float, _vp,
                                            _c_float, _c_float, _c_int, _c_float, _c_float, _c_int, _c_float, _c_float,
                                            _c_float, _c_float, _vp, _c_size, _vp]),
+    "cimekv_lost_waits": (ctypes.c_uint, [_c_int]),
+    "cimekv_debug_lose_wait": (_c_int, [_c_int, _c_float, _vp]),
     "cimekv_debug_build": (_c_int, []),
     "cimekv_debug_oob_count": (ctypes.c_uint, [_c_int]),
     "cimekv_fp32_probe": (_c_int, [_vp, _c_int, _c_int, ctypes.POINTER(ctypes.c_longlong), _vp]),

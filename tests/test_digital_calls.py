@@ -275,3 +275,69 @@ def test_muon_step_without_memory_leaves_everything_as_it_was(muons, shapes):
     assert all((t == 1.0).all() for t in p) and not any(t.any() for t in m)
     muon_step(p, g, m, lr=0.1)
     assert all(t.any() for t in m)
+
+
+# ------------------------------------------------------------- waits that run out --
+
+def test_lost_waits_without_a_device():
+    from isa_b200 import _lib
+    lib = _lib.load()
+    assert lib.cimekv_lost_waits(0) == 0 and lib.cimekv_lost_waits(1) == 0
+    for kind, ms in ((2, 1.0), (-1, 1.0), (0, 0.0), (0, -1.0), (0, 2000.0), (0, float("nan"))):
+        assert lib.cimekv_debug_lose_wait(kind, ms, None) == 1
+
+
+@gpu
+@pytest.mark.parametrize("kind", [0, 1])
+def test_a_wait_that_runs_out_is_told(norms, muons, kind):
+    """A wait for an arrival that never comes, given up after a millisecond: the next call fails, whichever it is, writes
+    nothing, and the one after it runs."""
+    from isa_b200 import _lib
+    lib = _lib.load()
+    (layer_norm, add_layer_norm), (orthogonalize, muon_step) = norms, muons
+    x = torch.randn(6, 32, device="cuda")
+    leaf, p, m = x.clone().requires_grad_(True), torch.ones_like(x), torch.zeros_like(x)
+    y = layer_norm(leaf)
+    calls = [lambda: layer_norm(x), lambda: add_layer_norm(x, x), lambda: orthogonalize(x), lambda: muon_step([p], [x], [m], lr=0.1),
+             lambda: torch.autograd.grad(y.sum(), leaf, retain_graph=True)]
+    for call in calls:
+        assert lib.cimekv_debug_lose_wait(kind, 1.0, torch.cuda.current_stream().cuda_stream) == 0
+        torch.cuda.synchronize()
+        assert lib.cimekv_lost_waits(0) == 1 << kind
+        with pytest.raises(RuntimeError, match="status 5.*ran out"):
+            call()
+        assert lib.cimekv_lost_waits(0) == 0 and (p == 1).all() and not m.any()
+        if call is not calls[3]:
+            call()
+    assert lib.cimekv_debug_lose_wait(kind, 1.0, None) == 0
+    torch.cuda.synchronize()
+    assert lib.cimekv_lost_waits(1) == 1 << kind  # read and cleared
+    muon_step([p], [x], [m], lr=0.1)
+    torch.cuda.synchronize()
+    assert lib.cimekv_lost_waits(0) == 0 and torch.isfinite(p).all()
+
+
+@gpu
+def test_first_call_of_a_process_inside_a_capture():
+    """What the library sets up at its first call is no part of the capture."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    code = f"""
+import sys
+sys.path.insert(0, {str(Path(__file__).resolve().parent.parent / 'isa-_b200')!r})
+import torch
+from isa_b200.kernels.muon import cuda_orthogonalize
+from isa_b200.kernels.transformer_norm import cuda_layer_norm
+x = torch.randn(64, 128, device="cuda")
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y, o = cuda_layer_norm(x), cuda_orthogonalize(x)
+for t in (y, o):
+    t.fill_(float("nan"))
+graph.replay()
+print(torch.equal(y, cuda_layer_norm(x)), torch.equal(o, cuda_orthogonalize(x)))
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and r.stdout.split() == ["True", "True"], (r.stdout, r.stderr[-2000:])
