@@ -341,3 +341,20 @@ print(torch.equal(y, cuda_layer_norm(x)), torch.equal(o, cuda_orthogonalize(x)))
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and r.stdout.split() == ["True", "True"], (r.stdout, r.stderr[-2000:])
+
+
+# --------------------------------------------------------------------- precision --
+
+@gpu
+@pytest.mark.parametrize("shape", [(64, 64), (192, 192), (40, 192, 192), (200, 130), (300, 700), (1, 768, 768), (10, 640, 640)])
+def test_fp32_parameters_get_the_precision_of_fp32_results(muons, shape):
+    """From zeros, with lr s = 1, no decay and no momentum, a step leaves exactly -NS(g): the bits of cuda_orthogonalize."""
+    orthogonalize, muon_step = muons
+    g = torch.randn(shape, device="cuda")
+    p, m = torch.zeros_like(g), torch.zeros_like(g)
+    scale = max(1.0, shape[-2] / shape[-1]) ** 0.5
+    muon_step([p], [g], [m], lr=1.0 / scale, momentum=0.0, weight_decay=0.0)
+    if scale == 1.0:
+        assert torch.equal(p, -orthogonalize(g))
+    else:  # lr s is 1 but for its roundings
+        assert float((p + orthogonalize(g)).abs().max()) <= 4 * 2.0 ** -24 * float(p.abs().max())
