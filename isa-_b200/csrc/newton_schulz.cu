@@ -12,10 +12,10 @@
 //   B = X X^T + (b / 2c) I,   P = c B B + (a - b^2 / 4c) I,   X <- P X
 //
 // all three are one product each with an epilogue alpha D + beta I, so none of
-// them reads anything but its operands.  For fp32 results of small matrices P is formed as it
+// them reads anything but its operands.  For fp32 results of fewer than 224 rows P is formed as it
 // stands, b A read by the second product's epilogue: the square's completion rounds A at
-// the size of b / 2c (42 x 47: 1.6e-6 off, where products in fp32 are by 0.95e-6, and
-// 0.97e-6 as it stands).  (c = 0: P = b X X^T + a I is the first product's, and the second falls away.)
+// the size of b / 2c (42 x 47: 1.7e-6 off, where products in fp32 are by 1.0e-6, and
+// 1.0e-6 as it stands).  (c = 0: P = b X X^T + a I is the first product's, and the second falls away.)
 //
 // Precision.  A singular value far below the largest grows by up to a per step
 // (x 485 in five steps), and so does any rounding noise in its direction: with
@@ -25,8 +25,8 @@
 // checked on the host from the coefficients, so the fixed scale neither overflows
 // nor loses small elements), and a
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
-// tensor core products.  fp32 results are off by 0.6 to 1.3 times what products in
-// fp32 give (4096 x 4096 to 192 x 192).
+// tensor core products.  fp32 results are off by 0.35 to 1.2 times what products in
+// fp32 give (4096 x 4096 Gaussian to a few dominant directions in 42 x 47).
 //
 // B and P are symmetric: only tiles on and below the diagonal are computed, the
 // epilogue stores each tile and its mirror image.
@@ -1456,11 +1456,12 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     // Sums as fine as an fp32 result or parameter shows (parameters of 0.02 N after a step of 0.02, 48 of 768 x 768: 0.9e-7
     // off, as with products in fp32; with the coarse sums 1.7e-7); a 16-bit one's own rounding, 1e-3, hides the difference.
     const bool fine = result.dst.type == CIMEKV_F32;
-    // Short sums leave products in fp32 so exact that the completed square's rounding shows:
-    // 64 x 128 is off by 1.72e-6 with it, 1.05e-6 without, fp32 products by 1.05e-6; from
-    // 192 rows on it costs more than it gives (192 x 192: 2.0e-6, 1.3e-6 and 1.65e-6, in 67
-    // and 74 us; 48 of 768 x 768: 2.3e-6, 1.5e-6 and 2.45e-6, in 1,442 and 1,643 us).
-    const bool plain = fine && squared && lay.m <= 160;
+    // Short sums are so exact that the completed square's rounding shows: on decaying spectra it leaves small matrices
+    // further off than products in fp32 are, large ones (whose fp32 sums are long) not.  Off by, against fp32
+    // products, completed and as it stands: 96 rows 1.33 and 0.87, 160 1.28 and 0.80, 192 1.13 and 0.70, 224 0.97
+    // and 0.69, 256 1.00 and 0.67, 384 0.98 and 0.59, 768 0.74 and 0.49.  As it stands costs 192 x 192 74 us instead
+    // of 68, 224 x 224 85 instead of 80, 48 of 768 x 768 a quarter: taken below the crossing.
+    const bool plain = fine && squared && lay.m < 224;
     Steps st = {};
     Product &gram = st.product[0], &square = st.product[1], &apply = st.product[2];
     st.steps = steps;

@@ -14,7 +14,7 @@ Threshold voltages are device parameters and stay with AdamW.
 
 Matrices are fp32, bf16 or fp16; momenta are fp32.  Products run on the tensor
 cores with operands of 22 bits and fp32 sums, so results are about as close
-to the exact iteration as with fp32 products (fp32 results 0.6 to 1.3 times their error).  Results are the same bits every time.
+to the exact iteration as with fp32 products (fp32 results 0.35 to 1.2 times their error).  Results are the same bits every time.
 """
 
 from __future__ import annotations

@@ -358,3 +358,28 @@ def test_fp32_parameters_get_the_precision_of_fp32_results(muons, shape):
         assert torch.equal(p, -orthogonalize(g))
     else:  # lr s is 1 but for its roundings
         assert float((p + orthogonalize(g)).abs().max()) <= 4 * 2.0 ** -24 * float(p.abs().max())
+
+
+def _products_in_fp32(g):
+    """Five steps on g[..., rows, cols] in the type of g, by its own products."""
+    tall = g.shape[-2] > g.shape[-1]
+    x = g.mT if tall else g
+    x = x / x.double().norm(dim=(-2, -1), keepdim=True).to(x.dtype)
+    for _ in range(5):
+        a = x @ x.mT
+        x = 3.4445 * x + (-4.7750 * a + 2.0315 * (a @ a)) @ x
+    return x.mT if tall else x
+
+
+@gpu
+@pytest.mark.parametrize("rows,cols", [(96, 96), (161, 161), (176, 176), (192, 192), (222, 200), (223, 223)])
+def test_fp32_results_below_the_crossing_are_no_further_off_than_fp32_products(muons, rows, cols):
+    """Decaying spectra, whose small directions show what rounds: the completed square leaves these sizes 1.13 to 1.33 times
+    as far off as products in fp32, the polynomial as it stands 0.70 to 0.87 times."""
+    from tests.test_muon import _update
+    orthogonalize, _ = muons
+    assert not torch.backends.cuda.matmul.allow_tf32
+    g = _update("cuda", 6, rows, cols, seed=11)
+    want = _products_in_fp32(g.double())
+    off = lambda t: float((t.double() - want).norm())  # noqa: E731
+    assert off(orthogonalize(g)) <= off(_products_in_fp32(g))
