@@ -65,7 +65,9 @@ class ModelConfig:
     voltage_max: float = 4.0
     affine_scope: str = "final"
     output_chunk_size: int = 16
-    fused_norm: bool = False  # layer norms and residual sums on this package's kernels (no counterpart there)
+    # layer norms and residual sums on this package's kernels (no counterpart there).  A block then hands on its stream and
+    # its FFN output as a pair, whose sum the next norm takes, and a norm with a branch (result, sum): hooks see these.
+    fused_norm: bool = False
 
     @classmethod
     def from_preset(cls, size: str, model_type: str, **kwargs) -> "ModelConfig":
@@ -152,7 +154,11 @@ class GPT2Block(nn.Module):
         y = F.scaled_dot_product_attention(q, k, v, dropout_p=p, is_causal=True)
         return F.linear(y.transpose(1, 2).reshape(b, t, d), self.attn.out_proj.weight, self.attn.out_proj.bias)
 
-    def forward(self, x: torch.Tensor, need_intermediate: bool = False):
+    def forward(self, x: torch.Tensor, need_intermediate: bool = False, delta: Optional[torch.Tensor] = None,
+                carry: bool = False):
+        """``carry`` (blocks with ``fused_norm``): the pair of :meth:`forward_fused` instead of the stream."""
+        if carry:
+            return self.forward_fused(x, delta)
         x = x + self.attention(x)
         ffn_out = self.ffn(self.ln2(x))
         out = x + ffn_out
@@ -206,7 +212,7 @@ class GPT2Model(nn.Module):
         if self.cfg.fused_norm and not need_intermediate:
             delta = None
             for blk in self.blocks:
-                x, delta = blk.forward_fused(x, delta)
+                x, delta = blk(x, False, delta, True)
             dtype = _projection_dtype(x)
             normed = self.ln_f(x, dtype) if delta is None else self.ln_f.add(x, delta, dtype)[0]
             return self.lm_head(normed)

@@ -2,7 +2,7 @@
 
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import Optional, Tuple, Union
 
 import torch
 import torch.nn as nn
@@ -36,14 +36,18 @@ class LayerNorm(nn.LayerNorm):
         if x.dim() < 1 or x.shape[-1] != self.normalized_shape[0]:
             raise RuntimeError(f"expected {self.normalized_shape[0]} features in the last axis, got shape {tuple(x.shape)}")
 
-    def forward(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None) -> torch.Tensor:
+    def forward(self, x: torch.Tensor, out_dtype: Optional[torch.dtype] = None,
+                delta: Optional[torch.Tensor] = None) -> Union[torch.Tensor, Tuple[torch.Tensor, torch.Tensor]]:
+        """``norm(x)``, or with a branch ``delta`` what :meth:`add` returns."""
         self._check(x)
-        return cuda_layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
-
-    def add(self, x: torch.Tensor, delta: torch.Tensor,
-            out_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
-        """``(norm(x + delta), x + delta)`` in one pass: the residual sum in front of the norm."""
-        self._check(x)
+        if delta is None:
+            return cuda_layer_norm(x, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
         if delta.dtype != x.dtype and x.dtype != torch.float32:  # as torch's sum: the wider type holds it
             x = x.to(torch.promote_types(x.dtype, delta.dtype))
         return cuda_add_layer_norm(x, delta, self.weight, self.bias, self.eps, self._dtype(x, out_dtype))
+
+    def add(self, x: torch.Tensor, delta: torch.Tensor,
+            out_dtype: Optional[torch.dtype] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+        """``(norm(x + delta), x + delta)`` in one pass: the residual sum in front of the norm.  A call of the module,
+        hooks included."""
+        return self(x, out_dtype, delta)

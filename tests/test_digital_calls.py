@@ -383,3 +383,52 @@ def test_fp32_results_below_the_crossing_are_no_further_off_than_fp32_products(m
     want = _products_in_fp32(g.double())
     off = lambda t: float((t.double() - want).norm())  # noqa: E731
     assert off(orthogonalize(g)) <= off(_products_in_fp32(g))
+
+
+# -------------------------------------------------------------------- in the models --
+
+@gpu
+@pytest.mark.parametrize("fused", [False, True])
+def test_hooks_and_wrappers_of_blocks_and_norms_run(fused):
+    """Hooks on every module, and a block's forward replaced by a checkpointed one, with and without fused norms."""
+    import torch.nn as nn
+    from torch.utils.checkpoint import checkpoint
+    from isa_b200.language import GPT2Model, ModelConfig
+    torch.manual_seed(0)
+    cfg = ModelConfig.from_preset("tiny", "standard", vocab_size=61, max_seq_len=24, fused_norm=fused)
+    cfg.depth = 2
+    model = GPT2Model(cfg).cuda()
+    ids = torch.randint(0, 61, (2, 24), device="cuda")
+    plain = model(ids)
+    want = torch.autograd.grad(plain.square().mean(), list(model.parameters()))
+    seen = {"pre": set(), "out": set(), "back": set()}
+    names = [f"blocks.{i}{k}" for i in range(2) for k in ("", ".ln1", ".ln2")] + ["ln_f"]
+    for name in names:
+        module = model.get_submodule(name)
+        module.register_forward_pre_hook(lambda m, args, name=name: seen["pre"].add(name))
+        module.register_forward_hook(lambda m, args, out, name=name: seen["out"].add(name))
+        module.register_full_backward_hook(lambda m, gi, go, name=name: seen["back"].add(name))
+    entered = []
+    for i, blk in enumerate(model.blocks):
+        def wrapped(*args, own=blk.forward, i=i):
+            entered.append(i)
+            return checkpoint(own, *args, use_reentrant=False)
+        blk.forward = wrapped
+    logits = model(ids)
+    assert torch.equal(logits, plain) and entered == [0, 1]
+    got = torch.autograd.grad(logits.square().mean(), list(model.parameters()))
+    for a, b in zip(got, want):  # the same sums, where torch's own gradients add in any order: 2^-24 of many terms
+        assert float((a - b).norm()) <= 1e-5 * float(b.norm())
+    assert all(seen[k] == set(names) for k in ("pre", "out"))
+    assert seen["back"] >= {f"blocks.{i}" for i in range(2)} | {"ln_f"}
+
+
+@gpu
+def test_hooks_of_the_vit_norms_run():
+    from isa_b200.harness.vit import PhysicalViT, ViTConfig
+    model = PhysicalViT(ViTConfig(img_size=16, patch_size=8, num_classes=5, embed_dim=48, num_heads=3, depth=1, fused_norm=True)).cuda()
+    seen = []
+    for name in ("blocks.0.norm1", "blocks.0.norm2", "norm"):
+        model.get_submodule(name).register_forward_hook(lambda m, args, out, name=name: seen.append(name))
+    model(torch.randn(2, 3, 16, 16, device="cuda"))
+    assert seen == ["blocks.0.norm1", "blocks.0.norm2", "norm"]
