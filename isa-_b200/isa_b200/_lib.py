@@ -17,6 +17,8 @@ from pathlib import Path
 
 import torch
 
+from isa_b200.build import binding_path
+
 _LIB_PATH = Path(os.environ.get("CIMEKV_LIB", Path(__file__).resolve().parent / "_lib" / "libcimekv.so"))
 
 _c_int, _c_float, _c_size, _vp = ctypes.c_int, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
@@ -76,8 +78,6 @@ SIGNATURES = {
     "cimekv_fp32_probe": (_c_int, [_vp, _c_int, _c_int, ctypes.POINTER(ctypes.c_longlong), _vp]),
 }
 
-_BINDING_PATH = Path(__file__).resolve().parent / "_lib" / "cimekv_torch.so"
-
 _lock = threading.Lock()
 _lib = None
 _binding = None
@@ -110,12 +110,13 @@ def binding():
         lib = load()
         with _lock:
             if _binding is None:
-                if not _BINDING_PATH.exists():
+                path = binding_path()
+                if not path.exists():
                     raise RuntimeError(
-                        f"cimekv_torch.so not found at {_BINDING_PATH}; build it with `python -m isa_b200.build` "
+                        f"no tensor binding for this torch and Python at {path}; build it with `python -m isa_b200.build` "
                         "(the layer norm and Newton-Schulz operators have no other implementation)"
                     )
-                spec = importlib.util.spec_from_file_location("cimekv_torch", _BINDING_PATH)
+                spec = importlib.util.spec_from_file_location("cimekv_torch", path)
                 module = importlib.util.module_from_spec(spec)
                 spec.loader.exec_module(module)
                 module.bind({name: ctypes.cast(getattr(lib, name), ctypes.c_void_p).value for name in SIGNATURES})

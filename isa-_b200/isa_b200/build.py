@@ -1,14 +1,17 @@
 """Build the sm_100a C-ABI library ``libcimekv.so`` and its C++ tensor binding
-``cimekv_torch.so`` in-tree.
+``cimekv_torch.<torch version>.<python>.so`` in-tree.
 
-    python -m isa_b200.build        (or isa_b200.build.build_library())
+    python -m isa_b200.build                  (or isa_b200.build.build_library())
+    python -m isa_b200.build --library-only   the C ABI alone, which needs nvcc and nothing else
 
 nvcc cross-compiles for sm_100a without a GPU.  Both land next to this file in
-``_lib/`` so they travel with the source tree.
+``_lib/`` so they travel with the source tree.  The binding's name says which torch
+and Python it is for: another one finds none and builds its own.
 """
 
 from __future__ import annotations
 
+import importlib.util
 import os
 import shutil
 import subprocess
@@ -22,7 +25,6 @@ REPO_ROOT = PKG_DIR.parent.parent
 INCLUDE_DIR = REPO_ROOT / "include"
 LIB_DIR = PKG_DIR / "_lib"
 LIB_PATH = LIB_DIR / "libcimekv.so"
-BINDING_PATH = LIB_DIR / "cimekv_torch.so"
 DEBUG_LIB_PATH = LIB_DIR / "libcimekv_debug.so"  # table-index bounds checks (CIMEKV_DEBUG_BOUNDS=1)
 
 NVCC_FLAGS = [
@@ -43,12 +45,30 @@ def sources() -> list[Path]:
     return sorted(SRC_DIR.glob("*.cu"))
 
 
-def build_library(force: bool = False, verbose: bool = False, debug: bool = False) -> Path:
+def binding_path() -> Path:
+    """Where the tensor binding for this torch and this Python is."""
+    import torch
+
+    return LIB_DIR / f"cimekv_torch.{torch.__version__}.{sys.implementation.cache_tag}.so"
+
+
+def build_library(force: bool = False, verbose: bool = False, debug: bool = False, binding: bool = True) -> Path:
     """Compile csrc/*.cu into _lib/libcimekv.so (or the bounds-checking
-    libcimekv_debug.so with debug=True); skipped when up to date.  The release
-    build brings the tensor binding with it."""
-    if not debug:
-        build_binding(force)
+    libcimekv_debug.so with debug=True); skipped when up to date.  After the release
+    library comes the tensor binding, unless ``binding`` is False or there is no torch or
+    no C++ compiler to build it with (its operators then say that it is missing)."""
+    out = _compile_library(force, verbose, debug)
+    if binding and not debug:
+        missing = [what for what, there in (("torch", importlib.util.find_spec("torch")), ("g++", shutil.which("g++")))
+                   if not there]
+        if missing:
+            print(f"{' and '.join(missing)} not found: the library is built, its tensor binding is not", file=sys.stderr)
+        else:
+            build_binding(force)
+    return out
+
+
+def _compile_library(force: bool, verbose: bool, debug: bool) -> Path:
     srcs = sources()
     deps = srcs + sorted(INCLUDE_DIR.glob("*.h")) + sorted(SRC_DIR.glob("*.cuh"))
     out = DEBUG_LIB_PATH if debug else LIB_PATH
@@ -70,8 +90,8 @@ def build_library(force: bool = False, verbose: bool = False, debug: bool = Fals
 
 
 def build_binding(force: bool = False) -> Path:
-    """Compile csrc/torch_binding.cpp into _lib/cimekv_torch.so; skipped when up to date."""
-    src, out = SRC_DIR / "torch_binding.cpp", BINDING_PATH
+    """Compile csrc/torch_binding.cpp into binding_path(); skipped when up to date."""
+    src, out = SRC_DIR / "torch_binding.cpp", binding_path()
     deps = [src, *INCLUDE_DIR.glob("*.h")]
     if not force and out.exists() and all(p.stat().st_mtime <= out.stat().st_mtime for p in deps):
         return out
@@ -95,4 +115,5 @@ def build_binding(force: bool = False) -> Path:
 
 
 if __name__ == "__main__":
-    print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv, debug="--debug" in sys.argv))
+    print(build_library(force="--force" in sys.argv, verbose="-v" in sys.argv, debug="--debug" in sys.argv,
+                        binding="--library-only" not in sys.argv))

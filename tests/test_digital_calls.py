@@ -432,3 +432,34 @@ def test_hooks_of_the_vit_norms_run():
         model.get_submodule(name).register_forward_hook(lambda m, args, out, name=name: seen.append(name))
     model(torch.randn(2, 3, 16, 16, device="cuda"))
     assert seen == ["blocks.0.norm1", "blocks.0.norm2", "norm"]
+
+
+# --------------------------------------------------------------------------- building --
+
+def test_the_library_needs_nvcc_alone(monkeypatch, tmp_path, capsys):
+    """Without torch, without g++ or unasked for the binding is left out and the library built all the same; the binding
+    of another torch is not taken for this one's."""
+    from isa_b200 import _lib, build
+    here = build.binding_path()
+    assert here.exists() and torch.__version__ in here.name
+    calls = []
+    monkeypatch.setattr(build, "build_binding", lambda force=False: calls.append(force))
+    build.build_library(binding=False)
+    build.build_library(debug=True)
+    assert not calls
+    build.build_library()
+    assert len(calls) == 1
+    with monkeypatch.context() as m:
+        m.setattr(build.shutil, "which", lambda name: None if name == "g++" else "/usr/bin/" + name)
+        assert build.build_library() == build.LIB_PATH
+        assert "g++ not found" in capsys.readouterr().err
+        m.setattr(build.importlib.util, "find_spec", lambda name: None)
+        assert build.build_library() == build.LIB_PATH
+        assert "torch and g++ not found" in capsys.readouterr().err
+    assert len(calls) == 1
+    with monkeypatch.context() as m:
+        m.setattr(torch, "__version__", "1.0.0+none")
+        m.setattr(_lib, "_binding", None)
+        assert build.binding_path() != here
+        with pytest.raises(RuntimeError, match="no tensor binding for this torch"):
+            _lib.binding()
