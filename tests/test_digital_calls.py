@@ -463,3 +463,38 @@ def test_the_library_needs_nvcc_alone(monkeypatch, tmp_path, capsys):
         assert build.binding_path() != here
         with pytest.raises(RuntimeError, match="no tensor binding for this torch"):
             _lib.binding()
+
+
+# ---------------------------------------------------------------------------- layouts --
+
+@gpu
+@pytest.mark.parametrize("dtype", [BF16, F16])
+@pytest.mark.parametrize("rows,cols", [(700, 100), (300, 256), (90, 1000), (41, 4000), (11, 16000), (9, 16384)])
+def test_16_bit_rows_that_no_vector_fits(norms, rows, cols, dtype):
+    """Rows from any element of a buffer, any distance apart, in input, branch and both gradients; the row before and behind
+    them is full of NaN."""
+    from tests.test_layer_norm import _assert_near, _plain
+    layer_norm, add_layer_norm = norms
+    gen = torch.Generator(device="cuda").manual_seed(rows + cols)
+
+    def rows_at(offset, apart):
+        buf = torch.full((rows + 2, cols + apart), float("nan"), device="cuda", dtype=dtype).view(-1)
+        t = buf[cols + apart + offset:][:rows * (cols + apart)].view(rows, cols + apart)[:, :cols]
+        t.copy_(torch.randn(rows, cols, device="cuda", generator=gen))
+        return t
+
+    w = (1 + 0.3 * torch.randn(cols, device="cuda", generator=gen)).to(dtype).requires_grad_(True)
+    b = (0.2 * torch.randn(cols, device="cuda", generator=gen)).to(dtype).requires_grad_(True)
+    for places in ([(1, 1)] * 4, [(0, 1), (1, 3), (2, 5), (3, 0)], [(3, 0), (5, 0), (7, 0), (1, 0)], [(4, 4), (0, 8), (4, 12), (0, 4)]):
+        x, d, dy, dh = (rows_at(*at) for at in places)
+        x, d = x.requires_grad_(True), d.requires_grad_(True)
+        want = _plain(x.detach(), d.detach(), w.detach(), b.detach(), 1e-5, dy, dh)
+        y, h = add_layer_norm(x, d, w, b)
+        assert torch.equal(h.double(), want["h"][0])
+        got = torch.autograd.grad((y, h), (x, d, w, b), (dy, dh))
+        for t, k in zip((y, *got), ("y", "dx", "dx", "dw", "db")):
+            _assert_near(t.detach(), *want[k], f"{k} {places}")
+        want = _plain(x.detach(), None, w.detach(), None, 1e-5, dy, None)
+        y = layer_norm(x, w)
+        for t, k in zip((y, *torch.autograd.grad(y, (x, w), dy)), ("y", "dx", "dw")):
+            _assert_near(t.detach(), *want[k], f"{k} alone {places}")
