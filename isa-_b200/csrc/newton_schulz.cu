@@ -1453,9 +1453,15 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
 
     // sums of products of two planes are 2^24 times the value, planes 2^12 times
     const bool squared = c != 0.0f;
-    // Sums as fine as an fp32 result or parameter shows (parameters of 0.02 N after a step of 0.02, 48 of 768 x 768: 0.9e-7
-    // off, as with products in fp32; with the coarse sums 1.7e-7); a 16-bit one's own rounding, 1e-3, hides the difference.
-    const bool fine = result.dst.type == CIMEKV_F32;
+    const StepCost cost = step_cost(batch, lay.m, lay.n, squared, sms);
+    const bool together = share || cost.together <= cost.each;  // all steps in one kernel
+    // Fine sums where the result shows them: a 16-bit result's own rounding, 1e-3, hides the difference.  An fp32
+    // parameter of 0.02 N after a step of 0.02 is off by 1.7e-7 with the coarse ones and by 0.9e-7 with the fine, as with
+    // products in fp32 (48 of 768 x 768, where the products are kernels and the power limit hides the cost: 1,730 and 1,700
+    // us).  In the one kernel of small matrices latency is all there is, and parameters take the coarse sums: 40 of 192 x 192
+    // are off by 1.8e-7 in 125 us, by 1.2e-7 in 146 with fine sums (products in fp32 1.1e-7); with 10 of 192 x 768
+    // beside them 180 and, with the polynomial as it stands too, 255 us.
+    const bool fine = result.dst.type == CIMEKV_F32 && !(result.update && together);
     // Short sums are so exact that the completed square's rounding shows: on decaying spectra it leaves small matrices
     // further off than products in fp32 are, large ones (whose fp32 sums are long) not.  Off by, against fp32
     // products, completed and as it stands: 96 rows 1.33 and 0.87, 160 1.28 and 0.80, 192 1.13 and 0.70, 224 0.97
@@ -1487,8 +1493,7 @@ int run(PrepParams& prep, Result& result, int batch, int rows, int cols, int ste
     result.transposed = prep.transposed;
     result.vec = lay.n % 8 == 0 && aligned(result.dst, batch, 16);
 
-    const StepCost cost = step_cost(batch, lay.m, lay.n, squared, sms);
-    if (share || cost.together <= cost.each) {
+    if (together) {
         const int group = cost.group;
         StepMaps maps;
         using T = Tile<64, true>;  // sizes are those of the fast one too
