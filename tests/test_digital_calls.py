@@ -499,3 +499,18 @@ def test_16_bit_rows_that_no_vector_fits(norms, rows, cols, dtype):
         y = layer_norm(x, w)
         for t, k in zip((y, *torch.autograd.grad(y, (x, w), dy)), ("y", "dx", "dw")):
             _assert_near(t.detach(), *want[k], f"{k} alone {places}")
+
+
+@gpu
+def test_matrices_beyond_32_bits(muons):
+    """2.7e9 elements in one call: the last matrices equal those of a call of their own."""
+    orthogonalize, muon_step = muons
+    g = torch.empty(40, 8192, 8192, device="cuda", dtype=BF16).normal_()
+    out = orthogonalize(g, steps=1)
+    assert torch.equal(out[-2:], orthogonalize(g[-2:], steps=1)) and torch.equal(out[:2], orthogonalize(g[:2], steps=1))
+    p = out  # as parameters
+    m = torch.zeros(40, 8192, 8192, device="cuda")
+    small = p[-2:].clone(), m[-2:].clone()
+    muon_step([p], [g], [m], lr=0.1, steps=1)
+    muon_step([small[0]], [g[-2:]], [small[1]], lr=0.1, steps=1)
+    assert torch.equal(p[-2:], small[0]) and torch.equal(m[-2:], small[1])
