@@ -467,7 +467,7 @@ __device__ __forceinline__ void row_sync() {
 
 // Measured (copy bandwidth 6.5 TB/s): 16,384 x 4,096 bf16 with a branch in 92 us, 5.9
 // TB/s; 32,736 x 768 fp32 with a bf16 branch in 55 us, 5.5 TB/s; 4,099 x 1,537 bf16 with a
-// branch (inside L2) in 18 us, where the instructions count: 59 % of the issue slots at
+// branch (inside L2) in 18 us, where the instructions count: 69 % of the issue slots at
 // 50,432 x 384 fp16 (22 us), two or three warps of a scheduler waiting for a row's sums.
 template <int V, int E, int W, bool kDelta>
 __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) norm_fwd_kernel(NormParams p) {
@@ -545,8 +545,8 @@ __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, true)) n
 // kSum: the sum's own gradient dh is added to dx.  p.part: the CTA's column sums
 // [gridDim][2][cols] (dw, db), or null when no weight gradient is wanted.
 // Measured: 16,384 x 4,096 bf16 with dh in 105 us, 5.1 TB/s; 32,736 x 768 fp32, bf16
-// branch, in 78 us, 5.2 TB/s; 50,432 x 384 fp16, fp32 dy, in 40 us, 3.9 TB/s: rows this
-// short pay for their two sums (49 % of the issue slots, the rest is their latency).
+// branch, in 74 to 78 us, 5.2 TB/s and more; 50,432 x 384 fp16, fp32 dy, in 40 us, 3.9 TB/s: rows this
+// short pay for their two sums (48 % of the issue slots, the rest is their latency).
 template <int V, int E, int W, bool kSum>
 __global__ void __launch_bounds__(cta_threads(W), ctas_per_sm(V * E, W, false)) norm_bwd_kernel(NormParams p) {
     constexpr int T = W * 32, kStep = T * V, N = kSum ? 3 : 2;
@@ -677,7 +677,17 @@ struct Shape {
 
 // Layouts of a row by width, for vectors of 4 (fp32 rows), of 8 (16-bit rows) and
 // single elements (strides or addresses that no vector fits): the first that
-// holds the row is taken.
+// holds the row is taken.  Measured over 64 Mi elements, forward and backward in TB/s:
+//                fp32         bf16         bf16 by single elements
+//      384    5.7   6.0    3.8   4.2    1.1   1.2
+//    1,024    5.9   5.2    4.5   3.3    2.7   3.1
+//    1,280    5.1   4.2    2.9   2.4    1.1   1.3    (a quarter and more of the threads idle between layouts)
+//    1,536    6.0   4.4    3.4   2.8    1.2   1.5
+//    4,096    5.8   5.8    4.2   4.5    2.7   3.6
+//    5,120    4.3   5.1    1.3   1.5    1.1   0.8    (16-bit: four CTAs take a second turn, see grid_size)
+//    8,192    5.7   6.2    2.0   2.3    1.6   1.1
+//   16,384    5.8   3.4    2.0   1.3    2.4   1.8    (32 elements a thread)
+// The backward has 128 registers a thread: with 16 elements in it it spills up to 140 bytes, with 32 about 1 KB.
 constexpr Shape kShapes[] = {{4, 1, 1}, {4, 2, 1}, {4, 3, 1}, {4, 4, 1}, {4, 3, 2}, {4, 4, 2}, {4, 4, 4}, {4, 4, 8},
                              {4, 4, 16}, {4, 8, 16},
                              {8, 1, 1}, {8, 2, 1}, {8, 2, 2}, {8, 2, 4}, {8, 2, 8}, {8, 2, 16}, {8, 4, 16},
@@ -726,7 +736,8 @@ int sm_count(int* sms) {
 }
 
 // CTAs of a launch: what is resident at once; a multiple of V, so that a group's rows
-// all begin at the same place of a vector.
+// all begin at the same place of a vector.  (One CTA an SM and V = 8 make it 152 for 148 places, which
+// costs the widest 16-bit rows a second turn.)
 long long grid_size(long long rows, const Shape& s, int sms, bool forward) {
     const long long need = (rows + cta_rows(s.w) - 1) / cta_rows(s.w);
     const long long most = (long long)sms * ctas_per_sm(s.v * s.e, s.w, forward);

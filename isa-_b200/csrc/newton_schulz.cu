@@ -21,9 +21,10 @@
 // (x 485 in five steps), and so does any rounding noise in its direction: with
 // operands rounded to 11 bits the result of a low-rank update is off by 1e-2, more
 // than the half step of a bf16 result.  X, B and P are therefore held as pairs of
-// fp16 planes, value * 2^12 = hi + lo (22 bits; singular values stay below 15,
-// checked on the host from the coefficients, so the fixed scale neither overflows
-// nor loses small elements), and a
+// fp16 planes, value * 2^12 = hi + lo.  Singular values stay below 15, checked on the host
+// from the coefficients, so the fixed scale does not overflow.  Values from 2^-14 on keep 22 bits; below,
+// where lo is subnormal, an element is off by up to 2^-37.  In norm that is 2^-37 sqrt(elements),
+// 2^-23 of |X| = 1 for 16,384 x 16,384, no more than what 22 bits round off, and later steps only grow |X|.  A
 // product is hi hi + hi lo + lo hi, accumulated in fp32 in tensor memory: three
 // tensor core products.  fp32 results are off by 0.35 to 1.2 times what products in
 // fp32 give (4096 x 4096 Gaussian to a few dominant directions in 42 x 47).
@@ -318,8 +319,8 @@ __device__ __forceinline__ void load4(const void* p, int type, long long i, floa
 // Momentum update and the partial sums of squares of one matrix, p.parts CTAs
 // to a matrix, in doubles (squares of fp32 values neither overflow nor vanish),
 // added in a fixed order.  kFlat: a matrix is one run of elements that vectors of
-// four fit; otherwise row by row.  Bound by HBM: 49 us for a Muon step's 48 of 768 x 768
-// (340 MB in fp32), 22 us for 4,096 x 4,096 bf16, whose 33 MB are latency.
+// four fit; otherwise row by row.  Bound by HBM: 52 us for a Muon step's 48 of 768 x 768
+// (340 MB in fp32, 6.5 TB/s), 22 to 27 us for 4,096 x 4,096 bf16, whose 33 MB are latency.
 template <bool kFlat>
 __global__ void __launch_bounds__(256) ns_norm_kernel(const __grid_constant__ PrepParams p) {
     const int b = blockIdx.y;
@@ -418,7 +419,7 @@ __device__ __forceinline__ float plane_factor(const PrepParams& p, int b, float*
 }
 
 // X0 as pairs of planes: a thread's eight neighbours of one row (8 x 256 tiles).
-// kVec: rows of G and of the momenta can be read in vectors of four.  Bound by HBM: 56 us
+// kVec: rows of G and of the momenta can be read in vectors of four.  Bound by HBM: 56 to 63 us
 // for 48 of 768 x 768 with momenta (340 MB).
 template <bool kVec>
 __global__ void __launch_bounds__(256) ns_prepare_kernel(const __grid_constant__ PrepParams p) {
@@ -808,10 +809,10 @@ __device__ __forceinline__ void meet_wait(const Meet& m) {
 // the errors that are measured), so errors grow with what is already summed and all
 // have one sign.  So a few steps (the small cross products before those at full size) go
 // into a fresh accumulator, one of several, and the collecting warps add them in
-// registers with round-to-nearest while the next ones run.  Fine sums: 192 x 192 is off
-// by 2.0e-6 where fp32 products are by 1.6e-6 (fast: 2.8e-6; both with the square
-// completed), 48 of 768 x 768 by 2.3e-6 (fp32 products 2.5e-6, fast 4.6e-6), in 1,442 us
-// (fast 1,385), 40 of 192 x 192 in 137 (fast 123).  The same accumulators let the next tile start while the last one is stored.
+// registers with round-to-nearest while the next ones run.  With the square completed 192 x 192 is off
+// by 1.8e-6 with fine sums (products in fp32 1.6e-6, coarse sums 2.8e-6), 48 of 768 x 768 by 2.6e-6 (2.4e-6,
+// 4.6e-6).  Fine sums take 40 of 192 x 192 146 us instead of 125 in the one kernel (a Muon step each); where the products
+// are kernels the power limit hides them.  The same accumulators let the next tile start while the last one is stored.
 template <int M, int kSide, bool kFine>
 __device__ __forceinline__ void product(Pipe& q, const CUtensorMap* left, const CUtensorMap* right,
                                         const CUtensorMap* out, const Product& p, const Result& result, int batch, int first, int step, int tiles,
@@ -1079,11 +1080,11 @@ __device__ __forceinline__ void pipe_close(Pipe& q, unsigned* word) {
 }
 
 // One product of all matrices, a persistent loop over its tiles.  Counting the three
-// tensor core products: 4,096 x 4,096 in 281 to 299 us (P X) and 150 us (X X^T), 1,450
-// TFLOP/s until the power limit takes the clock (1,330 to 1,400 in a loop of calls; a
-// library's 16-bit product sustains 1,380); 48 of 768 x 768 in 97 us, 1,340 TFLOP/s, and 78 us, 1,110
-// TFLOP/s: twelve stages a tile leave the intake of a tile's ends uncovered.  The last
-// product, with the parameters' update, takes 156 us there: it reads and writes 226 MB.
+// tensor core products, on a GPU that was idle before: 4,096 x 4,096 in 281 to 299 us (P X) and 150 us (X X^T), 1,450
+// TFLOP/s; 48 of 768 x 768 X X^T in 73 us at 1.8 GHz, 63 % of the tensor pipe: twelve stages a tile leave the intake
+// of a tile's ends uncovered.  In a loop of calls the power limit takes the clock, and these are 105 (X X^T), 127
+// (P X) and 200 us (the last product with the parameters' update, which reads and writes 226 MB).  The
+// pair's kernels spill 28 to 140 bytes a thread outside the loop over the sums.
 template <int M, int kSide, bool kFine>
 __global__ void __launch_bounds__(Tile<kSide, kFine>::kThreads, 1) ns_gemm_kernel(const __grid_constant__ CUtensorMap left,
                                                                            const __grid_constant__ CUtensorMap right,
@@ -1120,8 +1121,9 @@ struct StepMaps {
 
 // All steps of matrices whose tiles fit the SMs, a group of CTAs to a matrix that meet
 // after each product.  Bound by latency: a product of one 192 x 192 matrix is 63 us / 15 =
-// 4.2 us, of which the meeting is about 1 us, the first copy 0.4, a stage 0.45 each (three),
-// the way out 0.75; 40 of 192 x 192 take 115 us, 10 of 192 x 768 take 102, 2 of 257 x 1001 112.
+// 4.2 us (bf16; fp32 72 / 15 = 4.8), of which the meeting is about 1 us, the first copy 0.4, a stage 0.45 each (three),
+// the way out 0.75.  This kernel alone, 16-bit results or a step's parameters / fp32 results: 40 of 192 x 192 in 110 / 142 us,
+// 10 of 192 x 768 in 102 / 114, 2 of 257 x 1001 in 110.
 template <bool kFine>
 __global__ void __launch_bounds__(Tile<64, kFine>::kThreads, 1) ns_steps_kernel(const __grid_constant__ StepMaps maps,
                                                                          const __grid_constant__ Steps st,
@@ -1373,9 +1375,10 @@ int launch_gemm(const CUtensorMap& l, const CUtensorMap& r, const CUtensorMap& o
 }
 
 // What a step takes when all steps run in one kernel and when each product is a kernel;
-// the cheaper way is taken.  Measured a call, one kernel against fifteen: 73 against 112 us
-// for one 192 x 192 matrix, 131 against 202 for 768 x 768, 120 against 135 for 40 of
-// 192 x 192; 252 against 239 for 1024 x 1024, 176 against 159 for 12 of 384 x 384.
+// the cheaper way is taken.  Measured a call of five steps, one kernel against fifteen, 16-bit results (fp32): 72 against
+// 114 us for one 192 x 192 matrix (80 against 129), 127 against 215 for 768 x 768 (137, 220), 119 against 136 for 40 of
+// 192 x 192 (151, 151); 246 against 257 for 1024 x 1024 (278, 263), 168 against 163 for 12 of 384 x 384 (195, 168),
+// 401 against 310 for 1100 x 1300 (458, 313).  Off by most at 900 x 900 bf16, where it takes 277 us for 239.
 struct StepCost {
     int group;              // CTAs of a matrix in the one kernel
     double together, each;  // cycles of a step: one kernel, a kernel for each product

@@ -8,7 +8,8 @@
 
 Inputs are fp32, bf16 or fp16 with rows of contiguous elements (any row stride;
 other layouts are copied).  Statistics and sums are fp32, results are rounded
-once.  ``out_dtype`` is the type of ``y``: fp32 streams may hand out any of the
+once; a row whose sum or sum of squared deviations passes fp32 (means beyond 1e34,
+deviations beyond 1e17 at the widest) overflows.  ``out_dtype`` is the type of ``y``: fp32 streams may hand out any of the
 three, 16-bit streams their own type or fp32.  The backward is one pass over the
 rows and a fixed-order reduction for the weight gradients, so it gives the same
 bits every time; it cannot be differentiated again.  There is no forward-mode
