@@ -790,7 +790,7 @@ int layout_of(int x_type, int cols, std::initializer_list<Tensor> ts, int* place
 // per device (the attribute stays).
 int allow_smem(const void* kernel, int id, size_t bytes) {
     static std::atomic<uint64_t> done[4 * kNumShapes];
-    if (bytes <= (48 << 10)) return CIMEKV_OK;
+    if (bytes <= (47 << 10)) return CIMEKV_OK;  // 48 KB need no leave, the kernels' own variables (384 bytes) among them
     int dev;
     if (cudaGetDevice(&dev) != cudaSuccess) return fail(CIMEKV_ECUDA, "no current device");
     if (dev < 64 && (done[id].load(std::memory_order_acquire) >> dev & 1)) return CIMEKV_OK;

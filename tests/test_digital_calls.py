@@ -514,3 +514,37 @@ def test_matrices_beyond_32_bits(muons):
     muon_step([p], [g], [m], lr=0.1, steps=1)
     muon_step([small[0]], [g[-2:]], [small[1]], lr=0.1, steps=1)
     assert torch.equal(p[-2:], small[0]) and torch.equal(m[-2:], small[1])
+
+
+@gpu
+@pytest.mark.parametrize("x_t,d_t,y_t", [(F32, F32, F32), (F32, BF16, BF16), (BF16, BF16, F32), (F16, F16, F16)])
+def test_rows_that_just_fill_48_kb(x_t, d_t, y_t):
+    """Widths whose rows take all of the 48 KB of shared memory that a kernel has without asking, but for what its own
+    variables need: in a process of its own, where no wider row has asked before."""
+    import subprocess
+    import sys
+    from pathlib import Path
+    root = Path(__file__).resolve().parent.parent
+    widths = [108, 172, 216, 228, 344, 364, 492, 588, 728, 736, 748, 984, 996, 1204, 1496, 1504, 1516, 2008, 2020, 3032, 3052, 6104]
+    code = f"""
+import sys
+sys.path[:0] = [{str(root / 'isa-_b200')!r}, {str(root)!r}]
+import torch
+from tests.test_layer_norm import _assert_near, _case, _plain, _run_and_check
+from isa_b200.kernels.transformer_norm import cuda_add_layer_norm, cuda_layer_norm
+dev = torch.device("cuda")
+for cols in {widths}:
+    for d_t in (None, {d_t}):
+        _run_and_check(*_case(dev, 9, cols, {x_t}, d_t, {x_t}, {y_t}), {y_t})
+    buf = torch.randn(9 * cols + 1, device=dev).to({x_t})[1:].view(9, cols)  # rows that no vector fits
+    y, h = cuda_add_layer_norm(buf, buf)
+    _assert_near(y, *_plain(buf, buf, None, None, 1e-5, None, None)["y"], "y")
+    _assert_near(cuda_layer_norm(buf), *_plain(buf, None, None, None, 1e-5, None, None)["y"], "y")
+    w = torch.ones(cols, device=dev, requires_grad=True)
+    dy = torch.randn(9 * cols + 1, device=dev)[1:].view(9, cols)
+    gw, = torch.autograd.grad(cuda_layer_norm(buf, w, None, 1e-5, torch.float32), w, dy)
+    _assert_near(gw, *_plain(buf, None, w.detach(), None, 1e-5, dy, None)["dw"], "dw")
+print("all")
+"""
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.split() == ["all"], (r.stdout, r.stderr[-2000:])
