@@ -548,3 +548,43 @@ print("all")
 """
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.split() == ["all"], (r.stdout, r.stderr[-2000:])
+
+
+@gpu
+def test_calls_from_several_threads_at_once(muons):
+    """Kernels whose CTAs wait for one another, from streams of different priority, with others between them: the same bits
+    as alone, and no wait runs out."""
+    import threading
+    from isa_b200 import _lib
+    orthogonalize, muon_step = muons
+    wrong = []
+
+    def run(seed, shapes, priority):
+        stream = torch.cuda.Stream(priority=priority)
+        with torch.cuda.stream(stream):
+            gen = torch.Generator(device="cuda").manual_seed(seed)
+            g = [torch.randn(s, device="cuda", generator=gen) for s in shapes]
+
+            def call():
+                if len(g) == 1:
+                    return [orthogonalize(g[0])]
+                p, m = [torch.zeros_like(t) for t in g], [torch.zeros_like(t) for t in g]
+                muon_step(p, g, m, lr=1.0, weight_decay=0.0)
+                return p
+
+            want = call()
+            stream.synchronize()
+            for _ in range(20):
+                got = [call() for _ in range(10)]
+                stream.synchronize()
+                if not all(torch.equal(a, b) for out in got for a, b in zip(out, want)):
+                    wrong.append((shapes, priority))
+
+    threads = [threading.Thread(target=run, args=args) for args in
+               ((0, [(40, 192, 192)], 0), (1, [(768, 768)], -2), (2, [(30, 192, 192), (8, 192, 768)], -1), (3, [(6, 640, 640)], 0))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    torch.cuda.synchronize()
+    assert not wrong and _lib.load().cimekv_lost_waits(0) == 0
